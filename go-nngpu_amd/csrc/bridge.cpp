@@ -11,6 +11,8 @@
 #include <vector>
 
 #include "common.h"
+#include "logits.h"
+#include "mxfp4.h"
 
 using gn::Buffer;
 using gn::set_error;
@@ -934,6 +936,79 @@ int gn_add_bias_cyclic_f32(float *y, long n, const float *bias, long len, void *
   if (!gn::context(err)) return -1;
   if (n > 0 && (!y || !bias)) return set_error(err, -1, "cyclic bias add: NULL pointer");
   return gn::launch_add_cyclic_f32(y, n, bias, len, gn::resolve_stream(stream), err);
+}
+
+int gn_mxfp4_size(long rows, long cols, size_t *data_bytes, size_t *scale_bytes, CError *err) {
+  if (!data_bytes || !scale_bytes) return set_error(err, -1, "mxfp4 size: NULL output");
+  if (!gn::mxfp4_size(rows, cols, data_bytes, scale_bytes))
+    return set_error(err, -1, "mxfp4 size: invalid size %ld x %ld", rows, cols);
+  return 0;
+}
+
+int gn_mxfp4_quantize(int dtype, const void *x, long rows, long cols, long ldx, void *data, void *scales,
+                      void *stream, CError *err) {
+  if (int rc = gn::check_mxfp4_quantize(dtype, x, rows, cols, ldx, data, scales, err)) return rc;
+  if (!gn::context(err)) return -1;
+  return gn::launch_mxfp4_quantize(dtype, x, rows, cols, ldx, data, scales, gn::resolve_stream(stream), err);
+}
+
+int gn_mxfp4_dequantize(const void *data, const void *scales, long rows, long cols, int dtype, void *out, long ldo,
+                        void *stream, CError *err) {
+  if (int rc = gn::check_mxfp4_dequantize(data, scales, rows, cols, dtype, out, ldo, err)) return rc;
+  if (!gn::context(err)) return -1;
+  return gn::launch_mxfp4_dequantize(data, scales, rows, cols, dtype, out, ldo, gn::resolve_stream(stream), err);
+}
+
+int gn_mxfp4_gemm(int a_dtype, long M, long N, long K, float alpha, const void *A, long lda, const void *a_scales,
+                  const void *B, const void *b_scales, float beta, float *C, long ldc, const float *bias, int act,
+                  float act_alpha, void *stream, CError *err) {
+  const gn::MxGemmDesc d{a_dtype, M, N, K, alpha, beta, A, lda, a_scales, B, b_scales, C, ldc, bias, act, act_alpha};
+  if (int rc = gn::check_mxfp4_gemm(d, err)) return rc;
+  if (!gn::context(err)) return -1;
+  return gn::launch_mxfp4_gemm(d, gn::resolve_stream(stream), err);
+}
+
+size_t gn_logits_workspace(long rows, long cols, int k) { return gn::logits_workspace(rows, cols, k); }
+
+int gn_token_logprobs(int dtype, const void *logits, long rows, long cols, long ld, float temperature,
+                      const int64_t *targets, float *logprob, float *lse, float *entropy, int k, int64_t *top_ids,
+                      float *top_logprobs, void *workspace, size_t workspace_bytes, void *stream, CError *err) {
+  const gn::LogprobsDesc d{{dtype, logits, rows, cols, ld, temperature}, targets, logprob, lse, entropy, k, top_ids,
+                           top_logprobs, workspace, workspace_bytes};
+  if (int rc = gn::check_token_logprobs(d, err)) return rc;
+  if (!gn::context(err)) return -1;
+  return gn::launch_token_logprobs(d, gn::resolve_stream(stream), err);
+}
+
+int gn_token_logprobs_backward(int dtype, const void *logits, long rows, long cols, long ld, float temperature,
+                               const int64_t *targets, const float *lse, const float *entropy,
+                               const float *grad_logprob, const float *grad_entropy, void *grad_logits, long ldg,
+                               void *stream, CError *err) {
+  const gn::LogprobsGradDesc d{{dtype, logits, rows, cols, ld, temperature}, targets, lse, entropy, grad_logprob,
+                               grad_entropy, grad_logits, ldg};
+  if (int rc = gn::check_token_logprobs_backward(d, err)) return rc;
+  if (!gn::context(err)) return -1;
+  return gn::launch_token_logprobs_backward(d, gn::resolve_stream(stream), err);
+}
+
+int gn_distill_forward(int dtype, const void *logits, long rows, long cols, long ld, float temperature,
+                       const int64_t *ids, const float *teacher, int k, float *loss, float *lse, void *workspace,
+                       size_t workspace_bytes, void *stream, CError *err) {
+  const gn::DistillDesc d{{dtype, logits, rows, cols, ld, temperature}, ids, teacher, k, loss, lse, workspace,
+                          workspace_bytes, nullptr, nullptr, nullptr, 0};
+  if (int rc = gn::check_distill_forward(d, err)) return rc;
+  if (!gn::context(err)) return -1;
+  return gn::launch_distill_forward(d, gn::resolve_stream(stream), err);
+}
+
+int gn_distill_backward(int dtype, const void *logits, long rows, long cols, long ld, float temperature,
+                        const int64_t *ids, const float *teacher, int k, const float *lse, const float *grad_loss,
+                        void *grad_logits, long ldg, void *stream, CError *err) {
+  const gn::DistillDesc d{{dtype, logits, rows, cols, ld, temperature}, ids, teacher, k, nullptr, nullptr, nullptr, 0,
+                          lse, grad_loss, grad_logits, ldg};
+  if (int rc = gn::check_distill_backward(d, err)) return rc;
+  if (!gn::context(err)) return -1;
+  return gn::launch_distill_backward(d, gn::resolve_stream(stream), err);
 }
 
 int gn_spmm_csr(long M, long N, long K, long nnz, const int32_t *rowptr, const int32_t *col, const float *val,

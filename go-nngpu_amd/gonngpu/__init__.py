@@ -18,7 +18,7 @@ REPO_DIR = os.path.dirname(PKG_DIR)
 LIB_PATH = os.path.join(PKG_DIR, "lib", "libgonngpu.so")
 HEADER_PATH = os.path.join(REPO_DIR, "include", "gonngpu.h")
 
-GN_F32, GN_F16 = 0, 1
+GN_F32, GN_F16, GN_MXFP4 = 0, 1, 2
 ROUND_NEAREST_EVEN, ROUND_TOWARD_ZERO = 0, 1
 ACT_NONE, ACT_RELU, ACT_SIGMOID, ACT_TANH, ACT_LEAKY_RELU, ACT_ELU, ACT_SWISH, ACT_GELU = -1, 0, 1, 2, 4, 5, 6, 7
 
@@ -106,6 +106,15 @@ SIGNATURES = {
     "perform_activation_elu_forward": (_I, [_VP, _L, _F, _VP, _VP, _ERR]),
     "perform_activation_swish_forward": (_I, [_VP, _L, _VP, _VP, _ERR]),
     "perform_activation_gelu_forward": (_I, [_VP, _L, _VP, _VP, _ERR]),
+    "gn_mxfp4_size": (_I, [_L, _L, ctypes.POINTER(_SZ), ctypes.POINTER(_SZ), _ERR]),
+    "gn_mxfp4_quantize": (_I, [_I, _VP, _L, _L, _L, _VP, _VP, _VP, _ERR]),
+    "gn_mxfp4_dequantize": (_I, [_VP, _VP, _L, _L, _I, _VP, _L, _VP, _ERR]),
+    "gn_mxfp4_gemm": (_I, [_I, _L, _L, _L, _F, _VP, _L, _VP, _VP, _VP, _F, _VP, _L, _VP, _I, _F, _VP, _ERR]),
+    "gn_logits_workspace": (_SZ, [_L, _L, _I]),
+    "gn_token_logprobs": (_I, [_I, _VP, _L, _L, _L, _F, _VP, _VP, _VP, _VP, _I, _VP, _VP, _VP, _SZ, _VP, _ERR]),
+    "gn_token_logprobs_backward": (_I, [_I, _VP, _L, _L, _L, _F, _VP, _VP, _VP, _VP, _VP, _VP, _L, _VP, _ERR]),
+    "gn_distill_forward": (_I, [_I, _VP, _L, _L, _L, _F, _VP, _VP, _I, _VP, _VP, _VP, _SZ, _VP, _ERR]),
+    "gn_distill_backward": (_I, [_I, _VP, _L, _L, _L, _F, _VP, _VP, _I, _VP, _VP, _VP, _L, _VP, _ERR]),
     "gn_spmm_csr": (_I, [_L, _L, _L, _L, _VP, _VP, _VP, _VP, _L, _VP, _L, _VP, _VP, _ERR]),
     "gn_spmv_csr": (_I, [_L, _L, _L, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _ERR]),
     "gn_spmv_plan_create": (_I, [_L, _L, _L, _VP, _VP, ctypes.POINTER(_VP), _VP, _ERR]),
@@ -335,6 +344,204 @@ def softmax_rows(x, out, stream_ptr=None):
 
 def transpose(x, out, stream_ptr=None):
     _dispatch(stream_ptr, "gn_transpose_f32", _ptr(x), x.shape[0], x.shape[1], _ptr(out))
+
+
+def _refuse(message):
+    raise GonngpuError(-1, message)
+
+
+def _device_of(*tensors):
+    """The tensors' common device, which has to be the current one: kernels start there."""
+    import torch
+
+    tensors = [t for t in tensors if t is not None]
+    for t in tensors:
+        if not t.is_cuda or t.get_device() != torch.cuda.current_device():
+            _refuse(f"a tensor on {t.device}: all have to be on the current GPU")
+
+
+def _expect(what, t, dtype, shape):
+    """Checks an argument that is one dense array of the given type and shape."""
+    if t.dtype != dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+        _refuse(f"{what}: a contiguous {dtype} tensor of shape {tuple(shape)} is needed, got {t.dtype} {tuple(t.shape)}")
+
+
+def _matrix(what, t):
+    """(GN_F32 or GN_F16, rows, cols, elements from row to row) of a matrix whose rows are dense."""
+    import torch
+
+    if t.dtype not in (torch.float32, torch.float16):
+        _refuse(f"{what}: float32 or float16 is needed, got {t.dtype}")
+    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+        _refuse(f"{what}: a matrix of dense rows is needed, got shape {tuple(t.shape)}, strides {t.stride()}")
+    rows, cols = t.shape
+    return (GN_F16 if t.dtype == torch.float16 else GN_F32), rows, cols, (t.stride(0) if rows > 1 else cols)
+
+
+def _mxfp4_matrix(what, data, scales, cols):
+    """Checks the two arrays of a stored MXFP4 matrix of `cols` columns; its rows."""
+    import torch
+
+    groups = -(-cols // 128)
+    rows = data.shape[0] if data.dim() == 2 else -1
+    _expect(f"{what} data", data, torch.uint8, (rows, 64 * groups))
+    _expect(f"{what} scales", scales, torch.uint8, (rows, 4 * groups))
+    return rows
+
+
+def mxfp4_empty(rows, cols, device="cuda"):
+    """The two arrays (codes, scales) of a rows x cols MXFP4 matrix, not filled in."""
+    import torch
+
+    groups = -(-cols // 128)
+    return (torch.empty((rows, 64 * groups), dtype=torch.uint8, device=device),
+            torch.empty((rows, 4 * groups), dtype=torch.uint8, device=device))
+
+
+def mxfp4_quantize(x, data, scales, stream_ptr=None):
+    """A float32 or float16 matrix brought to MXFP4, into the arrays of mxfp4_empty(*x.shape)."""
+    dt, rows, cols, ld = _matrix("mxfp4_quantize", x)
+    if _mxfp4_matrix("mxfp4_quantize", data, scales, cols) != rows:
+        _refuse(f"mxfp4_quantize: {rows} rows into arrays of {data.shape[0]}")
+    _device_of(x, data, scales)
+    _dispatch(stream_ptr, "gn_mxfp4_quantize", dt, _ptr(x), rows, cols, ld, _ptr(data), _ptr(scales))
+
+
+def mxfp4_dequantize(data, scales, out, stream_ptr=None):
+    """The values of a stored MXFP4 matrix, to a float32 or float16 matrix of its size."""
+    dt, rows, cols, ld = _matrix("mxfp4_dequantize", out)
+    if _mxfp4_matrix("mxfp4_dequantize", data, scales, cols) != rows:
+        _refuse(f"mxfp4_dequantize: {data.shape[0]} rows into {rows}")
+    _device_of(data, scales, out)
+    _dispatch(stream_ptr, "gn_mxfp4_dequantize", _ptr(data), _ptr(scales), rows, cols, dt, _ptr(out), ld)
+
+
+def mxfp4_gemm(A, B, C, *, alpha=1.0, beta=0.0, bias=None, act=ACT_NONE, act_alpha=0.0, K=None, stream_ptr=None):
+    """C = act(alpha*A*B^T + beta*C + bias) with B = (codes, scales) of an outputs x inputs MXFP4 matrix. A is a float16
+    matrix, or a pair like B; then K is the number of columns (the arrays hold it rounded up to 128)."""
+    import torch
+
+    dtc, M, N, ldc = _matrix("mxfp4_gemm: C", C)
+    if dtc != GN_F32:
+        _refuse("mxfp4_gemm: C is float32")
+    if isinstance(A, (tuple, list)):
+        a, a_scales = A
+        if K is None:
+            K = 2 * a.shape[1]
+        dt, lda, rows = GN_MXFP4, 0, _mxfp4_matrix("mxfp4_gemm: A", a, a_scales, K)
+    else:
+        a, a_scales = A, None
+        dt, rows, cols, lda = _matrix("mxfp4_gemm: A", a)
+        if dt != GN_F16 or K not in (None, cols):
+            _refuse(f"mxfp4_gemm: A is float16 with K columns or a pair of MXFP4 arrays, got {a.dtype}, K = {K}")
+        K = cols
+    if rows != M:
+        _refuse(f"mxfp4_gemm: {rows} rows of A, {M} of C")
+    if _mxfp4_matrix("mxfp4_gemm: B", B[0], B[1], K) != N:
+        _refuse(f"mxfp4_gemm: {B[0].shape[0]} rows of B, {N} columns of C")
+    if bias is not None:
+        _expect("mxfp4_gemm: bias", bias, torch.float32, (N,))
+    _device_of(a, a_scales, B[0], B[1], C, bias)
+    _dispatch(stream_ptr, "gn_mxfp4_gemm", dt, M, N, K, alpha, _ptr(a), lda, _ptr(a_scales), _ptr(B[0]), _ptr(B[1]),
+              beta, _ptr(C), ldc, _ptr(bias), act, act_alpha)
+
+
+def _logits_workspace(rows, cols, k, device, stream_ptr):
+    """Scratch for one call, from torch's allocator (which keeps what a captured graph uses)."""
+    import torch
+
+    n = load().gn_logits_workspace(rows, cols, k)
+    if n == 0:
+        return None, 0
+    ws = torch.empty((n,), dtype=torch.uint8, device=device)
+    if stream_ptr is not None and stream_ptr != _current_stream():
+        ws.record_stream(torch.cuda.ExternalStream(stream_ptr))
+    return ws, n
+
+
+def token_logprobs(logits, targets, logprob, *, lse=None, entropy=None, top_ids=None, top_logprobs=None,
+                   temperature=1.0, stream_ptr=None):
+    """logprob[r] = log softmax(logits[r] / temperature)[targets[r]] (int64; below 0: no target, 0), log-sum-exp
+    and entropy of each row (float32), and the columns (int64) and log-probabilities of its k largest
+    logits, k the width of top_ids, at most 64. targets and logprob may be None together."""
+    import torch
+
+    dt, rows, cols, ld = _matrix("token_logprobs", logits)
+    if (targets is None) != (logprob is None) or (top_ids is None) != (top_logprobs is None):
+        _refuse("token_logprobs: targets and logprob, and top_ids and top_logprobs, are given together")
+    k = 0
+    if top_ids is not None:
+        k = top_ids.shape[-1] if top_ids.dim() == 2 else -1
+        _expect("token_logprobs: top_ids", top_ids, torch.int64, (rows, k))
+        _expect("token_logprobs: top_logprobs", top_logprobs, torch.float32, (rows, k))
+    if targets is not None:
+        _expect("token_logprobs: targets", targets, torch.int64, (rows,))
+    for what, t in (("logprob", logprob), ("lse", lse), ("entropy", entropy)):
+        if t is not None:
+            _expect("token_logprobs: " + what, t, torch.float32, (rows,))
+    _device_of(logits, targets, logprob, lse, entropy, top_ids, top_logprobs)
+    ws, n = _logits_workspace(rows, cols, k, logits.device, stream_ptr)
+    _dispatch(stream_ptr, "gn_token_logprobs", dt, _ptr(logits), rows, cols, ld, temperature, _ptr(targets),
+              _ptr(logprob), _ptr(lse), _ptr(entropy), k, _ptr(top_ids), _ptr(top_logprobs), _ptr(ws), n)
+
+
+def token_logprobs_backward(logits, targets, lse, grad_logprob, grad_logits, *, entropy=None, grad_entropy=None,
+                            temperature=1.0, stream_ptr=None):
+    """The gradient of the logits (their type; may be the logits themselves) from those of logprob and, with
+    the forward's entropy, of the entropy."""
+    import torch
+
+    dt, rows, cols, ld = _matrix("token_logprobs_backward", logits)
+    dg, grows, gcols, ldg = _matrix("token_logprobs_backward: grad_logits", grad_logits)
+    if (dg, grows, gcols) != (dt, rows, cols):
+        _refuse("token_logprobs_backward: grad_logits has the type and shape of logits")
+    if (targets is None) != (grad_logprob is None) or (entropy is None) != (grad_entropy is None):
+        _refuse("token_logprobs_backward: targets and grad_logprob, and entropy and grad_entropy, are given together")
+    if targets is not None:
+        _expect("token_logprobs_backward: targets", targets, torch.int64, (rows,))
+    for what, t in (("lse", lse), ("grad_logprob", grad_logprob), ("entropy", entropy), ("grad_entropy", grad_entropy)):
+        if t is not None:
+            _expect("token_logprobs_backward: " + what, t, torch.float32, (rows,))
+    _device_of(logits, targets, lse, grad_logprob, grad_logits, entropy, grad_entropy)
+    _dispatch(stream_ptr, "gn_token_logprobs_backward", dt, _ptr(logits), rows, cols, ld, temperature, _ptr(targets),
+              _ptr(lse), _ptr(entropy), _ptr(grad_logprob), _ptr(grad_entropy), _ptr(grad_logits), ldg)
+
+
+def distill(logits, ids, teacher, loss, *, lse=None, temperature=1.0, stream_ptr=None):
+    """loss[r] = temperature^2 KL(teacher || student) with the teacher's softmax over its entries ids[r] (int64, below 0:
+    absent), teacher[r] (float32 logits or log-probabilities), at most 256 of them, and the student's
+    over all columns of logits[r]; lse: the student's log-sum-exp."""
+    import torch
+
+    dt, rows, cols, ld = _matrix("distill", logits)
+    k = ids.shape[-1] if ids.dim() == 2 else -1
+    _expect("distill: ids", ids, torch.int64, (rows, k))
+    _expect("distill: teacher", teacher, torch.float32, (rows, k))
+    for what, t in (("loss", loss), ("lse", lse)):
+        if t is not None:
+            _expect("distill: " + what, t, torch.float32, (rows,))
+    _device_of(logits, ids, teacher, loss, lse)
+    ws, n = _logits_workspace(rows, cols, 0, logits.device, stream_ptr)
+    _dispatch(stream_ptr, "gn_distill_forward", dt, _ptr(logits), rows, cols, ld, temperature, _ptr(ids), _ptr(teacher),
+              k, _ptr(loss), _ptr(lse), _ptr(ws), n)
+
+
+def distill_backward(logits, ids, teacher, lse, grad_loss, grad_logits, *, temperature=1.0, stream_ptr=None):
+    """The gradient of the logits (their type; may be the logits themselves) from that of distill's loss."""
+    import torch
+
+    dt, rows, cols, ld = _matrix("distill_backward", logits)
+    dg, grows, gcols, ldg = _matrix("distill_backward: grad_logits", grad_logits)
+    if (dg, grows, gcols) != (dt, rows, cols):
+        _refuse("distill_backward: grad_logits has the type and shape of logits")
+    k = ids.shape[-1] if ids.dim() == 2 else -1
+    _expect("distill_backward: ids", ids, torch.int64, (rows, k))
+    _expect("distill_backward: teacher", teacher, torch.float32, (rows, k))
+    _expect("distill_backward: lse", lse, torch.float32, (rows,))
+    _expect("distill_backward: grad_loss", grad_loss, torch.float32, (rows,))
+    _device_of(logits, ids, teacher, lse, grad_loss, grad_logits)
+    _dispatch(stream_ptr, "gn_distill_backward", dt, _ptr(logits), rows, cols, ld, temperature, _ptr(ids),
+              _ptr(teacher), k, _ptr(lse), _ptr(grad_loss), _ptr(grad_logits), ldg)
 
 
 def spmm_csr(M, N, K, nnz, rowptr, col, val, D, C, flags=None, ldd=None, ldc=None, stream_ptr=None):

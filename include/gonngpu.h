@@ -264,7 +264,8 @@ void free_c_error_message(char *message);
 /* Part 2 — device-pointer API (no reference counterpart)                      */
 /* ========================================================================== */
 
-typedef enum { GN_F32 = 0, GN_F16 = 1 } gn_dtype;
+/* GN_MXFP4 is taken by the gn_mxfp4_* entry points only. */
+typedef enum { GN_F32 = 0, GN_F16 = 1, GN_MXFP4 = 2 } gn_dtype;
 typedef enum { GN_ROUND_NEAREST_EVEN = 0, GN_ROUND_TOWARD_ZERO = 1 } gn_round;
 /* Epilogue activations: GN_ACT_NONE plus the Go ActivationType codes. */
 enum { GN_ACT_NONE = -1, GN_ACT_RELU = 0, GN_ACT_SIGMOID = 1, GN_ACT_TANH = 2, GN_ACT_LEAKY_RELU = 4,
@@ -403,6 +404,83 @@ int gn_transpose_f32(const float *in, long rows, long cols, float *out, void *st
  * (gpu/matrix/mixed-precision.go:352-354), which adds a bias of any length cyclically over the
  * flat output (the GEMM epilogue covers len == output width). len == 0 with n > 0: -1. */
 int gn_add_bias_cyclic_f32(float *y, long n, const float *bias, long len, void *stream, CError *err);
+
+/* 4-bit matrices (MXFP4 of the OCP Microscaling Formats specification): a row is cut into blocks of
+ * 32 values; a block has one scale byte E, standing for 2^(E - 127) (255: the block is NaN), and
+ * each value a 4-bit code: a sign (bit 3) and the magnitudes 0, 0.5, 1, 1.5, 2, 3, 4, 6 (codes 0-7).
+ * Stored: G = ceil(cols / 128) groups of 4 blocks to a row, rows one after the other. data holds 64 G bytes
+ * to a row, two codes to a byte, the value with the even index in the low half; scales holds 4 G bytes to a row. data starts
+ * at a multiple of 16 bytes, scales at one of 4. Values past cols are 0 (gn_mxfp4_quantize writes
+ * them; a matrix from elsewhere must have code 0 and a scale byte below 255 there).
+ * gn_mxfp4_size: the bytes of the two arrays. -1 for a negative size or one that overflows. */
+int gn_mxfp4_size(long rows, long cols, size_t *data_bytes, size_t *scale_bytes, CError *err);
+/* x (GN_F32 or GN_F16, rows x cols, ldx >= cols elements from row to row) brought to MXFP4:
+ * E = clamp(floor(log2(max |x|)) - 2, -127, 125) + 127 for a block, 127 for one of zeros, 255 for one
+ * with an infinity or NaN (its codes are 0); a value is x 2^(127 - E) rounded to the nearest code, ties to the even one,
+ * and to 6 above 6 (zeros and values that round to 0 keep their sign). Asynchronous; allocates nothing. At most
+ * 2^25 rows and 65535 * 2048 columns here and in gn_mxfp4_dequantize.
+ * Codes: -1 invalid argument, -6 launch error. */
+int gn_mxfp4_quantize(int dtype, const void *x, long rows, long cols, long ldx, void *data, void *scales,
+                      void *stream, CError *err);
+/* The values that a stored matrix stands for, to GN_F32 (exact) or GN_F16 (rounded to nearest even)
+ * rows x cols, ldo >= cols elements from row to row; out[r, j] past cols is not written. */
+int gn_mxfp4_dequantize(const void *data, const void *scales, long rows, long cols, int dtype, void *out, long ldo,
+                        void *stream, CError *err);
+/* C[M,N] = act( alpha * A * B^T + beta * C + bias[n] ), B an N x K matrix in MXFP4 (a linear layer's weights,
+ * outputs x inputs), fp32 accumulation. A is M x K: GN_F16 (lda >= K elements from row to row, a_scales NULL; each weight
+ * takes part with its exact value) or GN_MXFP4 (data and scales as above, lda is not read).
+ * C and bias are fp32; bias may be NULL; beta == 0 never reads C; act and act_alpha as gn_gemm; K == 0
+ * gives act(beta * C + bias). Asynchronous; allocates nothing and may be captured.
+ * Codes: -1 invalid argument, -6 launch error. */
+int gn_mxfp4_gemm(int a_dtype, long M, long N, long K, float alpha, const void *A, long lda, const void *a_scales,
+                  const void *B, const void *b_scales, float beta, float *C, long ldc, const float *bias, int act,
+                  float act_alpha, void *stream, CError *err);
+
+/* Rows of logits (GN_F32 or GN_F16, rows x cols, cols >= 1, ld >= cols elements from row to row), z = x / temperature in
+ * fp32 (x times the temperature's fp32 reciprocal), temperature finite and above 0:
+ *   lse[r] = ln sum_j e^z[r,j]      logprob[r] = z[r, targets[r]] - lse[r]
+ *   entropy[r] = - sum_j p_j ln p_j, p = e^(z - lse)
+ *   top_ids[r, 0..k), top_logprobs[r, 0..k): the k largest logits' columns and z - lse, largest first, the
+ *   lower column first among equals (NaN counts as larger than any number, -0 equals 0); 0 <= k <= min(64, cols).
+ * A target below 0 gives logprob 0 (a row without one), one of cols or above NaN. Columns of -inf have p = 0. A row of
+ * -inf only has lse and log-probabilities of -inf and entropy 0; a row with NaN or +inf has NaN in all of them.
+ * lse, entropy may be NULL; targets and logprob are NULL together; the two top arrays may be NULL where k is 0.
+ * workspace: gn_logits_workspace(rows, cols, k) bytes at a multiple of 16 (may be NULL where that is 0), not
+ * shared by calls that may overlap. Asynchronous; allocates nothing and may be captured. No result
+ * depends on timing. Codes: -1 invalid argument, -6 launch error. */
+size_t gn_logits_workspace(long rows, long cols, int k);
+int gn_token_logprobs(int dtype, const void *logits, long rows, long cols, long ld, float temperature,
+                      const int64_t *targets, float *logprob, float *lse, float *entropy, int k, int64_t *top_ids,
+                      float *top_logprobs, void *workspace, size_t workspace_bytes, void *stream, CError *err);
+/* The gradient of the logits from those of logprob and entropy:
+ *   grad_logits[r,j] = ( g_l (1[j = targets[r]] - p_j) - g_h p_j (ln p_j + entropy[r]) ) / temperature
+ * with g_l = grad_logprob[r] (0 for a target below 0) and g_h = grad_entropy[r]. grad_logits has the
+ * logits' type, ldg >= cols elements from row to row, and may be the logits themselves (ldg == ld). lse and entropy are those that
+ * gn_token_logprobs gave for the same logits and temperature. targets and grad_logprob may be NULL together;
+ * so may entropy and grad_entropy. A row of -inf only has gradient 0; one with NaN or +inf, or with a target of
+ * cols or above, NaN. Where both of a row's gradients are 0 its gradient is 0 whatever the logits hold. */
+int gn_token_logprobs_backward(int dtype, const void *logits, long rows, long cols, long ld, float temperature,
+                               const int64_t *targets, const float *lse, const float *entropy,
+                               const float *grad_logprob, const float *grad_entropy, void *grad_logits, long ldg,
+                               void *stream, CError *err);
+/* Distillation from a teacher's top logits: ids[r, 0..k) are columns, teacher[r, 0..k) the teacher's
+ * logits (or log-probabilities) there, 1 <= k <= 256. With p = softmax over the present entries of
+ * teacher / temperature and q = softmax(logits[r] / temperature) over all columns,
+ *   loss[r] = temperature^2 sum_i p_i (ln p_i - ln q[ids[r,i]]),
+ *   lse[r] = ln sum_j e^(logits[r,j] / temperature).
+ * An entry whose id is below 0 or whose teacher logit is -inf is absent; a row of absent entries has loss 0 and gradient 0. An id
+ * may occur more than once. An id of cols or above, a NaN or +inf teacher logit, and a NaN or +inf logit
+ * make the row's loss NaN (its gradient too). Where a present id's logit is -inf the loss is +inf. lse may be NULL.
+ * workspace: gn_logits_workspace(rows, cols, 0) bytes, as for gn_token_logprobs. */
+int gn_distill_forward(int dtype, const void *logits, long rows, long cols, long ld, float temperature,
+                       const int64_t *ids, const float *teacher, int k, float *loss, float *lse, void *workspace,
+                       size_t workspace_bytes, void *stream, CError *err);
+/* grad_logits[r,j] = grad_loss[r] temperature (q_j - sum over i with ids[r,i] = j of p_i), in the logits'
+ * type; lse from gn_distill_forward; grad_logits may be the logits themselves (ldg == ld). A row whose
+ * grad_loss is 0 has gradient 0 whatever the logits hold. */
+int gn_distill_backward(int dtype, const void *logits, long rows, long cols, long ld, float temperature,
+                        const int64_t *ids, const float *teacher, int k, const float *lse, const float *grad_loss,
+                        void *grad_logits, long ldg, void *stream, CError *err);
 
 /* CSR SpMM on device arrays: C[M,N] = S[M,K] * D[K,N] (ld = row pitch in elements).
  * Accumulates each output in CSR order with one fused multiply-add per stored entry.
