@@ -5,6 +5,10 @@
 
 namespace gn {
 
+constexpr int kBlock = 32;   // values to a scale
+constexpr int kGroup = 128;  // values to a group of 4 blocks
+__host__ __device__ inline long groups_of(long cols) { return (cols + kGroup - 1) / kGroup; }
+
 // The scale byte of a block, from the bits of its largest magnitude (bits without the sign are ordered
 // as the values are, NaN above infinity): floor(log2(top)) - 2 + 127, at least 0; 127 for a block of
 // zeros, 255 for one with an infinity or NaN. The exponent field is floor(log2(top)) + 127 for a normal
@@ -14,13 +18,6 @@ __host__ __device__ inline unsigned block_scale(uint32_t top) {
   if (top == 0) return 127;
   if (field == 255) return 255;
   return (unsigned)(field > 2 ? field - 2 : 0);
-}
-
-// The value of an e2m1 code: exponent in bits 2:1, fraction in bit 0, sign in bit 3.
-__host__ __device__ inline float code_value(unsigned code) {
-  const unsigned e = (code >> 1) & 3, f = code & 1;
-  const float v = e ? (float)(2 + f) * 0.5f * (float)(1u << (e - 1)) : 0.5f * (float)f;
-  return code & 8 ? -v : v;
 }
 
 // Whether every code times 2^(e - 127) is a normal fp16 value or zero: 0.5 2^-13 to 6 2^13.
@@ -43,6 +40,9 @@ struct MxGemmDesc {
 
 // Bytes of a stored matrix; false for a negative size or one past 2^62 bytes.
 bool mxfp4_size(long rows, long cols, size_t *data, size_t *scales);
+// A stored matrix, and one of GN_F32 or GN_F16: 0, or -1 with a message.
+int check_mxfp4_matrix(const char *what, const void *data, const void *scales, long rows, long cols, CError *err);
+int check_plain_matrix(const char *what, int dtype, const void *x, long rows, long cols, long ld, CError *err);
 // The checks need no device; the launchers expect arguments that passed them.
 int check_mxfp4_quantize(int dtype, const void *x, long rows, long cols, long ldx, const void *data,
                          const void *scales, CError *err);

@@ -1,0 +1,347 @@
+// mxfp4_gemm.hip — products with MXFP4 weights, C = act(alpha A B^T + beta C + bias).
+#include <algorithm>
+#include <climits>
+
+#include "gemm_tile.h"
+#include "mxfp4.h"
+
+namespace gn {
+namespace {
+
+constexpr long kMaxK = 1L << 23;  // 256 rows of codes stay below 2^30 bytes: 32-bit offsets within a tile
+
+typedef int i32x8_t __attribute__((ext_vector_type(8)));
+typedef float float16_t __attribute__((ext_vector_type(16)));
+typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
+
+// 2^(E - 127); NaN for 255.
+__device__ __forceinline__ float scale_of(unsigned e) {
+  return __uint_as_float((e << 23) | ((e == 0 || e == 255) ? 0x00400000u : 0u));
+}
+
+struct MxParams : GemmParams {
+  const uint8_t *as, *bs;  // scales
+  int G;                   // groups to a row
+};
+
+// c + A B^T of 16 x 128 codes each; the scales are byte S of sa and sb.
+template <int S>
+__device__ __forceinline__ float4_t mfma_fp4(u32x4_t a, u32x4_t b, float4_t c, uint32_t sa, uint32_t sb) {
+  const i32x8_t x = {(int)a[0], (int)a[1], (int)a[2], (int)a[3], 0, 0, 0, 0};
+  const i32x8_t y = {(int)b[0], (int)b[1], (int)b[2], (int)b[3], 0, 0, 0, 0};
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, y, c, 4, 4, S, (int)sa, S, (int)sb);
+}
+
+// Eight codes as halves, times 2^(exponent of unit - 127).
+__device__ __forceinline__ half8_t half8_of(uint32_t w, float unit) {
+  const half2_t a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, unit, 0);
+  const half2_t b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, unit, 1);
+  const half2_t c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, unit, 2);
+  const half2_t d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, unit, 3);
+  return half8_t{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+__device__ __forceinline__ float finish(const MxParams &p, float acc, long m, long n) {
+  float v = p.alpha * acc;
+  if (p.beta != 0.0f) v += p.beta * p.C[m * p.ldc + n];
+  if (p.bias) v += p.bias[n];
+  return apply_act(p.act, v, p.act_alpha);
+}
+
+// One wave per 16 x 16 tile, operands from global memory.
+template <bool FP4>
+__global__ void __launch_bounds__(64) mx_tile_kernel(MxParams p) {
+  const int lane = threadIdx.x, l16 = lane & 15, g = lane >> 4;
+  const long tn = (p.N + 15) / 16, m0 = blockIdx.x / tn * 16, n0 = blockIdx.x % tn * 16;
+  const long am = min(m0 + l16, p.M - 1), bn = min(n0 + l16, p.N - 1), G = p.G;
+  const u32x4_t *b = static_cast<const u32x4_t *>(p.B) + bn * G * 4 + g;
+  const uint32_t *bs = reinterpret_cast<const uint32_t *>(p.bs) + bn * G;
+  float4_t acc = {0, 0, 0, 0};
+  for (long c = 0; c < G; ++c) {
+    const u32x4_t bq = b[c * 4];
+    const uint32_t bsc = bs[c];
+    if constexpr (FP4) {
+      const u32x4_t aq = (static_cast<const u32x4_t *>(p.A) + am * G * 4 + g)[c * 4];
+      const uint32_t asc = (reinterpret_cast<const uint32_t *>(p.as) + am * G)[c];
+      acc = mfma_fp4<0>(aq, bq, acc, asc >> (8 * g), bsc >> (8 * g));
+    } else {
+      const _Float16 *a = static_cast<const _Float16 *>(p.A) + am * p.lda;
+      half8_t av[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const long k = c * kGroup + g * kBlock + j * 8 + e;
+          av[j][e] = k < p.K ? a[k] : (_Float16)0;
+        }
+      const unsigned e = (bsc >> (8 * g)) & 255;
+      if (__all(half_exact(e))) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(av[j], half8_of(bq[j], scale_of(e)), acc, 0, 0, 0);
+      } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {  // block q of both sides, the rest zeros
+          float4_t part = {0, 0, 0, 0};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const half8_t z = {0, 0, 0, 0, 0, 0, 0, 0};
+            part = __builtin_amdgcn_mfma_f32_16x16x32_f16(g == q ? av[j] : z, g == q ? half8_of(bq[j], 1.0f) : z, part,
+                                                          0, 0, 0);
+          }
+          const float unit = scale_of((bsc >> (8 * q)) & 255);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[i] = fmaf(part[i], unit, acc[i]);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const long m = m0 + 4 * g + i, n = n0 + l16;
+    if (m < p.M && n < p.N) p.C[m * p.ldc + n] = finish(p, acc[i], m, n);
+  }
+}
+
+// K == 0: act(beta C + bias).
+__global__ void __launch_bounds__(256) mx_k0_kernel(MxParams p) {
+  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < p.M * p.N; i += (long)gridDim.x * 256)
+    p.C[i / p.N * p.ldc + i % p.N] = finish(p, 0.0f, i / p.N, i % p.N);
+}
+
+// ------------------------------------------------------------------ both sides in 4 bits
+// c + A B^T of 32 x 64 codes each; the scales are byte S of sa and sb.
+template <int S>
+__device__ __forceinline__ float16_t mfma32_fp4(u32x4_t a, u32x4_t b, float16_t c, uint32_t sa, uint32_t sb) {
+  const i32x8_t x = {(int)a[0], (int)a[1], (int)a[2], (int)a[3], 0, 0, 0, 0};
+  const i32x8_t y = {(int)b[0], (int)b[1], (int)b[2], (int)b[3], 0, 0, 0, 0};
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x, y, c, 4, 4, S, (int)sa, S, (int)sb);
+}
+
+// C = A B^T on v_mfma_scale_f32_32x32x64_f8f6f4 (from registers it sustains 6.4 PFLOP/s on random codes and 9.7 on
+// zeros, the 16 x 16 x 128 form 5.8 and 6.8). WM x WN waves, each FM x FN blocks of 32 x 32. K goes in stages of
+// a group (128 values, 64 bytes of codes to a row), copied straight to LDS by dma16 in chunks of 16 rows,
+// kSlots stages in flight. A row's 16 bytes o sit at place o ^ ((row >> 2) & 3) of its 64: the 16 rows that a phase of a
+// fragment read touches fall on distinct banks. Lane half h takes block 2 h + s of its row's four in step s of
+// two, on both sides, so its scales for the stage are two bytes next to each other, and the instruction's byte
+// selector is s. A row's scales for four stages are 16 bytes, copied to LDS by the same means: read into registers by each
+// wave they cost one cache line to a row and stage, and with two stages of 256 in flight that bound the kernel
+// (8192^3 369 us). A step multiplies while the next one's fragments are read; before a stage's second step the next
+// stage has landed (one wait and one barrier to a stage), and the copies of the one kSlots ahead go into the slot just left.
+constexpr int kSlots = 4;
+template <int WM, int WN, int FM, int FN, int WPE>
+__global__ void __launch_bounds__(WM * WN * 64) __attribute__((amdgpu_waves_per_eu(WPE, WPE)))
+mx_fp4_kernel(MxParams p) {
+  constexpr int NW = WM * WN, BM = WM * FM * 32, BN = WN * FN * 32;
+  constexpr int CA = BM / 16 / NW, CB = BN / 16 / NW, CPW = CA + CB;  // chunks of 16 rows to a wave
+  constexpr int STAGE = (BM + BN) * 64, SCALES = (BM + BN) * 16;      // bytes; SCALES: of four stages
+  constexpr int LDS = kSlots * STAGE + 2 * SCALES, EPI = WM * 16 * (BN + 4) * 4;
+  static_assert(CA * NW * 16 == BM && CB * NW * 16 == BN && BM % 64 == 0 && BN % 64 == 0 && kSlots == 4, "chunks");
+  __shared__ __attribute__((aligned(1024))) char smem[LDS > EPI ? LDS : EPI];
+
+  int tm, tn;
+  tile_coords(p, tm, tn);
+  const long m0 = (long)tm * BM, n0 = (long)tn * BN;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int wm = wave / WN, wn = wave % WN, l32 = lane & 31, h = lane >> 5;
+  const unsigned pitch = 64u * (unsigned)p.G, spitch = 4u * (unsigned)p.G;
+
+  // Codes: lane L of chunk c copies 16 bytes of row 16 c + L / 4, which land at 16 L of the chunk.
+  const char *a0 = static_cast<const char *>(p.A) + m0 * pitch, *b0 = static_cast<const char *>(p.B) + n0 * pitch;
+  const unsigned oct = 16u * ((lane & 3) ^ ((lane >> 4) & 3));
+  unsigned va[CA], vb[CB];
+#pragma unroll
+  for (int i = 0; i < CA; ++i) {
+    const int row = 16 * (wave * CA + i) + (lane >> 2);
+    va[i] = m0 + row < p.M ? row * pitch + oct : kOutOfRange;
+  }
+#pragma unroll
+  for (int i = 0; i < CB; ++i) {
+    const int row = 16 * (wave * CB + i) + (lane >> 2);
+    vb[i] = n0 + row < p.N ? row * pitch + oct : kOutOfRange;
+  }
+  const unsigned lds = lds_offset(smem);
+  auto issue = [&](int t) {  // past the last stage all reads are zeros
+    BufRsrc da = make_rsrc(a0 + 64L * t), db = make_rsrc(b0 + 64L * t);
+    da.r.z = db.r.z = __builtin_amdgcn_readfirstlane(t < p.G ? (int)ring::kNumRecords : 0);
+    const unsigned st = lds + (t & (kSlots - 1)) * STAGE;
+#pragma unroll
+    for (int i = 0; i < CA; ++i) dma16(da, va[i], __builtin_amdgcn_readfirstlane(st + (wave * CA + i) * 1024));
+#pragma unroll
+    for (int i = 0; i < CB; ++i) dma16(db, vb[i], __builtin_amdgcn_readfirstlane(st + BM * 64 + (wave * CB + i) * 1024));
+  };
+  // Scales: wave w copies rows 64 w .. 64 w + 63 of the tile's BM + BN (then 64 (w + NW) ..), 16 bytes of each. Rows past
+  // the matrix and bytes past its end are zeros, groups past a row's end are another row's; the stages that they belong to are
+  // not run.
+  constexpr int SB = (BM + BN) / 64;  // blocks of 64 rows
+  auto issue_scales = [&](int c) {  // of stages 4 c .. 4 c + 3
+#pragma unroll
+    for (int i = 0; i < (SB + NW - 1) / NW; ++i) {
+      const int blk = wave + i * NW;
+      const bool is_a = blk < BM / 64;
+      if (blk >= SB) break;
+      const long rows = is_a ? min(p.M - m0, (long)BM) : min(p.N - n0, (long)BN);
+      const int row = 64 * (is_a ? blk : blk - BM / 64) + lane;
+      BufRsrc ds = make_rsrc((is_a ? p.as : p.bs) + (is_a ? m0 : n0) * spitch);
+      ds.r.z = __builtin_amdgcn_readfirstlane((int)(rows * spitch));
+      dma16(ds, 4 * c < p.G && row < rows ? row * spitch + 16 * c : kOutOfRange,
+            __builtin_amdgcn_readfirstlane(lds + kSlots * STAGE + (c & 1) * SCALES + blk * 1024));
+    }
+  };
+
+  u32x4_t fa[2][FM], fb[2][FN];   // fragments of even and odd steps
+  u32x4_t qa[FM], qb[FN];         // scales of four stages
+  const unsigned arow = (wm * FM * 32 + l32) * 64, brow = BM * 64 + (wn * FN * 32 + l32) * 64;
+  const unsigned sw = ((2 * h) ^ ((l32 >> 2) & 3)) << 4;
+  auto read_frags = [&](int t, int s) {
+    const char *st = smem + (t & (kSlots - 1)) * STAGE + (sw ^ (s << 4));
+#pragma unroll
+    for (int i = 0; i < FM; ++i) fa[s][i] = *reinterpret_cast<const u32x4_t *>(st + arow + i * 2048);
+#pragma unroll
+    for (int i = 0; i < FN; ++i) fb[s][i] = *reinterpret_cast<const u32x4_t *>(st + brow + i * 2048);
+  };
+  auto read_scales = [&](int t) {  // of stages t .. t + 3
+    const char *st = smem + kSlots * STAGE + ((t >> 2) & 1) * SCALES + l32 * 16;
+#pragma unroll
+    for (int i = 0; i < FM; ++i) qa[i] = *reinterpret_cast<const u32x4_t *>(st + (wm * FM + i) * 512);
+#pragma unroll
+    for (int i = 0; i < FN; ++i) qb[i] = *reinterpret_cast<const u32x4_t *>(st + (BM + (wn * FN + i) * 32) * 16);
+  };
+  // Stage s of the four: a lane's two bytes to the low end.
+  uint32_t ca[FM], cb[FN];
+  auto take_scales = [&](int s) {
+#pragma unroll
+    for (int i = 0; i < FM; ++i) ca[i] = qa[i][s] >> (16 * h);
+#pragma unroll
+    for (int i = 0; i < FN; ++i) cb[i] = qb[i][s] >> (16 * h);
+  };
+  float16_t acc[FM][FN];
+#pragma unroll
+  for (int i = 0; i < FM; ++i)
+#pragma unroll
+    for (int j = 0; j < FN; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+  auto mfma_rows = [&](auto step, int i0, int i1) {
+    constexpr int S = decltype(step)::value;
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+      if (i >= i0 && i < i1)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) acc[i][j] = mfma32_fp4<S>(fa[S][i], fb[S][j], acc[i][j], ca[i], cb[j]);
+  };
+  auto stage = [&](int t, auto of) {
+    constexpr int Q = decltype(of)::value;  // t % 4
+    __builtin_amdgcn_sched_barrier(0);
+    read_frags(t, 1);
+    take_scales(Q);
+    mfma_rows(ActCode<0>{}, 0, FM);
+    sched_interleave<FM * FN, FM + FN>();
+    __builtin_amdgcn_sched_barrier(0);
+    // All but the copies of stages t + 2 and t + 3 (and scales between them) are done: stage t + 1 is there.
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm(2 * CPW));
+    __syncthreads();
+    __builtin_amdgcn_sched_barrier(0);
+    mfma_rows(ActCode<1>{}, 0, 1);
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (Q == 0) issue_scales(t / 4 + 1);  // before stage t + 4's codes: there when they are
+    issue(t + kSlots);
+    read_frags(t + 1, 0);  // past the last stage: zeros, never used
+    if constexpr (Q == 3) read_scales(t + 1);
+    mfma_rows(ActCode<1>{}, 1, FM);
+    sched_interleave<(FM - 1) * FN, FM + FN>();
+  };
+
+  issue_scales(0);
+#pragma unroll
+  for (int t = 0; t < kSlots; ++t) issue(t);
+  __builtin_amdgcn_s_waitcnt(vmcnt_imm(3 * CPW));
+  __syncthreads();
+  read_frags(0, 0);
+  read_scales(0);
+  for (int t = 0;;) {
+    stage(t, ActCode<0>{});
+    if (++t == p.G) break;
+    stage(t, ActCode<1>{});
+    if (++t == p.G) break;
+    stage(t, ActCode<2>{});
+    if (++t == p.G) break;
+    stage(t, ActCode<3>{});
+    if (++t == p.G) break;
+  }
+  __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+  __syncthreads();  // no copy is under way and all waves are done with the slots: the epilogue takes their place
+  // Block (i, j): register r of lane (l32, h) holds row 8 (r / 4) + 4 h + r % 4 of column l32.
+  constexpr int LP = BN + 4;
+  float *stg = reinterpret_cast<float *>(smem);
+  store_tile_passes<BM, BN, WM, WN>(p, m0, n0, 0, stg, [&](int f) {
+#pragma unroll
+    for (int j = 0; j < FN; ++j)
+#pragma unroll
+      for (int r = 0; r < 8; ++r)
+        stg[(wm * 16 + 8 * (r / 4) + 4 * h + r % 4) * LP + (wn * FN + j) * 32 + l32] = acc[f / 2][j][8 * (f & 1) + r];
+  });
+}
+
+unsigned grid_of(long n, long per) { return (unsigned)std::max(1L, std::min((n + per - 1) / per, 1L << 20)); }
+
+template <int WM, int WN, int FM, int FN, int WPE>
+void launch_fp4(MxParams p, hipStream_t s) {
+  constexpr int BM = WM * FM * 32, BN = WN * FN * 32;
+  p.tiles_m = (int)((p.M + BM - 1) / BM);
+  p.tiles_n = (int)((p.N + BN - 1) / BN);
+  hipLaunchKernelGGL((mx_fp4_kernel<WM, WN, FM, FN, WPE>), dim3((unsigned)(p.tiles_m * p.tiles_n)), dim3(WM * WN * 64), 0, s, p);
+}
+
+}  // namespace
+
+int check_mxfp4_gemm(const MxGemmDesc &d, CError *err) {
+  if (d.a_dtype != GN_F16 && d.a_dtype != GN_MXFP4)
+    return set_error(err, -1, "mxfp4 gemm: unsupported dtype %d of A", d.a_dtype);
+  size_t n;
+  if (d.K > kMaxK) return set_error(err, -1, "mxfp4 gemm: K of %ld is too large", d.K);
+  if (d.M < 0 || d.N < 0 || d.K < 0) return set_error(err, -1, "mxfp4 gemm: negative size");
+  if (!act_supported(d.act)) return set_error(err, -1, "mxfp4 gemm: unsupported activation %d", d.act);
+  if (d.M == 0 || d.N == 0) return 0;
+  if (!d.C) return set_error(err, -1, "mxfp4 gemm: NULL C");
+  if (d.ldc < d.N) return set_error(err, -1, "mxfp4 gemm: leading dimension smaller than row length");
+  if ((uintptr_t)d.C % 4 || (uintptr_t)d.bias % 4) return set_error(err, -1, "mxfp4 gemm: C or bias not aligned to fp32");
+  if (!matrix_bytes(d.M, d.ldc, 4, &n) || n > ((size_t)1 << 62) || (d.M + 15) / 16 > (1L << 26) / ((d.N + 15) / 16))
+    return set_error(err, -1, "mxfp4 gemm: problem too large for the grid");
+  if (d.K == 0) return 0;
+  if (int rc = check_mxfp4_matrix("mxfp4 gemm: B", d.B, d.b_scales, d.N, d.K, err)) return rc;
+  if (d.a_dtype == GN_MXFP4) return check_mxfp4_matrix("mxfp4 gemm: A", d.A, d.a_scales, d.M, d.K, err);
+  if (d.a_scales) return set_error(err, -1, "mxfp4 gemm: scales given for an fp16 A");
+  return check_plain_matrix("mxfp4 gemm: A", GN_F16, d.A, d.M, d.K, d.lda, err);
+}
+
+int launch_mxfp4_gemm(const MxGemmDesc &d, hipStream_t s, CError *err) {
+  if (d.M == 0 || d.N == 0) return 0;
+  MxParams p{};
+  p.A = d.A;
+  p.as = static_cast<const uint8_t *>(d.a_scales);
+  p.B = d.B;
+  p.bs = static_cast<const uint8_t *>(d.b_scales);
+  p.G = (int)groups_of(d.K);
+  p.C = d.C;
+  p.bias = d.bias;
+  p.M = d.M, p.N = d.N, p.K = d.K, p.lda = d.lda, p.ldc = d.ldc;
+  p.alpha = d.alpha, p.beta = d.beta, p.act = d.act, p.act_alpha = d.act_alpha;
+  if (d.K == 0) {
+    hipLaunchKernelGGL(mx_k0_kernel, dim3(grid_of(d.M * d.N, 256)), dim3(256), 0, s, p);
+  } else {
+    const dim3 grid((unsigned)(((d.M + 15) / 16) * ((d.N + 15) / 16)));
+    if (d.a_dtype == GN_MXFP4 && d.M > 64 && d.M * d.N > (1L << 24))
+      launch_fp4<2, 4, 4, 2, 2>(p, s);
+    else if (d.a_dtype == GN_MXFP4 && d.M > 64)
+      launch_fp4<2, 2, 2, 2, 2>(p, s);
+    else if (d.a_dtype == GN_MXFP4)
+      hipLaunchKernelGGL(mx_tile_kernel<true>, grid, dim3(64), 0, s, p);
+    else
+      hipLaunchKernelGGL(mx_tile_kernel<false>, grid, dim3(64), 0, s, p);
+  }
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? 0 : hip_error(err, -6, "mxfp4 gemm launch", e);
+}
+
+}  // namespace gn
