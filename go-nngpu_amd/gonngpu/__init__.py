@@ -350,52 +350,66 @@ def _refuse(message):
     raise GonngpuError(-1, message)
 
 
-def _device_of(*tensors):
-    """The tensors' common device, which has to be the current one: kernels start there."""
-    import torch
+_torch = None
 
-    tensors = [t for t in tensors if t is not None]
-    for t in tensors:
-        if not t.is_cuda or t.get_device() != torch.cuda.current_device():
-            _refuse(f"a tensor on {t.device}: all have to be on the current GPU")
+
+def _types():
+    """torch, imported once at the first call that needs it (asking the import system each time costs a call 0.3 us)."""
+    global _torch
+    if _torch is None:
+        import torch
+
+        _torch = torch
+    return _torch
+
+
+def _device_of(first, *others):
+    """The tensors' common device, which has to be the current one: kernels start there."""
+    device = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != device:
+            _refuse(f"tensors on {first.device} and {t.device}")
+    if device < 0 or device != _types().cuda.current_device():
+        _refuse(f"a tensor on {first.device}: all have to be on the current GPU")
 
 
 def _expect(what, t, dtype, shape):
     """Checks an argument that is one dense array of the given type and shape."""
-    if t.dtype != dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
-        _refuse(f"{what}: a contiguous {dtype} tensor of shape {tuple(shape)} is needed, got {t.dtype} {tuple(t.shape)}")
+    if t.dtype is not dtype or t.shape != shape or not t.is_contiguous():
+        _refuse(f"{what}: a contiguous {dtype} tensor of shape {shape} is needed, got {t.dtype} {tuple(t.shape)}")
 
 
 def _matrix(what, t):
     """(GN_F32 or GN_F16, rows, cols, elements from row to row) of a matrix whose rows are dense."""
-    import torch
-
-    if t.dtype not in (torch.float32, torch.float16):
+    T = _types()
+    if t.dtype is T.float32:
+        dtype = GN_F32
+    elif t.dtype is T.float16:
+        dtype = GN_F16
+    else:
         _refuse(f"{what}: float32 or float16 is needed, got {t.dtype}")
-    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
-        _refuse(f"{what}: a matrix of dense rows is needed, got shape {tuple(t.shape)}, strides {t.stride()}")
-    rows, cols = t.shape
-    return (GN_F16 if t.dtype == torch.float16 else GN_F32), rows, cols, (t.stride(0) if rows > 1 else cols)
+    shape, strides = t.shape, t.stride()
+    if len(shape) != 2 or (strides[1] != 1 and shape[1] > 1) or (strides[0] < shape[1] and shape[0] > 1):
+        _refuse(f"{what}: a matrix of dense rows is needed, got shape {tuple(shape)}, strides {strides}")
+    return dtype, shape[0], shape[1], (strides[0] if shape[0] > 1 else shape[1])
 
 
 def _mxfp4_matrix(what, data, scales, cols):
     """Checks the two arrays of a stored MXFP4 matrix of `cols` columns; its rows."""
-    import torch
-
     groups = -(-cols // 128)
     rows = data.shape[0] if data.dim() == 2 else -1
-    _expect(f"{what} data", data, torch.uint8, (rows, 64 * groups))
-    _expect(f"{what} scales", scales, torch.uint8, (rows, 4 * groups))
+    u8 = _types().uint8
+    _expect(what, data, u8, (rows, 64 * groups))
+    _expect(what, scales, u8, (rows, 4 * groups))
     return rows
 
 
 def mxfp4_empty(rows, cols, device="cuda"):
     """The two arrays (codes, scales) of a rows x cols MXFP4 matrix, not filled in."""
-    import torch
-
+    T = _types()
     groups = -(-cols // 128)
-    return (torch.empty((rows, 64 * groups), dtype=torch.uint8, device=device),
-            torch.empty((rows, 4 * groups), dtype=torch.uint8, device=device))
+    return (T.empty((rows, 64 * groups), dtype=T.uint8, device=device),
+            T.empty((rows, 4 * groups), dtype=T.uint8, device=device))
 
 
 def mxfp4_quantize(x, data, scales, stream_ptr=None):
@@ -419,8 +433,7 @@ def mxfp4_dequantize(data, scales, out, stream_ptr=None):
 def mxfp4_gemm(A, B, C, *, alpha=1.0, beta=0.0, bias=None, act=ACT_NONE, act_alpha=0.0, K=None, stream_ptr=None):
     """C = act(alpha*A*B^T + beta*C + bias) with B = (codes, scales) of an outputs x inputs MXFP4 matrix. A is a float16
     matrix, or a pair like B; then K is the number of columns (the arrays hold it rounded up to 128)."""
-    import torch
-
+    T = _types()
     dtc, M, N, ldc = _matrix("mxfp4_gemm: C", C)
     if dtc != GN_F32:
         _refuse("mxfp4_gemm: C is float32")
@@ -440,7 +453,7 @@ def mxfp4_gemm(A, B, C, *, alpha=1.0, beta=0.0, bias=None, act=ACT_NONE, act_alp
     if _mxfp4_matrix("mxfp4_gemm: B", B[0], B[1], K) != N:
         _refuse(f"mxfp4_gemm: {B[0].shape[0]} rows of B, {N} columns of C")
     if bias is not None:
-        _expect("mxfp4_gemm: bias", bias, torch.float32, (N,))
+        _expect("mxfp4_gemm: bias", bias, T.float32, (N,))
     _device_of(a, a_scales, B[0], B[1], C, bias)
     _dispatch(stream_ptr, "gn_mxfp4_gemm", dt, M, N, K, alpha, _ptr(a), lda, _ptr(a_scales), _ptr(B[0]), _ptr(B[1]),
               beta, _ptr(C), ldc, _ptr(bias), act, act_alpha)
@@ -448,14 +461,13 @@ def mxfp4_gemm(A, B, C, *, alpha=1.0, beta=0.0, bias=None, act=ACT_NONE, act_alp
 
 def _logits_workspace(rows, cols, k, device, stream_ptr):
     """Scratch for one call, from torch's allocator (which keeps what a captured graph uses)."""
-    import torch
-
+    T = _types()
     n = load().gn_logits_workspace(rows, cols, k)
     if n == 0:
         return None, 0
-    ws = torch.empty((n,), dtype=torch.uint8, device=device)
+    ws = T.empty((n,), dtype=T.uint8, device=device)
     if stream_ptr is not None and stream_ptr != _current_stream():
-        ws.record_stream(torch.cuda.ExternalStream(stream_ptr))
+        ws.record_stream(T.cuda.ExternalStream(stream_ptr))
     return ws, n
 
 
@@ -464,21 +476,20 @@ def token_logprobs(logits, targets, logprob, *, lse=None, entropy=None, top_ids=
     """logprob[r] = log softmax(logits[r] / temperature)[targets[r]] (int64; below 0: no target, 0), log-sum-exp
     and entropy of each row (float32), and the columns (int64) and log-probabilities of its k largest
     logits, k the width of top_ids, at most 64. targets and logprob may be None together."""
-    import torch
-
+    T = _types()
     dt, rows, cols, ld = _matrix("token_logprobs", logits)
     if (targets is None) != (logprob is None) or (top_ids is None) != (top_logprobs is None):
         _refuse("token_logprobs: targets and logprob, and top_ids and top_logprobs, are given together")
     k = 0
     if top_ids is not None:
         k = top_ids.shape[-1] if top_ids.dim() == 2 else -1
-        _expect("token_logprobs: top_ids", top_ids, torch.int64, (rows, k))
-        _expect("token_logprobs: top_logprobs", top_logprobs, torch.float32, (rows, k))
+        _expect("token_logprobs: top_ids", top_ids, T.int64, (rows, k))
+        _expect("token_logprobs: top_logprobs", top_logprobs, T.float32, (rows, k))
     if targets is not None:
-        _expect("token_logprobs: targets", targets, torch.int64, (rows,))
+        _expect("token_logprobs: targets", targets, T.int64, (rows,))
     for what, t in (("logprob", logprob), ("lse", lse), ("entropy", entropy)):
         if t is not None:
-            _expect("token_logprobs: " + what, t, torch.float32, (rows,))
+            _expect("token_logprobs: " + what, t, T.float32, (rows,))
     _device_of(logits, targets, logprob, lse, entropy, top_ids, top_logprobs)
     ws, n = _logits_workspace(rows, cols, k, logits.device, stream_ptr)
     _dispatch(stream_ptr, "gn_token_logprobs", dt, _ptr(logits), rows, cols, ld, temperature, _ptr(targets),
@@ -489,8 +500,7 @@ def token_logprobs_backward(logits, targets, lse, grad_logprob, grad_logits, *, 
                             temperature=1.0, stream_ptr=None):
     """The gradient of the logits (their type; may be the logits themselves) from those of logprob and, with
     the forward's entropy, of the entropy."""
-    import torch
-
+    T = _types()
     dt, rows, cols, ld = _matrix("token_logprobs_backward", logits)
     dg, grows, gcols, ldg = _matrix("token_logprobs_backward: grad_logits", grad_logits)
     if (dg, grows, gcols) != (dt, rows, cols):
@@ -498,10 +508,10 @@ def token_logprobs_backward(logits, targets, lse, grad_logprob, grad_logits, *, 
     if (targets is None) != (grad_logprob is None) or (entropy is None) != (grad_entropy is None):
         _refuse("token_logprobs_backward: targets and grad_logprob, and entropy and grad_entropy, are given together")
     if targets is not None:
-        _expect("token_logprobs_backward: targets", targets, torch.int64, (rows,))
+        _expect("token_logprobs_backward: targets", targets, T.int64, (rows,))
     for what, t in (("lse", lse), ("grad_logprob", grad_logprob), ("entropy", entropy), ("grad_entropy", grad_entropy)):
         if t is not None:
-            _expect("token_logprobs_backward: " + what, t, torch.float32, (rows,))
+            _expect("token_logprobs_backward: " + what, t, T.float32, (rows,))
     _device_of(logits, targets, lse, grad_logprob, grad_logits, entropy, grad_entropy)
     _dispatch(stream_ptr, "gn_token_logprobs_backward", dt, _ptr(logits), rows, cols, ld, temperature, _ptr(targets),
               _ptr(lse), _ptr(entropy), _ptr(grad_logprob), _ptr(grad_entropy), _ptr(grad_logits), ldg)
@@ -511,15 +521,14 @@ def distill(logits, ids, teacher, loss, *, lse=None, temperature=1.0, stream_ptr
     """loss[r] = temperature^2 KL(teacher || student) with the teacher's softmax over its entries ids[r] (int64, below 0:
     absent), teacher[r] (float32 logits or log-probabilities), at most 256 of them, and the student's
     over all columns of logits[r]; lse: the student's log-sum-exp."""
-    import torch
-
+    T = _types()
     dt, rows, cols, ld = _matrix("distill", logits)
     k = ids.shape[-1] if ids.dim() == 2 else -1
-    _expect("distill: ids", ids, torch.int64, (rows, k))
-    _expect("distill: teacher", teacher, torch.float32, (rows, k))
+    _expect("distill: ids", ids, T.int64, (rows, k))
+    _expect("distill: teacher", teacher, T.float32, (rows, k))
     for what, t in (("loss", loss), ("lse", lse)):
         if t is not None:
-            _expect("distill: " + what, t, torch.float32, (rows,))
+            _expect("distill: " + what, t, T.float32, (rows,))
     _device_of(logits, ids, teacher, loss, lse)
     ws, n = _logits_workspace(rows, cols, 0, logits.device, stream_ptr)
     _dispatch(stream_ptr, "gn_distill_forward", dt, _ptr(logits), rows, cols, ld, temperature, _ptr(ids), _ptr(teacher),
@@ -528,17 +537,16 @@ def distill(logits, ids, teacher, loss, *, lse=None, temperature=1.0, stream_ptr
 
 def distill_backward(logits, ids, teacher, lse, grad_loss, grad_logits, *, temperature=1.0, stream_ptr=None):
     """The gradient of the logits (their type; may be the logits themselves) from that of distill's loss."""
-    import torch
-
+    T = _types()
     dt, rows, cols, ld = _matrix("distill_backward", logits)
     dg, grows, gcols, ldg = _matrix("distill_backward: grad_logits", grad_logits)
     if (dg, grows, gcols) != (dt, rows, cols):
         _refuse("distill_backward: grad_logits has the type and shape of logits")
     k = ids.shape[-1] if ids.dim() == 2 else -1
-    _expect("distill_backward: ids", ids, torch.int64, (rows, k))
-    _expect("distill_backward: teacher", teacher, torch.float32, (rows, k))
-    _expect("distill_backward: lse", lse, torch.float32, (rows,))
-    _expect("distill_backward: grad_loss", grad_loss, torch.float32, (rows,))
+    _expect("distill_backward: ids", ids, T.int64, (rows, k))
+    _expect("distill_backward: teacher", teacher, T.float32, (rows, k))
+    _expect("distill_backward: lse", lse, T.float32, (rows,))
+    _expect("distill_backward: grad_loss", grad_loss, T.float32, (rows,))
     _device_of(logits, ids, teacher, lse, grad_loss, grad_logits)
     _dispatch(stream_ptr, "gn_distill_backward", dt, _ptr(logits), rows, cols, ld, temperature, _ptr(ids),
               _ptr(teacher), k, _ptr(lse), _ptr(grad_loss), _ptr(grad_logits), ldg)
