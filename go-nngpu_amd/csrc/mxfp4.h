@@ -20,8 +20,8 @@ __host__ __device__ inline unsigned block_scale(uint32_t top) {
   return (unsigned)(field > 2 ? field - 2 : 0);
 }
 
-// Whether every code times 2^(e - 127) is a normal fp16 value or zero: 0.5 2^-13 to 6 2^13.
-__host__ __device__ inline bool half_exact(unsigned e) { return e >= 114 && e <= 140; }
+// Whether every code times 2^(e - 127) is an fp16 value: 0.5 2^-23 (the smallest subnormal one) to 6 2^13.
+__host__ __device__ inline bool half_exact(unsigned e) { return e >= 104 && e <= 140; }
 
 struct MxGemmDesc {
   int a_dtype;

@@ -8,16 +8,14 @@
 namespace gn {
 namespace {
 
-constexpr long kMaxK = 1L << 23;  // 256 rows of codes stay below 2^30 bytes: 32-bit offsets within a tile
+// 256 rows of codes, and of fp16 activations, stay below 2^31 bytes: 32-bit offsets within a tile.
+constexpr long kMaxK = 1L << 22;
 
 typedef int i32x8_t __attribute__((ext_vector_type(8)));
 typedef float float16_t __attribute__((ext_vector_type(16)));
 typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
-
-// 2^(E - 127); NaN for 255.
-__device__ __forceinline__ float scale_of(unsigned e) {
-  return __uint_as_float((e << 23) | ((e == 0 || e == 255) ? 0x00400000u : 0u));
-}
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 
 struct MxParams : GemmParams {
   const uint8_t *as, *bs;  // scales
@@ -43,6 +41,35 @@ __device__ __forceinline__ half8_t half8_of(uint32_t w, float unit) {
   const half2_t c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, unit, 2);
   const half2_t d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, unit, 3);
   return half8_t{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+// Where a scale would take the weights out of fp16's normal range, the products go through bf16, whose range is
+// fp32's: a code times any 2^(E - 127) is a bf16 number (down to 2^-128, a subnormal one), and an fp16 number is exactly
+// the sum of two. Twice the matrix instructions, the same accumulators, every product still exact.
+__device__ __forceinline__ bf16x8_t bf16x8_of(uint32_t w, unsigned e) {
+  const float unit = __uint_as_float(e << 23);
+  const bf16x2_t a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, unit, 0);
+  const bf16x2_t b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, unit, 1);
+  const bf16x2_t c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, unit, 2);
+  const bf16x2_t d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, unit, 3);
+  const bf16x8_t v = {a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+  const u32x4_t nan = {0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u};
+  return e == 255 ? __builtin_bit_cast(bf16x8_t, nan) : v;
+}
+// c + A B^T of an fp16 A, as its upper 8 bits and the rest (0 for infinities and NaN).
+__device__ __forceinline__ float4_t mfma_halves_bf16(half8_t a, bf16x8_t b, float4_t c) {
+  u32x4_t hi, lo;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float x = (float)a[2 * i], y = (float)a[2 * i + 1];
+    const uint32_t xh = __float_as_uint(x) & 0xffff0000u, yh = __float_as_uint(y) & 0xffff0000u;
+    const float xl = copysignf(fmaxf(fabsf(x - __uint_as_float(xh)), 0.0f), x);  // NaN to 0
+    const float yl = copysignf(fmaxf(fabsf(y - __uint_as_float(yh)), 0.0f), y);
+    hi[i] = xh >> 16 | yh;
+    lo[i] = __float_as_uint(xl) >> 16 | (__float_as_uint(yl) & 0xffff0000u);
+  }
+  c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, hi), b, c, 0, 0, 0);
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, lo), b, c, 0, 0, 0);
 }
 
 __device__ __forceinline__ float finish(const MxParams &p, float acc, long m, long n) {
@@ -129,9 +156,7 @@ __global__ void __launch_bounds__(512) mx_fp4_rows_kernel(MxParams p) {
 // NF blocks of columns. The next slab's A and B are on their way while one is multiplied. The lane's 32 weights become
 // four fragments of v_mfma_f32_16x16x32_f16 whose k are 8 j .. 8 j + 7 of each lane's own block, and A's lanes read the same.
 // Where the scales of a wave's blocks all keep the weights normal fp16 numbers (half_exact; weights of ordinary size do) the
-// conversion applies them, exactly. Otherwise the codes are converted as they are, one block of 32 goes through the matrix
-// core at a time (the other lanes' operands 0, on both sides: a 0 weight must not meet another block's infinity), and its
-// sum is scaled in fp32.
+// conversion applies them, exactly; otherwise both sides go through bf16.
 // Read from the caches by every wave instead of through LDS, A took as long as B and more (4096 -> 11008, fp16 against
 // 4-bit activations: 1 row 12.4 against 9.7 us, 16 rows 20 against 14, 64 rows 42 against 25).
 // R: the rows of LDS that there may be, 16 MF or fewer.
@@ -219,23 +244,17 @@ __global__ void __launch_bounds__(WK * WN * 64) mx_half_rows_kernel(MxParams p, 
           }
         }
       } else {
-        const half8_t z = {0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
-        for (int j = 0; j < NF; ++j)
+        for (int k = 0; k < 4; ++k)
 #pragma unroll
-          for (int i = 0; i < MF; ++i)
-#pragma unroll 1
-            for (int q = 0; q < 4; ++q) {
-              float4_t part = {0, 0, 0, 0};
+          for (int j = 0; j < NF; ++j) {
+            const bf16x8_t w = bf16x8_of(bq[e][u][j][k], (bsc[e][u][j] >> (8 * g)) & 255);
 #pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                const half8_t a = *reinterpret_cast<const half8_t *>(slab + arow[i] + u * kGroup + 8 * k);
-                part = __builtin_amdgcn_mfma_f32_16x16x32_f16(g == q ? a : z, g == q ? half8_of(bq[e][u][j][k], 1.0f) : z, part, 0, 0, 0);
-              }
-              const float unit = scale_of((bsc[e][u][j] >> (8 * q)) & 255);
-#pragma unroll
-              for (int x = 0; x < 4; ++x) acc[j][i][x] = fmaf(part[x], unit, acc[j][i][x]);
+            for (int i = 0; i < MF; ++i) {
+              acc[j][i] = mfma_halves_bf16(*reinterpret_cast<const half8_t *>(slab + arow[i] + u * kGroup + 8 * k), w, acc[j][i]);
+              __builtin_amdgcn_sched_barrier(0);  // one product's operands in registers at a time
             }
+          }
       }
     }
   };
@@ -445,6 +464,281 @@ mx_fp4_kernel(MxParams p) {
   });
 }
 
+// ------------------------------------------------------------------ fp16 activations, many rows
+// C = A B^T on v_mfma_f32_16x16x32_f16, the weights converted in registers. WM x WN waves, each FM x FN blocks of 16 x 16;
+// K in stages of 64, NS of them in LDS: 128 bytes of A to a row (ring_plan.h's plan and swizzle) and 32 of codes. Lane (r,
+// g) takes k = 16 g .. 16 g + 15 of the stage on both sides, 8 in each of two steps, so its 16 codes are 8 consecutive bytes (a
+// wave's read of 16 rows is 512 consecutive ones) and lie in one block. A row's scales for 8 stages are 16 bytes in LDS. The
+// scales are applied as in the few-rows kernel: in fp16 where all of the wave's allow it, else in bf16.
+// DMA: A is copied to LDS by dma16 (16-byte aligned rows, K a multiple of 8); otherwise through registers, its tail masked.
+template <int WM, int WN, int FM, int FN, int NS>
+struct HalfTile {
+  static constexpr int BM = WM * FM * 16, BN = WN * FN * 16;
+  static constexpr int STAGE = BM * 128 + BN * 32, SCALES = BN * 16, SPARE = BN / 32 % (WM * WN) ? 1024 : 0;
+  static constexpr int LDS = NS * STAGE + 2 * SCALES + SPARE, EPI = WM * 16 * (BN + 4) * 4;
+  static constexpr int BYTES = LDS > EPI ? LDS : EPI;
+};
+
+// The tile in fp16 (PLAIN) or bf16. With CHECK it looks at its scales on the way, and returns with nothing written where fp16
+// did not do; otherwise the wave ends. A branch to the other form in each stage, or after the first one that needs it, had the
+// compiler move all accumulators between registers (4096 -> 11008, 512 rows: 72 us against 63).
+template <int WM, int WN, int FM, int FN, int NS, bool DMA, bool PLAIN, bool CHECK>
+__device__ __forceinline__ void half_tile(const MxParams &p, char *smem, int tm, int tn, int tid) {
+  constexpr int NW = WM * WN, BM = WM * FM * 16, BN = WN * FN * 16;
+  constexpr int CA = BM / 8 / NW, NB = BN / 32, CB = (NB + NW - 1) / NW;  // 1 KiB chunks of A to a wave; of B, and to a wave
+  constexpr int SB = BN / 64;
+  using Tile = HalfTile<WM, WN, FM, FN, NS>;
+  constexpr int STAGE = Tile::STAGE, SCALES = Tile::SCALES, LDS = Tile::LDS;
+  static_assert(CA * NW * 8 == BM && CA % 2 == 0 && BN % 64 == 0 && SB <= NW, "chunks");
+  const long m0 = (long)tm * BM, n0 = (long)tn * BN;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  const int wm = wave / WN, wn = wave % WN, r = lane & 15, g = lane >> 4;
+  const unsigned pitch = 64u * (unsigned)p.G, spitch = 4u * (unsigned)p.G;
+  const int ns = (int)((p.K + 63) / 64);
+  const unsigned lds = lds_offset(smem);
+
+  // A: lane L of chunk c copies octet kc8_octet(row, L & 7) of row 8 c + L / 8.
+  const char *a0 = static_cast<const char *>(p.A) + m0 * p.lda * 2, *b0 = static_cast<const char *>(p.B) + n0 * pitch;
+  unsigned va[CA], vb[CB];
+  // The copy's first k in the stage, for even i; for odd i the octet's upper bit is the other way round (row >> 1 is 4 more).
+  const int ka = 8 * kc8_octet(8 * wave * CA + (lane >> 3), lane & 7);
+  auto k_of = [&](int i) { return ka ^ (i & 1 ? 32 : 0); };
+#pragma unroll
+  for (int i = 0; i < CA; ++i) {
+    const int row = 8 * (wave * CA + i) + (lane >> 3), o = kc8_octet(row, lane & 7);
+    va[i] = m0 + row < p.M ? (unsigned)(row * p.lda * 2 + 16 * o) : kOutOfRange;
+  }
+#pragma unroll
+  for (int i = 0; i < CB; ++i) {
+    const int row = 32 * (wave + i * NW) + (lane >> 1);
+    // A wave without a chunk copies zeros to a place of its own: every wave has as many copies in flight.
+    vb[i] = row < BN && n0 + row < p.N ? row * pitch + 16 * (lane & 1) : kOutOfRange;
+  }
+  unsigned sl[NS];  // the slots of stages t, t + 1, ..
+#pragma unroll
+  for (int i = 0; i < NS; ++i) sl[i] = i * STAGE;
+  auto issue = [&](int t, unsigned slot) {  // past the last stage all reads are zeros
+    const int left = (int)p.K - 64 * t;
+    const unsigned st = lds + slot;
+    if constexpr (DMA) {
+      BufRsrc da = make_rsrc(a0 + 128L * t);
+      if (left >= 64) {
+#pragma unroll
+        for (int i = 0; i < CA; ++i) dma16(da, va[i], __builtin_amdgcn_readfirstlane(st + (wave * CA + i) * 1024));
+      } else {
+#pragma unroll
+        for (int i = 0; i < CA; ++i)
+          dma16(da, k_of(i) < left ? va[i] : kOutOfRange, __builtin_amdgcn_readfirstlane(st + (wave * CA + i) * 1024));
+      }
+    }
+    BufRsrc db = make_rsrc(b0 + 32L * t);
+    db.r.z = __builtin_amdgcn_readfirstlane(left > 0 ? (int)ring::kNumRecords : 0);
+#pragma unroll
+    for (int i = 0; i < CB; ++i)
+      dma16(db, vb[i], __builtin_amdgcn_readfirstlane(wave + i * NW < NB ? st + BM * 128 + (wave + i * NW) * 1024 : lds + LDS - 1024));
+  };
+  half8_t ar[DMA ? 1 : CA];
+  auto load_a = [&](int t) {  // A's part of issue(), to registers
+    const long left = p.K - 64L * t;
+#pragma unroll
+    for (int i = 0; i < CA; ++i) {
+      ar[DMA ? 0 : i] = half8_t{0, 0, 0, 0, 0, 0, 0, 0};
+      const _Float16 *a = reinterpret_cast<const _Float16 *>(a0 + 128L * t + va[i]);
+      if (va[i] != kOutOfRange) {
+        if (k_of(i) + 8 <= left) {
+          ar[DMA ? 0 : i] = reinterpret_cast<const UnalignedHalf8 *>(a)->v;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (k_of(i) + e < left) ar[DMA ? 0 : i][e] = a[e];
+        }
+      }
+    }
+  };
+  auto store_a = [&](unsigned slot) {
+    char *st = smem + slot;
+#pragma unroll
+    for (int i = 0; i < CA; ++i) *reinterpret_cast<half8_t *>(st + (wave * CA + i) * 1024 + lane * 16) = ar[DMA ? 0 : i];
+  };
+  const long s_rows = min(p.N - n0, (long)BN);
+  auto issue_scales = [&](int c) {  // of stages 8 c .. 8 c + 7; bytes past a row's end are another row's, not used
+    if (wave < SB) {
+      const int row = min(64 * wave + lane, (int)s_rows - 1);  // past the matrix the last row's, against zeros
+      BufRsrc ds = make_rsrc(p.bs + n0 * spitch);
+      ds.r.z = __builtin_amdgcn_readfirstlane((int)(s_rows * spitch));
+      dma16(ds, 4 * c < p.G ? row * spitch + 16 * c : kOutOfRange,
+            __builtin_amdgcn_readfirstlane(lds + NS * STAGE + (c & 1) * SCALES + wave * 1024));
+    }
+  };
+
+  half8_t fa[FM];
+  u32x2_t bq[FN];
+  unsigned be[FN];  // scale bytes
+  const unsigned arow = (wm * FM * 16 + r) * 128, asw = (2 * g) ^ ((r >> 1) & 7);
+  auto read_a = [&](unsigned slot, int s, int i) {
+    return *reinterpret_cast<const half8_t *>(smem + slot + arow + i * 2048 + ((asw ^ s) << 4));
+  };
+  auto scale_at = [&](int t, int j) {
+    return smem + NS * STAGE + ((t >> 3) & 1) * SCALES + ((wn * FN + j) * 16 + r) * 16 + 2 * (t & 7);
+  };
+  auto read_b = [&](int t, unsigned slot) {
+    const char *st = smem + slot + BM * 128 + (wn * FN * 16 + r) * 32 + 8 * g;
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+      bq[j] = *reinterpret_cast<const u32x2_t *>(st + j * 512);
+      be[j] = *reinterpret_cast<const uint8_t *>(scale_at(t, j) + (g >> 1));
+    }
+  };
+  float4_t acc[FM][FN];
+#pragma unroll
+  for (int i = 0; i < FM; ++i)
+#pragma unroll
+    for (int j = 0; j < FN; ++j) acc[i][j] = float4_t{0.f, 0.f, 0.f, 0.f};
+
+  // The step's products, row by row; each fragment of A is read anew, into the same registers, once it has been used. In fp16
+  // the other step's weights are converted on the way (from row `from` on), in bf16 this one's before.
+  u32x4_t w[PLAIN ? 2 : 1][FN];
+  bool fits = true;
+  auto check = [&] {
+#pragma unroll
+    for (int j = 0; j < FN; ++j) fits &= half_exact(be[j]);
+  };
+  auto weight = [&](int s, int j) {
+    if constexpr (PLAIN)
+      w[s][j] = __builtin_bit_cast(u32x4_t, half8_of(bq[j][s], __uint_as_float(be[j] << 23)));
+    else
+      w[0][j] = __builtin_bit_cast(u32x4_t, bf16x8_of(bq[j][s], be[j]));
+  };
+  auto multiply = [&](auto step, unsigned slot, int from) {
+    constexpr int S = decltype(step)::value;
+    if constexpr (!PLAIN) {
+#pragma unroll
+      for (int j = 0; j < FN; ++j) weight(S, j);
+    }
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+#pragma unroll
+      for (int j = 0; j < FN; ++j) {
+        if constexpr (PLAIN) {
+          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fa[i], __builtin_bit_cast(half8_t, w[S][j]), acc[i][j], 0, 0, 0);
+        } else {
+          acc[i][j] = mfma_halves_bf16(fa[i], __builtin_bit_cast(bf16x8_t, w[0][j]), acc[i][j]);
+          __builtin_amdgcn_sched_barrier(0);  // one product's operands in registers at a time
+        }
+      }
+      fa[i] = read_a(slot, 1 - S, i);
+      if constexpr (PLAIN) {
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+          if (from + j * (FM - from) / FN == i) weight(1 - S, j);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+
+  issue_scales(0);
+#pragma unroll
+  for (int i = 0; i < NS; ++i) issue(i, sl[i]);
+  if constexpr (!DMA) {
+#pragma unroll
+    for (int i = 0; i < NS - 1; ++i) {
+      load_a(i);
+      store_a(sl[i]);
+    }
+    load_a(NS - 1);
+  }
+  __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+  __syncthreads();
+  read_b(0, sl[0]);
+#pragma unroll
+  for (int i = 0; i < FM; ++i) fa[i] = read_a(sl[0], 0, i);
+  if constexpr (PLAIN) {
+#pragma unroll
+    for (int j = 0; j < FN; ++j) weight(0, j);
+  }
+  for (int t = 0; t < ns; ++t) {
+    if constexpr (CHECK) check();
+    multiply(ActCode<0>{}, sl[0], 0);
+    // All but the copies of stage t + 2 and later are done: stage t + 1 is there.
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm(DMA ? (NS - 2) * (CA + CB) : 0));
+    __syncthreads();
+    if ((t & 7) == 0) issue_scales(t / 8 + 1);
+    if constexpr (!DMA) {
+      store_a(sl[NS - 1]);
+      load_a(t + NS);
+    }
+    issue(t + NS, sl[0]);
+    // Past the last stage zeros, and scales that are not looked at.
+    if constexpr (PLAIN) read_b(t + 1, sl[1]);
+    multiply(ActCode<1>{}, sl[1], FM / 2);
+    if constexpr (!PLAIN) read_b(t + 1, sl[1]);
+    const unsigned s = sl[0];
+#pragma unroll
+    for (int i = 0; i < NS - 1; ++i) sl[i] = sl[i + 1];
+    sl[NS - 1] = s;
+  }
+  __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+  // No copy is under way and all waves are done with the slots: the epilogue takes their place.
+  if constexpr (CHECK) {
+    if (__builtin_amdgcn_readfirstlane(__syncthreads_or(!fits))) return;
+  } else {
+    __syncthreads();
+  }
+  // What only the epilogue needs of the arguments is read again: kept through the loop it takes scalar registers that the loop has not.
+  auto *args = (const CONST_AS MxParams *)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(args));
+  const MxParams e = *(const MxParams *)args;
+  store_tile_rows<BM, BN, WM, WN>(e, m0, n0, 0, reinterpret_cast<float *>(smem), acc);
+  if constexpr (CHECK) __builtin_amdgcn_endpgm();
+}
+
+// Whether fp16 does for the columns of a tile: all their scales, which lie one after the other.
+template <int NT, int BN>
+__device__ __forceinline__ bool scan_scales(const MxParams &p, int tn) {
+  const long n0 = (long)tn * BN, count = min(p.N - n0, (long)BN) * p.G;
+  const uint32_t *s = reinterpret_cast<const uint32_t *>(p.bs) + n0 * p.G;
+  bool fits = true;
+#pragma unroll 8
+  for (long i = threadIdx.x; i < count; i += NT) {
+    const uint32_t v = s[i];
+#pragma unroll
+    for (int k = 0; k < 32; k += 8) fits &= half_exact((v >> k) & 255);
+  }
+  return !__builtin_amdgcn_readfirstlane(__syncthreads_or(!fits));
+}
+
+template <int WM, int WN, int FM, int FN, int NS, int WPE, bool DMA>
+__global__ void __launch_bounds__(WM * WN * 64) __attribute__((amdgpu_waves_per_eu(WPE, WPE)))
+mx_half_kernel(MxParams p) {
+  __shared__ __attribute__((aligned(1024))) char smem[HalfTile<WM, WN, FM, FN, NS>::BYTES];
+  int tm, tn;
+  tile_coords(p, tm, tn);
+  // The tall tile looks at the scales first, 1% of its time: its accumulators leave no registers to keep through the other
+  // form's code, as the compiler does where that follows.
+  constexpr bool TALL = FM > 4;
+  bool fp16 = true;
+  if constexpr (TALL) fp16 = scan_scales<WM * WN * 64, HalfTile<WM, WN, FM, FN, NS>::BN>(p, tn);
+  if (fp16) {
+    half_tile<WM, WN, FM, FN, NS, DMA, true, !TALL>(p, smem, tm, tn, threadIdx.x);
+    if constexpr (TALL) return;
+  }
+  // bf16 takes more registers: a tall tile in two halves, with arguments (the kernel's, p is the only one) and addresses that
+  // the compiler does not keep from the first form.
+  constexpr int H = TALL ? 2 : 1;
+  auto *args = (const CONST_AS MxParams *)__builtin_amdgcn_kernarg_segment_ptr();
+  int tid = threadIdx.x;
+#pragma unroll 1
+  for (int h = 0; h < H; ++h) {
+    __syncthreads();
+    asm volatile("" : "+v"(tid), "+s"(args));
+    const MxParams q = *(const MxParams *)args;
+    int um, un;
+    tile_coords(q, um, un);
+    if ((long)(um * H + h) * (WM * FM / H * 16) < q.M)
+      half_tile<WM, WN, FM / H, FN, NS, DMA, false, false>(q, smem, um * H + h, un, tid);
+  }
+}
+
 unsigned grid_of(long n, long per) { return (unsigned)std::max(1L, std::min((n + per - 1) / per, 1L << 20)); }
 
 template <int WM, int WN, int FM, int FN, int WPE>
@@ -453,6 +747,32 @@ void launch_fp4(MxParams p, hipStream_t s) {
   p.tiles_m = (int)((p.M + BM - 1) / BM);
   p.tiles_n = (int)((p.N + BN - 1) / BN);
   hipLaunchKernelGGL((mx_fp4_kernel<WM, WN, FM, FN, WPE>), dim3((unsigned)(p.tiles_m * p.tiles_n)), dim3(WM * WN * 64), 0, s, p);
+}
+
+template <int WM, int WN, int FM, int FN, int NS, int WPE, bool DMA>
+void launch_half(MxParams p, hipStream_t s) {
+  constexpr int BM = WM * FM * 16, BN = WN * FN * 16;
+  p.tiles_m = (int)((p.M + BM - 1) / BM);
+  p.tiles_n = (int)((p.N + BN - 1) / BN);
+  hipLaunchKernelGGL((mx_half_kernel<WM, WN, FM, FN, NS, WPE, DMA>), dim3((unsigned)(p.tiles_m * p.tiles_n)), dim3(WM * WN * 64), 0, s, p);
+}
+
+// fp16 activations, more than 64 rows. 256 x 256 tiles where there is one for each CU (8192^3: 852 us, 128 x 128 1038),
+// then 128 x 128 (512 x 4096 -> 11008: 66 us, 64 x 128 69), 64 x 128 and 64 x 64 ones while those of the size before leave CUs without
+// one: a tile alone on a CU waits for its copies (256 x 4096 -> 11008: 128 x 128 48 us, 64 x 128 40; 128 x 4096 -> 4096: 48, 33,
+// 64 x 64 27). Rows of A that are not 16-byte aligned go through registers in 128 x 64 tiles.
+void launch_half_tiles(const MxParams &p, hipStream_t s) {
+  auto tiles = [&](long bm, long bn) { return ((p.M + bm - 1) / bm) * ((p.N + bn - 1) / bn); };
+  if ((uintptr_t)p.A % 16 != 0 || p.lda % 8 != 0 || p.K % 8 != 0)
+    launch_half<2, 2, 4, 2, 3, 2, false>(p, s);
+  else if (tiles(256, 256) >= 256)
+    launch_half<2, 4, 8, 4, 3, 2, true>(p, s);
+  else if (tiles(128, 128) >= 256)
+    launch_half<2, 2, 4, 4, 3, 2, true>(p, s);
+  else if (tiles(64, 128) >= 256)
+    launch_half<1, 4, 4, 2, 4, 2, true>(p, s);
+  else
+    launch_half<1, 4, 4, 1, 4, 3, true>(p, s);
 }
 
 template <int MF, int NF, int U>
@@ -528,6 +848,7 @@ int check_mxfp4_gemm(const MxGemmDesc &d, CError *err) {
   if (int rc = check_mxfp4_matrix("mxfp4 gemm: B", d.B, d.b_scales, d.N, d.K, err)) return rc;
   if (d.a_dtype == GN_MXFP4) return check_mxfp4_matrix("mxfp4 gemm: A", d.A, d.a_scales, d.M, d.K, err);
   if (d.a_scales) return set_error(err, -1, "mxfp4 gemm: scales given for an fp16 A");
+  if (d.lda > kMaxK && d.M > 1) return set_error(err, -1, "mxfp4 gemm: leading dimension %ld of A is too large", d.lda);
   return check_plain_matrix("mxfp4 gemm: A", GN_F16, d.A, d.M, d.K, d.lda, err);
 }
 
@@ -546,12 +867,15 @@ int launch_mxfp4_gemm(const MxGemmDesc &d, hipStream_t s, CError *err) {
   if (d.K == 0) {
     hipLaunchKernelGGL(mx_k0_kernel, dim3(grid_of(d.M * d.N, 256)), dim3(256), 0, s, p);
   } else {
-    if (d.a_dtype == GN_MXFP4 && d.M > 64 && d.M * d.N > (1L << 24))
+    const bool big = d.M * d.N > (1L << 24);
+    if (d.M <= 64)
+      launch_rows(d.a_dtype == GN_MXFP4, p, s);
+    else if (d.a_dtype == GN_MXFP4 && big)
       launch_fp4<2, 4, 4, 2, 2>(p, s);
-    else if (d.a_dtype == GN_MXFP4 && d.M > 64)
+    else if (d.a_dtype == GN_MXFP4)
       launch_fp4<2, 2, 2, 2, 2>(p, s);
     else
-      launch_rows(d.a_dtype == GN_MXFP4, p, s);
+      launch_half_tiles(p, s);
   }
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? 0 : hip_error(err, -6, "mxfp4 gemm launch", e);

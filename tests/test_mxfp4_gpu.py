@@ -168,6 +168,19 @@ def test_product_scales_over_the_whole_range(dev, M, N, K, fp4):
     _bounded(y.cpu(), a, R.values(*w, K), K)
 
 
+@pytest.mark.parametrize("M,N,K", [(1, 40, 256), (20, 600, 384), (70, 200, 512), (270, 300, 128), (3000, 5700, 64)])
+@pytest.mark.parametrize("lo,hi", [(104, 114), (114, 141), (137, 145), (100, 108)])
+def test_product_scales_at_the_ends_of_fp16(dev, M, N, K, lo, hi):
+    """Scales whose weights are all fp16 numbers, the subnormal ones included, and scales around both ends of that range."""
+    w, x = _weights(N, K, 25, lo, hi), _x(M, K, torch.float16, 26)
+    y = torch.empty((M, N), device=dev)
+    G.mxfp4_gemm(x.to(dev), tuple(t.to(dev) for t in w), y)
+    _bounded(y.cpu(), x.double(), R.values(*w, K), K)
+    w[1][N - 1, 1] = 3  # one block elsewhere
+    G.mxfp4_gemm(x.to(dev), tuple(t.to(dev) for t in w), y)
+    _bounded(y.cpu(), x.double(), R.values(*w, K), K)
+
+
 @pytest.mark.parametrize("fp4", [False, True])
 @pytest.mark.parametrize("M", [2, 200])
 def test_product_nan_and_inf(dev, M, fp4):
