@@ -2,7 +2,8 @@
 // alternatives, distillation from a teacher's top logits, and the gradients of the logits.
 //
 // With z = x / T, m = max z, s = sum e^(z - m) and t = sum (z - m) e^(z - m): lse = m + ln s and the entropy is
-// ln s - t / s, two terms that are never negative (no cancellation). All sums are fp32.
+// ln s - t / s, two terms that are never negative (no cancellation). All sums are fp32. Exponents are taken in base 2, of
+// (x - max x) c with the rounded c = log2(e) / T.
 //
 // All of it is bound by one pass over the logits (and one over the gradients). A workgroup takes a segment of a
 // row, up to 8192 logits, in one go into registers: all loads are in flight together, the maximum is known before the
@@ -18,11 +19,10 @@ namespace gn {
 namespace {
 
 constexpr int kThreads = 256, kWaves = kThreads / 64;
-constexpr float kLog2e = 1.44269504088896340736f;
-constexpr float kFloor = -200.0f;  // e^x is 0 in fp32 from here down: stands in for -inf where that meets a 0
+constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
+constexpr float kFloor = -300.0f;  // 2^x is 0 in fp32 from here down: stands in for -inf where that meets a 0
 
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
-typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
 
 // ------------------------------------------------------------------ a segment in registers
 // 16 bytes at any address that is a multiple of T's size (the hardware takes unaligned vectors).
@@ -33,69 +33,56 @@ struct __attribute__((packed, aligned(sizeof(T)))) Unaligned16 {
 template <typename T>
 constexpr int kVec = 16 / (int)sizeof(T);
 
-__device__ __forceinline__ void unpack(u32x4_t a, float (&v)[4]) {
-#pragma unroll
-  for (int j = 0; j < 4; ++j) v[j] = __uint_as_float(a[j]);
-}
-__device__ __forceinline__ void unpack(u32x4_t a, float (&v)[8]) {
-  const half8_t h = __builtin_bit_cast(half8_t, a);
-#pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = (float)h[j];
-}
-
 // Value e of a thread is the segment's number position<T>(e).
 template <typename T>
 __device__ __forceinline__ int position(int e) {
   return (e / kVec<T> * kThreads + (int)threadIdx.x) * kVec<T> + e % kVec<T>;
 }
 
-// E values of the `left` at x, -inf past them.
+// A thread's E values of a segment, in their own type.
 template <typename T, int E>
-__device__ __forceinline__ void load_segment(const T *x, int left, float (&v)[E]) {
-  constexpr int V = kVec<T>;
-#pragma unroll
-  for (int i = 0; i < E / V; ++i) {
-    const int at = position<T>(i * V);
-    float u[V];
-    if (at + V <= left) {
-      unpack(reinterpret_cast<const Unaligned16<T> *>(x + at)->v, u);
-    } else {
-#pragma unroll
-      for (int j = 0; j < V; ++j) u[j] = at + j < left ? (float)x[at + j] : -INFINITY;
-    }
-#pragma unroll
-    for (int j = 0; j < V; ++j) v[i * V + j] = u[j];
-  }
-}
+struct Segment {
+  typedef T V __attribute__((ext_vector_type(kVec<T>)));
+  V v[E / kVec<T>];
+  __device__ __forceinline__ float operator[](int e) const { return (float)v[e / kVec<T>][e % kVec<T>]; }
 
-__device__ __forceinline__ u32x4_t pack(const float (&v)[4]) {
-  return u32x4_t{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
-}
-__device__ __forceinline__ u32x4_t pack(const float (&v)[8]) {
-  half8_t h;
+  // The `left` values at x, -inf past them.
+  __device__ __forceinline__ void load(const T *x, int left) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) h[j] = (_Float16)v[j];
-  return __builtin_bit_cast(u32x4_t, h);
-}
-
-template <typename T, int E>
-__device__ __forceinline__ void store_segment(T *g, int left, const float (&v)[E]) {
-  constexpr int V = kVec<T>;
+    for (int i = 0; i < E / kVec<T>; ++i) {
+      const int at = position<T>(i * kVec<T>);
+      if (at + kVec<T> <= left) {
+        v[i] = __builtin_bit_cast(V, reinterpret_cast<const Unaligned16<T> *>(x + at)->v);
+      } else {
 #pragma unroll
-  for (int i = 0; i < E / V; ++i) {
-    const int at = position<T>(i * V);
-    if (at + V <= left) {
-      float u[V];
-#pragma unroll
-      for (int j = 0; j < V; ++j) u[j] = v[i * V + j];
-      reinterpret_cast<Unaligned16<T> *>(g + at)->v = pack(u);
-    } else {
-#pragma unroll
-      for (int j = 0; j < V; ++j)
-        if (at + j < left) g[at + j] = (T)v[i * V + j];
+        for (int j = 0; j < kVec<T>; ++j) v[i][j] = at + j < left ? x[at + j] : (T)-INFINITY;
+      }
     }
   }
-}
+  __device__ __forceinline__ void store(T *g, int left) const {
+#pragma unroll
+    for (int i = 0; i < E / kVec<T>; ++i) {
+      const int at = position<T>(i * kVec<T>);
+      if (at + kVec<T> <= left) {
+        reinterpret_cast<Unaligned16<T> *>(g + at)->v = __builtin_bit_cast(u32x4_t, v[i]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < kVec<T>; ++j)
+          if (at + j < left) g[at + j] = v[i][j];
+      }
+    }
+  }
+  // Of the numbers among them (fp16: two to an instruction), -inf without any.
+  __device__ __forceinline__ float max_value() const {
+    V m = v[0];
+#pragma unroll
+    for (int i = 1; i < E / kVec<T>; ++i) m = __builtin_elementwise_max(m, v[i]);
+    float r = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < kVec<T>; ++j) r = fmaxf(r, (float)m[j]);
+    return r;
+  }
+};
 
 // ------------------------------------------------------------------ reductions
 // Over the workgroup's threads; every thread gets the result. red: one value for each wave.
@@ -118,42 +105,51 @@ __device__ __forceinline__ float block_sum(float v, float *red) {
   return block_all(v, red, [](float a, float b) { return a + b; });
 }
 
+// m: the largest x; s: the sum of 2^d, d = (x - m) c; t: that of d 2^d.
 struct RowStats {
-  float m, s, t;  // max z; sums of e^(z - m) and (z - m) e^(z - m)
+  float m, s, t;
 };
 
-// e^d. The argument is rounded once (2^-24 |d| relative in the result), results below 2^-126 are 0.
-__device__ __forceinline__ float exp_of(float d) { return __builtin_amdgcn_exp2f(d * kLog2e); }
+__device__ __forceinline__ float exp2_of(float d) { return __builtin_amdgcn_exp2f(d); }  // results below 2^-126 are 0
 
-template <int E>
-__device__ __forceinline__ RowStats segment_stats(const float (&x)[E], float inv_t, float *red) {
-  RowStats r{-INFINITY, 0.0f, 0.0f};
-#pragma unroll
-  for (int e = 0; e < E; ++e) r.m = fmaxf(r.m, x[e] * inv_t);
-  r.m = block_max(r.m, red);
-  const float m = r.m == -INFINITY ? 0.0f : r.m;  // a row of -inf: all terms e^-inf = 0
+// T: with t.
+template <bool T, typename S, int E>
+__device__ __forceinline__ RowStats segment_stats(const Segment<S, E> &x, float c, float *red) {
+  RowStats r{block_max(x.max_value(), red), 0.0f, 0.0f};
+  const float m = r.m == -INFINITY ? 0.0f : r.m;  // a segment of -inf: all terms 2^-inf = 0
+  const float mc = m * c;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    const float d = x[e] * inv_t - m, p = exp_of(d);
+    // fp16: one fma, as it is bound by its instructions, each d too large by what rounding m c lost; fp32: the lowest value times
+    // c would be -inf.
+    const float d = sizeof(S) == 2 ? fmaf(x[e], c, -mc) : (x[e] - m) * c, p = exp2_of(d);
     r.s += p;
-    r.t += p * fmaxf(d, kFloor);  // 0 where p is 0 and d is -inf; NaN where p is
+    if (T) r.t += p * fmaxf(d, kFloor);  // 0 where p is 0 and d is -inf; NaN where p is
   }
   r.s = block_sum(r.s, red);
-  r.t = block_sum(r.t, red);
+  if (T) r.t = block_sum(r.t, red);
+  if (sizeof(S) == 2) {
+    const float lost = fmaf(m, c, -mc);
+    r.s *= exp2_of(-lost);
+    if (T) r.t = r.t * exp2_of(-lost) - lost * r.s;
+  }
   return r;
 }
-__device__ __forceinline__ float lse_of(const RowStats &r) { return r.s == 0.0f ? -INFINITY : r.m + logf(r.s); }
-__device__ __forceinline__ float entropy_of(const RowStats &r) { return r.s == 0.0f ? 0.0f : logf(r.s) - r.t / r.s; }
-__device__ __forceinline__ float logprob_of(float z, float lse) { return lse == -INFINITY ? -INFINITY : z - lse; }
+__device__ __forceinline__ float lse_of(const RowStats &r, float inv_t) { return r.s == 0.0f ? -INFINITY : fmaf(r.m, inv_t, log2f(r.s) * kLn2); }
+__device__ __forceinline__ float entropy_of(const RowStats &r) { return r.s == 0.0f ? 0.0f : (log2f(r.s) - r.t / r.s) * kLn2; }
+// Of x, from its distance to the maximum: lse may be too large to hold ln s beside it.
+__device__ __forceinline__ float logprob_of(float x, const RowStats &r, float inv_t) {
+  return r.s == 0.0f ? -INFINITY : fmaf(x - r.m, inv_t, -log2f(r.s) * kLn2);
+}
 
 // a and b as of one row (b the later segment).
-__device__ __forceinline__ RowStats join_stats(const RowStats &a, const RowStats &b) {
+__device__ __forceinline__ RowStats join_stats(const RowStats &a, const RowStats &b, float c) {
   const float m = fmaxf(a.m, b.m), n = m == -INFINITY ? 0.0f : m;
-  const float da = fmaxf(a.m - n, kFloor), db = fmaxf(b.m - n, kFloor);  // a segment of -inf has s = t = 0
-  const float ea = exp_of(da), eb = exp_of(db);
+  const float da = fmaxf((a.m - n) * c, kFloor), db = fmaxf((b.m - n) * c, kFloor);  // a segment of -inf has s = t = 0
+  const float ea = exp2_of(da), eb = exp2_of(db);
+  // A NaN among the logits is in s, and so is +inf (inf - inf); m does not show NaN.
   RowStats r{m, a.s * ea + b.s * eb, 0.0f};
   r.t = (a.s == 0.0f ? 0.0f : ea * (a.t + da * a.s)) + (b.s == 0.0f ? 0.0f : eb * (b.t + db * b.s));
-  // A NaN among the logits is in s, and so is +inf (inf - inf); m does not show NaN.
   return r;
 }
 
@@ -183,32 +179,58 @@ __device__ __forceinline__ uint32_t wave_kth(uint32_t v, int k) {
   return t;
 }
 
-constexpr int kCandidates = 1024;
+constexpr int kCandidates = 1024;                    // of a segment
+constexpr int kJoined = kTopMax * (kTopMax + 1);     // of some segments of a row and the best of those before
 
+template <int N>
 struct TopShared {
-  uint64_t key[kCandidates], bound[kWaves];
+  uint64_t key[N + 8], bound[kWaves];
   int count;
 };
 
-// Writes the k largest of n keys in sh.key to out, in order; 0 where there are fewer. Each key's place is the number of
-// larger ones (no two are equal).
-__device__ __forceinline__ void write_ranked(const TopShared &sh, int n, int k, uint64_t *out) {
+// A key that at least k of the workgroup's values reach (some of its threads have one each, no two equal, 0 none):
+// each of the `waves` first waves finds the one that ceil(k / waves) of its own reach, and the smallest of these is reached by
+// k. About 1.5 k values of k waves' in no particular order do. 1 where a wave has too few.
+__device__ __forceinline__ uint64_t block_bound(uint64_t mine, int k, int waves, uint64_t *bound) {
+  const int share = (k + waves - 1) / waves;
+  const uint32_t hi = (uint32_t)(mine >> 32), lo = (uint32_t)mine;
+  const uint32_t value = wave_kth(hi, share);
+  const int above = __popcll(__ballot(hi > value)), equal = __popcll(__ballot(hi == value));
+  // All of that value, or where those are too many as many as are wanted by their columns.
+  uint64_t key = (uint64_t)value << 32;
+  if (value != 0 && above + equal > share) key |= wave_kth(hi == value ? lo : 0, share - above);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) bound[threadIdx.x >> 6] = (int)(threadIdx.x >> 6) < waves ? max(key, (uint64_t)1) : ~0ull;
+  __syncthreads();
+  key = bound[0];
+#pragma unroll
+  for (int i = 1; i < kWaves; ++i) key = min(key, bound[i]);
+  return key;
+}
+
+// Writes the k largest of n keys to out, in order; 0 where there are fewer. Each key's place is the number of
+// larger ones (no two are equal). key has room for 8 more.
+__device__ __forceinline__ void write_ranked(uint64_t *key, int n, int k, uint64_t *out) {
+  if (threadIdx.x < 8) key[n + threadIdx.x] = 0;
+  __syncthreads();
   for (int i = threadIdx.x; i < n; i += kThreads) {
-    const uint64_t mine = sh.key[i];
+    const uint64_t mine = key[i];
     int rank = 0;
-    for (int j = 0; j < n; ++j) rank += sh.key[j] > mine;
+    for (int j = 0; j < n; j += 8) {
+#pragma unroll
+      for (int u = 0; u < 8; ++u) rank += key[j + u] > mine;
+    }
     if (rank < k) out[rank] = mine;
   }
   for (int i = n + threadIdx.x; i < k; i += kThreads) out[i] = 0;
 }
 
-// The k largest entries of a segment, in order, to out (LDS or memory). The k-th largest of a wave's 64 lane maxima bounds
-// its own k-th largest value from below, the largest of the waves' bounds the segment's; what reaches that (some 4 k values of
-// 8192 in no particular order) is gathered in LDS and ranked. The bound is a whole key, so equal values do not all
-// reach it: at most k entries to a lane and wave do. Where they are too many all the same (large values side by side
-// in few lanes), the best is looked for k times.
+// The k largest entries of a segment, in order, to out (LDS or memory): a bound from the lanes' best entries, which is
+// a whole key, so that equal values do not all reach it; what reaches it is gathered in LDS and ranked. Where that is too
+// much (large values side by side in few lanes), the best is looked for k times.
 template <typename T, int E>
-__device__ __forceinline__ void segment_top(const float (&x)[E], int left, uint32_t col0, int k, TopShared &sh, uint64_t *out) {
+__device__ __forceinline__ void segment_top(const Segment<T, E> &x, int left, uint32_t col0, int k, TopShared<kCandidates> &sh,
+                                            uint64_t *out) {
   uint32_t best = 0, best_col = 0;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
@@ -216,22 +238,16 @@ __device__ __forceinline__ void segment_top(const float (&x)[E], int left, uint3
     const uint32_t v = at < left ? value_key(x[e]) : 0;
     if (v > best) best = v, best_col = at;  // a lane's columns go up with e
   }
-  const uint32_t bound = wave_kth(best, k);
-  uint64_t key = entry_key(bound, 0xffffffffu);  // all entries of that value, or with several lanes there the best of them
-  const int above = __popcll(__ballot(best > bound)), equal = __popcll(__ballot(best == bound));
-  if (bound != 0 && above + equal > k) key = entry_key(bound, 0) & ~0xffffffffull | wave_kth(best == bound ? ~(col0 + best_col) : 0, k - above);
-  if ((threadIdx.x & 63) == 0) sh.bound[threadIdx.x >> 6] = bound ? key : 1;
   if (threadIdx.x == 0) sh.count = 0;
-  __syncthreads();
-  key = sh.bound[0];
-#pragma unroll
-  for (int i = 1; i < kWaves; ++i) key = max(key, sh.bound[i]);
-  const uint32_t key_value = (uint32_t)(key >> 32);
+  // The waves whose lanes all have an entry, or the first one.
+  const int waves = max(1, min(kWaves, left / (64 * kVec<T>)));
+  const uint64_t key = block_bound(best ? entry_key(best, col0 + best_col) : 0, k, waves, sh.bound);
+  const uint32_t value = (uint32_t)(key >> 32);
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     const int at = position<T>(e);
     const uint32_t v = value_key(x[e]);
-    if (v >= key_value && at < left) {
+    if (v >= value && at < left) {
       const uint64_t c = entry_key(v, col0 + at);
       if (c >= key) {
         const int i = atomicAdd(&sh.count, 1);  // the places' order changes nothing: they are ranked
@@ -242,7 +258,7 @@ __device__ __forceinline__ void segment_top(const float (&x)[E], int left, uint3
   __syncthreads();
   const int n = sh.count;
   if (n <= kCandidates) {
-    write_ranked(sh, n, k, out);
+    write_ranked(sh.key, n, k, out);
   } else {
     uint64_t last = ~0ull;
     for (int i = 0; i < k; ++i) {
@@ -267,23 +283,55 @@ __device__ __forceinline__ void segment_top(const float (&x)[E], int left, uint3
   __syncthreads();
 }
 
+// The k largest of segs lists of k in order (0 past their ends), to best in order: some lists at a time, as many as there is
+// room for if all of their entries are kept. The threads hold the lists' first entries, or the largest of several lists' first
+// ones, and bound the k-th largest from below.
+__device__ __forceinline__ void join_top(const uint64_t *keys, int segs, int k, TopShared<kJoined> &sh, uint64_t *best) {
+  const int group = kJoined / k - 1;
+  int kept = 0;
+  for (int s0 = 0; s0 < segs; s0 += group, keys += (long)group * k) {
+    const int lists = min(group, segs - s0), depth = kThreads / lists;  // entries of each list that the threads hold
+    uint64_t key = 1;
+    if (lists * k > kThreads) {  // otherwise all are ranked
+      uint64_t mine = 0;
+      const int held = depth > 0 ? lists * min(depth, k) : kThreads;
+      if (depth == 0) {
+        for (int s = threadIdx.x; s < lists; s += kThreads) mine = max(mine, keys[(long)s * k]);
+      } else if ((int)threadIdx.x < held) {
+        mine = keys[threadIdx.x % lists * k + threadIdx.x / lists];
+      }
+      key = block_bound(mine, k, max(1, held / 64), sh.bound);
+    }
+    for (int i = threadIdx.x; i < kept; i += kThreads) sh.key[i] = best[i];
+    if (threadIdx.x == 0) sh.count = kept;
+    __syncthreads();
+    for (int i = threadIdx.x; i < lists * k; i += kThreads) {
+      const uint64_t c = keys[i];
+      if (c >= key) sh.key[atomicAdd(&sh.count, 1)] = c;  // ranked, whatever the places' order
+    }
+    __syncthreads();
+    kept = min(sh.count, k);
+    write_ranked(sh.key, sh.count, k, best);
+    __syncthreads();
+  }
+}
+
 // ------------------------------------------------------------------ a row's results
 template <typename T>
 __device__ __forceinline__ void finish_logprobs(const LogprobsDesc &p, long r, const RowStats &st, const uint64_t *top, float inv_t) {
-  const float lse = lse_of(st);
   if (threadIdx.x == 0) {
-    if (p.lse) p.lse[r] = lse;
+    if (p.lse) p.lse[r] = lse_of(st, inv_t);
     if (p.entropy) p.entropy[r] = entropy_of(st);
     if (p.targets) {
       const long t = p.targets[r];
       const T *x = static_cast<const T *>(p.in.x) + r * p.in.ld;
-      p.logprob[r] = t < 0 ? 0.0f : t >= p.in.cols ? NAN : logprob_of((float)x[t] * inv_t, lse);
+      p.logprob[r] = t < 0 ? 0.0f : t >= p.in.cols ? NAN : logprob_of((float)x[t], st, inv_t);
     }
   }
   if ((int)threadIdx.x < p.k) {
     const uint64_t key = top[threadIdx.x];
     p.top_ids[r * p.k + threadIdx.x] = (int64_t)(uint32_t)~key;
-    p.top_logprobs[r * p.k + threadIdx.x] = logprob_of(key_value((uint32_t)(key >> 32)) * inv_t, lse);
+    p.top_logprobs[r * p.k + threadIdx.x] = logprob_of(key_value((uint32_t)(key >> 32)), st, inv_t);
   }
 }
 
@@ -322,7 +370,6 @@ __device__ __forceinline__ bool teacher_row(const DistillDesc &p, long r, float 
 
 template <typename T>
 __device__ __forceinline__ void finish_distill(const DistillDesc &p, long r, const RowStats &st, float inv_t, Teacher &sh) {
-  const float lse = lse_of(st);
   const bool some = teacher_row(p, r, inv_t, sh);
   const int i = threadIdx.x;
   float part = 0.0f;
@@ -330,14 +377,14 @@ __device__ __forceinline__ void finish_distill(const DistillDesc &p, long r, con
     if (sh.w[i] != sh.w[i]) {
       part = NAN;
     } else if (sh.at[i] >= 0 && sh.w[i] > 0.0f) {
-      const float z = (float)(static_cast<const T *>(p.in.x) + r * p.in.ld)[sh.at[i]] * inv_t;
-      part = z == -INFINITY && lse == lse ? INFINITY : sh.w[i] * (sh.lw[i] - (z - lse));
+      const float lq = logprob_of((float)(static_cast<const T *>(p.in.x) + r * p.in.ld)[sh.at[i]], st, inv_t);
+      part = sh.w[i] * (sh.lw[i] - lq);  // +inf where lq is -inf
     }
   }
   part = block_sum(part, sh.red);
   if (i == 0) {
     p.loss[r] = part * (p.in.temperature * p.in.temperature);
-    if (p.lse) p.lse[r] = lse;
+    if (p.lse) p.lse[r] = lse_of(st, inv_t);
   }
 }
 
@@ -357,18 +404,18 @@ template <typename T, int E, typename D, bool TOP, bool ONE>
 __global__ void __launch_bounds__(kThreads) segment_kernel(D p, float inv_t, int segs) {
   constexpr bool DISTILL = std::is_same_v<D, DistillDesc>;
   __shared__ float red[kWaves];
-  __shared__ std::conditional_t<TOP, TopShared, int> top;
+  __shared__ std::conditional_t<TOP, TopShared<kCandidates>, int> top;
   __shared__ uint64_t best[TOP && ONE ? kTopMax : 1];
   __shared__ std::conditional_t<DISTILL && ONE, Teacher, int> teacher;
   const long r = blockIdx.x / segs;
   const int seg = blockIdx.x % segs;
   const long col0 = (long)seg * kThreads * E;
   const int left = (int)min(p.in.cols - col0, (long)kThreads * E);
-  float x[E];
-  load_segment<T, E>(static_cast<const T *>(p.in.x) + r * p.in.ld + col0, left, x);
-  const RowStats st = segment_stats<E>(x, inv_t, red);
+  Segment<T, E> x;
+  x.load(static_cast<const T *>(p.in.x) + r * p.in.ld + col0, left);
+  const RowStats st = segment_stats<!DISTILL>(x, inv_t * kLog2e, red);
   const Work w = work_of(p.workspace, p.in.rows, segs);
-  if constexpr (TOP) segment_top<T, E>(x, left, (uint32_t)col0, p.k, top, ONE ? best : w.keys + (r * segs + seg) * p.k);
+  if constexpr (TOP) segment_top(x, left, (uint32_t)col0, p.k, top, ONE ? best : w.keys + (r * segs + seg) * p.k);
   if constexpr (ONE) {
     if constexpr (DISTILL)
       finish_distill<T>(p, r, st, inv_t, teacher);
@@ -382,62 +429,45 @@ __global__ void __launch_bounds__(kThreads) segment_kernel(D p, float inv_t, int
 template <typename T, typename D>
 __global__ void __launch_bounds__(kThreads) join_kernel(D p, float inv_t, int segs) {
   constexpr bool DISTILL = std::is_same_v<D, DistillDesc>;
-  __shared__ std::conditional_t<DISTILL, Teacher, TopShared> sh;
+  __shared__ std::conditional_t<DISTILL, Teacher, TopShared<kJoined>> sh;
   __shared__ uint64_t best[kTopMax];
   __shared__ RowStats part[kWaves];
   const long r = blockIdx.x;
   const Work w = work_of(p.workspace, p.in.rows, segs);
   // Each thread its segments in order, then the threads in pairs: an order that depends on the sizes alone.
+  const float c = inv_t * kLog2e;
   RowStats st{-INFINITY, 0.0f, 0.0f};
-  for (int i = threadIdx.x; i < segs; i += kThreads) st = join_stats(st, w.stats[r * segs + i]);
+  for (int i = threadIdx.x; i < segs; i += kThreads) st = join_stats(st, w.stats[r * segs + i], c);
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
     const RowStats b{__shfl_xor(st.m, o, 64), __shfl_xor(st.s, o, 64), __shfl_xor(st.t, o, 64)};
-    st = threadIdx.x & o ? join_stats(b, st) : join_stats(st, b);
+    st = threadIdx.x & o ? join_stats(b, st, c) : join_stats(st, b, c);
   }
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = st;
   __syncthreads();
   st = part[0];
 #pragma unroll
-  for (int i = 1; i < kWaves; ++i) st = join_stats(st, part[i]);
+  for (int i = 1; i < kWaves; ++i) st = join_stats(st, part[i], c);
   if constexpr (DISTILL) {
     finish_distill<T>(p, r, st, inv_t, sh);
   } else {
-    if (p.k > 0) {
-      // Every segment's k are in order: the largest of their last ones bounds the row's k-th from below. What reaches it is
-      // ranked, a part of the segments at a time where they are more than there is room for (with the best so far).
-      const uint64_t *keys = w.keys + r * segs * p.k;
-      const int k = p.k, group = kCandidates / k - 1;
-      int kept = 0;
-      for (int s0 = 0; s0 < segs; s0 += group) {
-        const int count = min(group, segs - s0);
-        if (threadIdx.x == 0) sh.count = kept;
-        uint64_t bound = 1;
-        for (int i = threadIdx.x; i < count; i += kThreads) bound = max(bound, keys[(long)(s0 + i) * k + k - 1]);
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) bound = max(bound, (uint64_t)__shfl_xor((unsigned long long)bound, o, 64));
-        if ((threadIdx.x & 63) == 0) sh.bound[threadIdx.x >> 6] = bound;
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < kWaves; ++i) bound = max(bound, sh.bound[i]);
-        for (int i = threadIdx.x; i < kept; i += kThreads) sh.key[i] = best[i];
-        for (int i = threadIdx.x; i < count * k; i += kThreads) {
-          const uint64_t c = keys[(long)s0 * k + i];
-          if (c >= bound) sh.key[atomicAdd(&sh.count, 1)] = c;  // ranked, whatever the places' order
-        }
-        __syncthreads();
-        const int n = sh.count;
-        write_ranked(sh, n, k, best);
-        kept = min(n, k);
-        __syncthreads();
-      }
-    }
+    if (p.k > 0) join_top(w.keys + r * segs * p.k, segs, p.k, sh, best);
     finish_logprobs<T>(p, r, st, best, inv_t);
   }
 }
 
 // ------------------------------------------------------------------ backward kernels
-// A workgroup to a segment, as in the forward pass: one read and one write. A row whose gradient is 0 is not read.
+// A workgroup to a segment, as in the forward pass: one read and one write. A row whose gradient is 0 is not read. A row
+// with an lse this low has nothing but masked columns (-inf or the type's lowest value, which would leave no room
+// for ln s beside it): its p are taken as 0.
+constexpr float kMasked = -0x1p100f;
+
+// ln p in base 2, of x with an lse: fp16 in one fma; fp32's lowest value times log2(e) would be -inf.
+template <typename T>
+__device__ __forceinline__ float log2_p(float x, float inv_t, float lse) {
+  return sizeof(T) == 2 ? fmaf(x, inv_t * kLog2e, -lse * kLog2e) : fmaf(x, inv_t, -lse) * kLog2e;
+}
+
 template <typename T, int E>
 __global__ void __launch_bounds__(kThreads) logprobs_backward_kernel(LogprobsGradDesc p, float inv_t, int segs) {
   const long r = blockIdx.x / segs, col0 = (long)(blockIdx.x % segs) * kThreads * E;
@@ -446,23 +476,25 @@ __global__ void __launch_bounds__(kThreads) logprobs_backward_kernel(LogprobsGra
   const float lse = p.lse[r], gh = p.grad_entropy ? p.grad_entropy[r] : 0.0f, h = p.grad_entropy ? p.entropy[r] : 0.0f;
   float gl = t >= 0 ? p.grad_logprob[r] : 0.0f;
   if (t >= p.in.cols) gl = NAN;
-  const bool none = (gl == 0.0f && gh == 0.0f) || (lse == -INFINITY && t < p.in.cols);
-  float x[E];
+  const bool none = (gl == 0.0f && gh == 0.0f) || (lse <= kMasked && t < p.in.cols);
+  Segment<T, E> x;
   if (none) {
 #pragma unroll
-    for (int e = 0; e < E; ++e) x[e] = 0.0f;
+    for (int i = 0; i < E / kVec<T>; ++i) x.v[i] = 0;
   } else {
-    load_segment<T, E>(static_cast<const T *>(p.in.x) + r * p.in.ld + col0, left, x);
+    x.load(static_cast<const T *>(p.in.x) + r * p.in.ld + col0, left);
     const int at = t >= col0 && t < col0 + left ? (int)(t - col0) : -1;
+    // In base 2: ln p = d ln 2. With the entropy's gradient as a and b: -p (gl + gh (ln p + h)) / T = p (a + b d).
+    const float a = -(gl + gh * h) * inv_t, b = -gh * kLn2 * inv_t;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const float lp = x[e] * inv_t - lse, q = exp_of(lp);
-      float v = -q * (gl + gh * (fmaxf(lp, kFloor) + h));  // 0 where q is 0 and lp is -inf
-      if (position<T>(e) == at) v += gl;
-      x[e] = v * inv_t;
+      const float d = log2_p<T>(x[e], inv_t, lse);
+      float v = exp2_of(d) * fmaf(fmaxf(d, kFloor), b, a);  // 0 where p is 0 and d is -inf
+      if (position<T>(e) == at) v += gl * inv_t;
+      x.v[e / kVec<T>][e % kVec<T>] = (T)v;
     }
   }
-  store_segment<T, E>(static_cast<T *>(p.grad) + r * p.ldg + col0, left, x);
+  x.store(static_cast<T *>(p.grad) + r * p.ldg + col0, left);
 }
 
 template <typename T, int E>
@@ -472,9 +504,9 @@ __global__ void __launch_bounds__(kThreads) distill_backward_kernel(DistillDesc 
   const int left = (int)min(p.in.cols - col0, (long)kThreads * E);
   const T *row = static_cast<const T *>(p.in.x) + r * p.in.ld + col0;
   T *out = static_cast<T *>(p.grad) + r * p.ldg + col0;
-  const float lse = p.lse_in[r], gt = p.grad_loss[r] * p.in.temperature;
-  float x[E];
-  if (gt != 0.0f) load_segment<T, E>(row, left, x);
+  const float gt = p.grad_loss[r] * p.in.temperature, lse = p.lse_in[r] <= kMasked ? INFINITY : p.lse_in[r];  // q = 0
+  Segment<T, E> x;
+  if (gt != 0.0f) x.load(row, left);
   const bool some = teacher_row(p, r, inv_t, sh);
   const bool none = !some || gt == 0.0f;
   const float bad = some && sh.w[0] != sh.w[0] ? NAN : 0.0f;
@@ -486,13 +518,15 @@ __global__ void __launch_bounds__(kThreads) distill_backward_kernel(DistillDesc 
   float fix = 0.0f;
   if (mine) {
     float sum = 0.0f;
+#pragma unroll 8
     for (int j = 0; j < p.k; ++j) sum += sh.at[j] == sh.at[i] ? sh.w[j] : 0.0f;
-    fix = gt * ((lse == -INFINITY ? 0.0f : exp_of((float)row[at] * inv_t - lse)) - sum + bad);
+    fix = gt * (exp2_of(log2_p<T>((float)row[at], inv_t, lse)) - sum + bad);
   }
   const bool any = __syncthreads_or(mine);
 #pragma unroll
-  for (int e = 0; e < E; ++e) x[e] = none ? 0.0f : gt * ((lse == -INFINITY ? 0.0f : exp_of(x[e] * inv_t - lse)) + bad);
-  store_segment<T, E>(out, left, x);
+  for (int e = 0; e < E; ++e)
+    x.v[e / kVec<T>][e % kVec<T>] = none ? (T)0.0f : (T)(gt * (exp2_of(log2_p<T>(x[e], inv_t, lse)) + bad));
+  x.store(out, left);
   if (any) {
     __syncthreads();
     if (mine) out[at] = (T)fix;

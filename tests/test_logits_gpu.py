@@ -132,6 +132,28 @@ def test_many_equal_and_clustered_values(dev):
             _check_forward(dev, x, torch.zeros(6, dtype=torch.int64), k, 1.0)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_many_segments(dev, dtype):
+    """A row of more segments than the joining kernel takes at a time, its best entries anywhere, in one place, and equal."""
+    g = torch.Generator().manual_seed(21)
+    for rows, cols in ((1, 300000), (600, 17000), (1, 2**20 + 3)):
+        x = torch.randn((rows, cols), generator=g).to(dtype)
+        if rows == 1:
+            x = torch.cat((x, x, x, x))
+            x[1, 2 * cols // 3 : 2 * cols // 3 + 100] = 6.0 + torch.arange(100).to(dtype) / 64
+            x[2] = torch.arange(cols).to(dtype) if dtype == torch.float32 else torch.arange(cols).float().div(cols).to(dtype)
+            x[3] = 0.5
+        xd = x.to(dev)
+        for k in (1, 64):
+            ids, tops = torch.empty((len(x), k), dtype=torch.int64, device=dev), torch.empty((len(x), k), device=dev)
+            G.token_logprobs(xd, None, None, top_ids=ids, top_logprobs=tops)
+            want = torch.sort(x.float(), dim=1, descending=True, stable=True)
+            assert torch.equal(ids.cpu(), want.indices[:, :k])
+            z = x.double()
+            lp = want.values[:, :k].double() - torch.logsumexp(z, 1, keepdim=True)
+            assert bool(((tops.cpu().double() - lp).abs() <= E * (512 + 16 * z.abs().amax())).all())
+
+
 def test_strides_offsets_and_optional_outputs(dev):
     for dtype in (torch.float32, torch.float16):
         base = _logits(30, 1203, dtype, 7).to(dev)
@@ -227,6 +249,42 @@ def test_backward_of_special_rows(dev):
         assert bool((dx[0] == 0).all()) and bool((dx[4] == 0).all()) and bool((dx[5] == 0).all())
         assert bool(torch.isnan(dx[1:4]).all())
         assert bool(torch.isfinite(dx[6:]).all()) and bool((dx[6:].abs().sum(1) > 0).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("cols", [100, 20000])
+def test_rows_of_the_lowest_value(dev, cols, dtype):
+    """A mask of the type's lowest value that leaves no column: the log-probabilities are those of equal logits (lse has
+    no room for ln cols beside the lowest fp32 value), and the gradient does not take 1 for each p."""
+    low = torch.finfo(dtype).min
+    x = torch.full((2, cols), low, dtype=dtype)
+    x[1, 7] = 1.0
+    t = torch.tensor([3, 7], device=dev)
+    lp, lse, h, ids, tops = _forward(dev, x.to(dev), t, 5, 1.0)
+    ln = math.log(cols)
+    # fp16: x - m and its product with T's reciprocal are exact here; ln s has the roundings of a sum and a logarithm
+    assert abs(lp[0].item() + ln) <= 256 * E * (1 + ln) and abs(h[0].item() - ln) <= 512 * E * (1 + ln)
+    assert abs(lp[1].item()) <= 256 * E and ids.tolist() == [[0, 1, 2, 3, 4], [7, 0, 1, 2, 3]]
+    assert float((tops[0].cpu() + ln).abs().max()) <= 256 * E * (1 + ln)
+    g, dx = torch.ones(2, device=dev), torch.empty((2, cols), dtype=dtype, device=dev)
+    G.token_logprobs_backward(x.to(dev), t, lse, g, dx)
+    if dtype == torch.float32:
+        assert bool((dx[0] == 0).all())
+    else:  # lse is off by half a step at 65504: 2^-9, and p by as much relatively
+        want = torch.full((cols,), -1.0 / cols, dtype=torch.float64)
+        want[3] += 1
+        assert bool(((dx[0].cpu().double() - want).abs() <= 2.0**-8 / cols + 2.0**-11 * want.abs() + 2.0**-25).all())
+    want = torch.zeros(cols, dtype=torch.float64)  # one column left: p = 1 there
+    assert bool(((dx[1].cpu().double() - want).abs() <= 512 * E).all())
+    loss = torch.empty(2, device=dev)
+    ids, teacher = torch.tensor([[1, 2], [7, 7]], device=dev), torch.zeros((2, 2), device=dev)
+    G.distill(x.to(dev), ids, teacher, loss, lse=lse)
+    assert abs(loss[0].item() - (ln - math.log(2))) <= 512 * E * (1 + ln) and abs(loss[1].item() + math.log(2)) <= 512 * E
+    G.distill_backward(x.to(dev), ids, teacher, lse, g, dx)
+    if dtype == torch.float32:
+        want[1:3] = -0.5
+        assert bool((dx[0].cpu().double() == want).all())
+    assert bool((dx[1].abs() <= 512 * E).all())
 
 
 def _teacher(rows, cols, k, seed):
