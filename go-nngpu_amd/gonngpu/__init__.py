@@ -10,6 +10,7 @@ from __future__ import annotations
 import ctypes
 import os
 import re
+import threading
 
 import numpy as np
 
@@ -175,13 +176,20 @@ def _check(rc, err):
         if err.message:
             msg = ctypes.string_at(err.message).decode(errors="replace")
             _lib.free_c_error_message(err.message)
+            err.message = None
         raise GonngpuError(rc, msg)
 
 
+_errors = threading.local()
+
+
 def call(name, *args):
-    """Calls a C-ABI entry point whose last argument is CError*; raises GonngpuError on failure."""
+    """Calls a C-ABI entry point whose last argument is CError*; raises GonngpuError on failure. The CError is the
+    thread's own, kept for its next call (a new one takes 0.5 us)."""
     L = load()
-    err = CError()
+    err = getattr(_errors, "err", None)
+    if err is None:
+        err = _errors.err = CError()
     rc = getattr(L, name)(*args, ctypes.byref(err))
     _check(rc, err)
     return rc
@@ -257,8 +265,8 @@ class Buffer:
 
 
 # --------------------------------------------------------------------------- device-pointer API
-def _current_stream():
-    """Handle of torch's current stream. Building torch's Stream object for it takes 2.7 us, a
+def _current_stream(device=None):
+    """Handle of torch's current stream (on the current device). Building torch's Stream object for it takes 2.7 us, a
     third of what a small call costs the host; asking for the handle takes 0.4 us. The function for
     that is not part of torch's public interface: without it, the Stream object is built."""
     import torch
@@ -267,7 +275,7 @@ def _current_stream():
         raw = torch._C._cuda_getCurrentRawStream
     except AttributeError:
         return torch.cuda.current_stream().cuda_stream
-    return raw(torch.cuda.current_device())
+    return raw(torch.cuda.current_device() if device is None else device)
 
 
 def _run_ordered(name, *args):
@@ -350,15 +358,17 @@ def _refuse(message):
     raise GonngpuError(-1, message)
 
 
-_torch = None
+_torch = _current_device = None
 
 
 def _types():
     """torch, imported once at the first call that needs it (asking the import system each time costs a call 0.3 us)."""
-    global _torch
+    global _torch, _current_device
     if _torch is None:
         import torch
 
+        # The function behind current_device() is not part of torch's public interface; asking it takes 0.2 us less.
+        _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
         _torch = torch
     return _torch
 
@@ -369,39 +379,55 @@ def _device_of(first, *others):
     for t in others:
         if t is not None and t.get_device() != device:
             _refuse(f"tensors on {first.device} and {t.device}")
-    if device < 0 or device != _types().cuda.current_device():
+    if device < 0 or device != _current_device():
         _refuse(f"a tensor on {first.device}: all have to be on the current GPU")
+    return device
 
 
-def _expect(what, t, dtype, shape):
-    """Checks an argument that is one dense array of the given type and shape."""
-    if t.dtype is not dtype or t.shape != shape or not t.is_contiguous():
-        _refuse(f"{what}: a contiguous {dtype} tensor of shape {shape} is needed, got {t.dtype} {tuple(t.shape)}")
+def _expect(what, t, dtype, n):
+    """Checks an argument that is a dense array of n values of the given type. (numel and is_contiguous take 0.06 us each,
+    a size 0.1, the shape 0.7.)"""
+    if t.dtype is not dtype or t.numel() != n or not t.is_contiguous():
+        _refuse(f"{what}: {n} contiguous values of {dtype} are needed, got {t.dtype} {tuple(t.shape)}")
 
 
 def _matrix(what, t):
     """(GN_F32 or GN_F16, rows, cols, elements from row to row) of a matrix whose rows are dense."""
     T = _types()
-    if t.dtype is T.float32:
+    dtype = t.dtype
+    if dtype is T.float32:
         dtype = GN_F32
-    elif t.dtype is T.float16:
+    elif dtype is T.float16:
         dtype = GN_F16
     else:
         _refuse(f"{what}: float32 or float16 is needed, got {t.dtype}")
-    shape, strides = t.shape, t.stride()
-    if len(shape) != 2 or (strides[1] != 1 and shape[1] > 1) or (strides[0] < shape[1] and shape[0] > 1):
-        _refuse(f"{what}: a matrix of dense rows is needed, got shape {tuple(shape)}, strides {strides}")
-    return dtype, shape[0], shape[1], (strides[0] if shape[0] > 1 else shape[1])
+    strides = t.stride()
+    if len(strides) == 2:
+        rows, cols = t.size(0), t.size(1)
+        if (strides[1] == 1 or cols <= 1) and (strides[0] >= cols or rows <= 1):
+            return dtype, rows, cols, (strides[0] if rows > 1 else cols)
+    _refuse(f"{what}: a matrix of dense rows is needed, got shape {tuple(t.shape)}, strides {strides}")
 
 
-def _mxfp4_matrix(what, data, scales, cols):
-    """Checks the two arrays of a stored MXFP4 matrix of `cols` columns; its rows."""
-    groups = -(-cols // 128)
-    rows = data.shape[0] if data.dim() == 2 else -1
-    u8 = _types().uint8
-    _expect(what, data, u8, (rows, 64 * groups))
-    _expect(what, scales, u8, (rows, 4 * groups))
-    return rows
+def _mxfp4_matrix(what, data, scales, rows, cols):
+    """Checks the two arrays of a stored MXFP4 matrix."""
+    u8, groups = _types().uint8, rows * (-(-cols // 128))
+    _expect(what, data, u8, 64 * groups)
+    _expect(what, scales, u8, 4 * groups)
+
+
+def _width(t):
+    """k of a rows x k array."""
+    return t.size(1) if t.dim() == 2 else -1
+
+
+def _dispatch_on(device, stream_ptr, name, *args):
+    """_dispatch for arguments whose device is known to be the current one."""
+    if stream_ptr is None:
+        stream_ptr = _current_stream(device)
+        if not stream_ptr:
+            return _run_ordered(name, *args)
+    return call(name, *args, stream_ptr)
 
 
 def mxfp4_empty(rows, cols, device="cuda"):
@@ -415,19 +441,17 @@ def mxfp4_empty(rows, cols, device="cuda"):
 def mxfp4_quantize(x, data, scales, stream_ptr=None):
     """A float32 or float16 matrix brought to MXFP4, into the arrays of mxfp4_empty(*x.shape)."""
     dt, rows, cols, ld = _matrix("mxfp4_quantize", x)
-    if _mxfp4_matrix("mxfp4_quantize", data, scales, cols) != rows:
-        _refuse(f"mxfp4_quantize: {rows} rows into arrays of {data.shape[0]}")
-    _device_of(x, data, scales)
-    _dispatch(stream_ptr, "gn_mxfp4_quantize", dt, _ptr(x), rows, cols, ld, _ptr(data), _ptr(scales))
+    _mxfp4_matrix("mxfp4_quantize: data, scales", data, scales, rows, cols)
+    device = _device_of(x, data, scales)
+    _dispatch_on(device, stream_ptr, "gn_mxfp4_quantize", dt, x.data_ptr(), rows, cols, ld, data.data_ptr(), scales.data_ptr())
 
 
 def mxfp4_dequantize(data, scales, out, stream_ptr=None):
     """The values of a stored MXFP4 matrix, to a float32 or float16 matrix of its size."""
     dt, rows, cols, ld = _matrix("mxfp4_dequantize", out)
-    if _mxfp4_matrix("mxfp4_dequantize", data, scales, cols) != rows:
-        _refuse(f"mxfp4_dequantize: {data.shape[0]} rows into {rows}")
-    _device_of(data, scales, out)
-    _dispatch(stream_ptr, "gn_mxfp4_dequantize", _ptr(data), _ptr(scales), rows, cols, dt, _ptr(out), ld)
+    _mxfp4_matrix("mxfp4_dequantize: data, scales", data, scales, rows, cols)
+    device = _device_of(data, scales, out)
+    _dispatch_on(device, stream_ptr, "gn_mxfp4_dequantize", data.data_ptr(), scales.data_ptr(), rows, cols, dt, out.data_ptr(), ld)
 
 
 def mxfp4_gemm(A, B, C, *, alpha=1.0, beta=0.0, bias=None, act=ACT_NONE, act_alpha=0.0, K=None, stream_ptr=None):
@@ -440,35 +464,36 @@ def mxfp4_gemm(A, B, C, *, alpha=1.0, beta=0.0, bias=None, act=ACT_NONE, act_alp
     if isinstance(A, (tuple, list)):
         a, a_scales = A
         if K is None:
-            K = 2 * a.shape[1]
-        dt, lda, rows = GN_MXFP4, 0, _mxfp4_matrix("mxfp4_gemm: A", a, a_scales, K)
+            K = 2 * _width(a)
+        dt, lda = GN_MXFP4, 0
+        _mxfp4_matrix("mxfp4_gemm: A", a, a_scales, M, K)
     else:
         a, a_scales = A, None
         dt, rows, cols, lda = _matrix("mxfp4_gemm: A", a)
         if dt != GN_F16 or K not in (None, cols):
             _refuse(f"mxfp4_gemm: A is float16 with K columns or a pair of MXFP4 arrays, got {a.dtype}, K = {K}")
+        if rows != M:
+            _refuse(f"mxfp4_gemm: {rows} rows of A, {M} of C")
         K = cols
-    if rows != M:
-        _refuse(f"mxfp4_gemm: {rows} rows of A, {M} of C")
-    if _mxfp4_matrix("mxfp4_gemm: B", B[0], B[1], K) != N:
-        _refuse(f"mxfp4_gemm: {B[0].shape[0]} rows of B, {N} columns of C")
+    _mxfp4_matrix("mxfp4_gemm: B", B[0], B[1], N, K)
     if bias is not None:
-        _expect("mxfp4_gemm: bias", bias, T.float32, (N,))
-    _device_of(a, a_scales, B[0], B[1], C, bias)
-    _dispatch(stream_ptr, "gn_mxfp4_gemm", dt, M, N, K, alpha, _ptr(a), lda, _ptr(a_scales), _ptr(B[0]), _ptr(B[1]),
-              beta, _ptr(C), ldc, _ptr(bias), act, act_alpha)
+        _expect("mxfp4_gemm: bias", bias, T.float32, N)
+    device = _device_of(a, a_scales, B[0], B[1], C, bias)
+    _dispatch_on(device, stream_ptr, "gn_mxfp4_gemm", dt, M, N, K, alpha, a.data_ptr(), lda, _ptr(a_scales), B[0].data_ptr(),
+                 B[1].data_ptr(), beta, C.data_ptr(), ldc, _ptr(bias), act, act_alpha)
 
 
 def _logits_workspace(rows, cols, k, device, stream_ptr):
-    """Scratch for one call, from torch's allocator (which keeps what a captured graph uses)."""
+    """Scratch for one call, from torch's allocator (which keeps what a captured graph uses), of the pool of the stream
+    that the call runs on: a block of another stream's pool may still be in use there."""
     T = _types()
     n = load().gn_logits_workspace(rows, cols, k)
     if n == 0:
         return None, 0
-    ws = T.empty((n,), dtype=T.uint8, device=device)
-    if stream_ptr is not None and stream_ptr != _current_stream():
-        ws.record_stream(T.cuda.ExternalStream(stream_ptr))
-    return ws, n
+    if stream_ptr is None or stream_ptr == _current_stream(device):
+        return T.empty((n,), dtype=T.uint8, device=T.device("cuda", device)), n
+    with T.cuda.stream(T.cuda.ExternalStream(stream_ptr or stream(), device=device)):
+        return T.empty((n,), dtype=T.uint8, device=T.device("cuda", device)), n
 
 
 def token_logprobs(logits, targets, logprob, *, lse=None, entropy=None, top_ids=None, top_logprobs=None,
@@ -482,18 +507,19 @@ def token_logprobs(logits, targets, logprob, *, lse=None, entropy=None, top_ids=
         _refuse("token_logprobs: targets and logprob, and top_ids and top_logprobs, are given together")
     k = 0
     if top_ids is not None:
-        k = top_ids.shape[-1] if top_ids.dim() == 2 else -1
-        _expect("token_logprobs: top_ids", top_ids, T.int64, (rows, k))
-        _expect("token_logprobs: top_logprobs", top_logprobs, T.float32, (rows, k))
+        k = _width(top_ids)
+        _expect("token_logprobs: top_ids", top_ids, T.int64, rows * k)
+        _expect("token_logprobs: top_logprobs", top_logprobs, T.float32, rows * k)
     if targets is not None:
-        _expect("token_logprobs: targets", targets, T.int64, (rows,))
+        _expect("token_logprobs: targets", targets, T.int64, rows)
     for what, t in (("logprob", logprob), ("lse", lse), ("entropy", entropy)):
         if t is not None:
-            _expect("token_logprobs: " + what, t, T.float32, (rows,))
-    _device_of(logits, targets, logprob, lse, entropy, top_ids, top_logprobs)
-    ws, n = _logits_workspace(rows, cols, k, logits.device, stream_ptr)
-    _dispatch(stream_ptr, "gn_token_logprobs", dt, _ptr(logits), rows, cols, ld, temperature, _ptr(targets),
-              _ptr(logprob), _ptr(lse), _ptr(entropy), k, _ptr(top_ids), _ptr(top_logprobs), _ptr(ws), n)
+            _expect("token_logprobs: " + what, t, T.float32, rows)
+    device = _device_of(logits, targets, logprob, lse, entropy, top_ids, top_logprobs)
+    ws, n = _logits_workspace(rows, cols, k, device, stream_ptr)
+    _dispatch_on(device, stream_ptr, "gn_token_logprobs", dt, logits.data_ptr(), rows, cols, ld, temperature,
+                 _ptr(targets), _ptr(logprob), _ptr(lse), _ptr(entropy), k, _ptr(top_ids), _ptr(top_logprobs),
+                 _ptr(ws), n)
 
 
 def token_logprobs_backward(logits, targets, lse, grad_logprob, grad_logits, *, entropy=None, grad_entropy=None,
@@ -508,13 +534,14 @@ def token_logprobs_backward(logits, targets, lse, grad_logprob, grad_logits, *, 
     if (targets is None) != (grad_logprob is None) or (entropy is None) != (grad_entropy is None):
         _refuse("token_logprobs_backward: targets and grad_logprob, and entropy and grad_entropy, are given together")
     if targets is not None:
-        _expect("token_logprobs_backward: targets", targets, T.int64, (rows,))
+        _expect("token_logprobs_backward: targets", targets, T.int64, rows)
     for what, t in (("lse", lse), ("grad_logprob", grad_logprob), ("entropy", entropy), ("grad_entropy", grad_entropy)):
         if t is not None:
-            _expect("token_logprobs_backward: " + what, t, T.float32, (rows,))
-    _device_of(logits, targets, lse, grad_logprob, grad_logits, entropy, grad_entropy)
-    _dispatch(stream_ptr, "gn_token_logprobs_backward", dt, _ptr(logits), rows, cols, ld, temperature, _ptr(targets),
-              _ptr(lse), _ptr(entropy), _ptr(grad_logprob), _ptr(grad_entropy), _ptr(grad_logits), ldg)
+            _expect("token_logprobs_backward: " + what, t, T.float32, rows)
+    device = _device_of(logits, targets, lse, grad_logprob, grad_logits, entropy, grad_entropy)
+    _dispatch_on(device, stream_ptr, "gn_token_logprobs_backward", dt, logits.data_ptr(), rows, cols, ld, temperature,
+                 _ptr(targets), _ptr(lse), _ptr(entropy), _ptr(grad_logprob), _ptr(grad_entropy), grad_logits.data_ptr(),
+                 ldg)
 
 
 def distill(logits, ids, teacher, loss, *, lse=None, temperature=1.0, stream_ptr=None):
@@ -523,16 +550,16 @@ def distill(logits, ids, teacher, loss, *, lse=None, temperature=1.0, stream_ptr
     over all columns of logits[r]; lse: the student's log-sum-exp."""
     T = _types()
     dt, rows, cols, ld = _matrix("distill", logits)
-    k = ids.shape[-1] if ids.dim() == 2 else -1
-    _expect("distill: ids", ids, T.int64, (rows, k))
-    _expect("distill: teacher", teacher, T.float32, (rows, k))
+    k = _width(ids)
+    _expect("distill: ids", ids, T.int64, rows * k)
+    _expect("distill: teacher", teacher, T.float32, rows * k)
     for what, t in (("loss", loss), ("lse", lse)):
         if t is not None:
-            _expect("distill: " + what, t, T.float32, (rows,))
-    _device_of(logits, ids, teacher, loss, lse)
-    ws, n = _logits_workspace(rows, cols, 0, logits.device, stream_ptr)
-    _dispatch(stream_ptr, "gn_distill_forward", dt, _ptr(logits), rows, cols, ld, temperature, _ptr(ids), _ptr(teacher),
-              k, _ptr(loss), _ptr(lse), _ptr(ws), n)
+            _expect("distill: " + what, t, T.float32, rows)
+    device = _device_of(logits, ids, teacher, loss, lse)
+    ws, n = _logits_workspace(rows, cols, 0, device, stream_ptr)
+    _dispatch_on(device, stream_ptr, "gn_distill_forward", dt, logits.data_ptr(), rows, cols, ld, temperature, ids.data_ptr(),
+                 teacher.data_ptr(), k, loss.data_ptr(), _ptr(lse), _ptr(ws), n)
 
 
 def distill_backward(logits, ids, teacher, lse, grad_loss, grad_logits, *, temperature=1.0, stream_ptr=None):
@@ -542,14 +569,14 @@ def distill_backward(logits, ids, teacher, lse, grad_loss, grad_logits, *, tempe
     dg, grows, gcols, ldg = _matrix("distill_backward: grad_logits", grad_logits)
     if (dg, grows, gcols) != (dt, rows, cols):
         _refuse("distill_backward: grad_logits has the type and shape of logits")
-    k = ids.shape[-1] if ids.dim() == 2 else -1
-    _expect("distill_backward: ids", ids, T.int64, (rows, k))
-    _expect("distill_backward: teacher", teacher, T.float32, (rows, k))
-    _expect("distill_backward: lse", lse, T.float32, (rows,))
-    _expect("distill_backward: grad_loss", grad_loss, T.float32, (rows,))
-    _device_of(logits, ids, teacher, lse, grad_loss, grad_logits)
-    _dispatch(stream_ptr, "gn_distill_backward", dt, _ptr(logits), rows, cols, ld, temperature, _ptr(ids),
-              _ptr(teacher), k, _ptr(lse), _ptr(grad_loss), _ptr(grad_logits), ldg)
+    k = _width(ids)
+    _expect("distill_backward: ids", ids, T.int64, rows * k)
+    _expect("distill_backward: teacher", teacher, T.float32, rows * k)
+    _expect("distill_backward: lse", lse, T.float32, rows)
+    _expect("distill_backward: grad_loss", grad_loss, T.float32, rows)
+    device = _device_of(logits, ids, teacher, lse, grad_loss, grad_logits)
+    _dispatch_on(device, stream_ptr, "gn_distill_backward", dt, logits.data_ptr(), rows, cols, ld, temperature, ids.data_ptr(),
+                 teacher.data_ptr(), k, _ptr(lse), grad_loss.data_ptr(), grad_logits.data_ptr(), ldg)
 
 
 def spmm_csr(M, N, K, nnz, rowptr, col, val, D, C, flags=None, ldd=None, ldc=None, stream_ptr=None):

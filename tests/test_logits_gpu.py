@@ -436,6 +436,20 @@ def test_streams(dev):
     G.token_logprobs(x, t, lp, top_ids=ids, top_logprobs=tops, stream_ptr=other.cuda_stream)
     other.synchronize()
     assert torch.equal(lp, want[0]) and torch.equal(ids, want[3]) and torch.equal(tops, want[4])
+    # Calls on two streams at once, each with a workspace of its own stream's.
+    x2 = _logits(2, 60000, torch.float16, 22).to(dev)
+    want2 = _forward(dev, x2, t, 20, 1.0)
+    lp2, ids2, tops2 = torch.zeros(2, device=dev), torch.zeros((2, 20), dtype=torch.int64, device=dev), torch.zeros((2, 20), device=dev)
+    torch.cuda.synchronize()
+    for _ in range(50):
+        G.token_logprobs(x, t, lp, top_ids=ids, top_logprobs=tops, stream_ptr=other.cuda_stream)
+        G.token_logprobs(x2, t, lp2, top_ids=ids2, top_logprobs=tops2)
+    torch.cuda.synchronize()
+    assert torch.equal(ids, want[3]) and torch.equal(tops, want[4]) and torch.equal(lp, want[0])
+    assert torch.equal(ids2, want2[3]) and torch.equal(tops2, want2[4]) and torch.equal(lp2, want2[0])
+    G.token_logprobs(x, t, lp, top_ids=ids, top_logprobs=tops, stream_ptr=0)  # the library's stream
+    G.synchronize()
+    assert torch.equal(ids, want[3]) and torch.equal(lp, want[0])
     lp.zero_()
     torch.cuda.synchronize()
     with torch.cuda.stream(torch.cuda.default_stream()):

@@ -113,16 +113,19 @@ BINDING = [
     ("float32 or float16", lambda: G.mxfp4_quantize(_t(4, 8, dtype=torch.float64), *_pair(4, 8))),
     ("dense rows", lambda: G.mxfp4_quantize(_t(8, 4).t(), *_pair(4, 8))),
     ("dense rows", lambda: G.mxfp4_quantize(_t(1, 8).expand(4, 8), *_pair(4, 8))),
-    ("shape", lambda: G.mxfp4_quantize(_t(4, 129), *_pair(4, 128))),
-    ("rows", lambda: G.mxfp4_quantize(_t(4, 8), *_pair(5, 8))),
+    ("values", lambda: G.mxfp4_quantize(_t(4, 129), *_pair(4, 128))),
+    ("values", lambda: G.mxfp4_quantize(_t(4, 8), *_pair(5, 8))),
+    ("values", lambda: G.mxfp4_quantize(_t(4, 8), _pair(4, 8)[0], _t(4, 4))),
+    ("values", lambda: G.mxfp4_quantize(_t(4, 8), _pair(8, 8)[0][::2], _pair(4, 8)[1])),
+    ("gemm: A", lambda: G.mxfp4_gemm(_pair(3, 8), _pair(3, 8), _t(2, 3), K=8)),
     ("current GPU", lambda: G.mxfp4_quantize(_t(4, 8), *_pair(4, 8))),
-    ("rows", lambda: G.mxfp4_dequantize(*_pair(4, 8), _t(3, 8))),
+    ("values", lambda: G.mxfp4_dequantize(*_pair(4, 8), _t(3, 8))),
     ("C is float32", lambda: G.mxfp4_gemm(_t(2, 8, dtype=H), _pair(3, 8), _t(2, 3, dtype=H))),
     ("A is float16", lambda: G.mxfp4_gemm(_t(2, 8), _pair(3, 8), _t(2, 3))),
     ("A is float16", lambda: G.mxfp4_gemm(_t(2, 8, dtype=H), _pair(3, 8), _t(2, 3), K=9)),
     ("rows of A", lambda: G.mxfp4_gemm(_t(4, 8, dtype=H), _pair(3, 8), _t(2, 3))),
-    ("rows of B", lambda: G.mxfp4_gemm(_t(2, 8, dtype=H), _pair(4, 8), _t(2, 3))),
-    ("shape", lambda: G.mxfp4_gemm(_pair(2, 129), _pair(3, 128), _t(2, 3), K=129)),
+    ("gemm: B", lambda: G.mxfp4_gemm(_t(2, 8, dtype=H), _pair(4, 8), _t(2, 3))),
+    ("gemm: B", lambda: G.mxfp4_gemm(_pair(2, 129), _pair(3, 128), _t(2, 3), K=129)),
     ("bias", lambda: G.mxfp4_gemm(_t(2, 8, dtype=H), _pair(3, 8), _t(2, 3), bias=_t(2))),
     ("together", lambda: G.token_logprobs(_t(2, 8), _t(2, dtype=I64), None)),
     ("together", lambda: G.token_logprobs(_t(2, 8), None, None, top_ids=_t(2, 3, dtype=I64))),
