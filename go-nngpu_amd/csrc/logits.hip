@@ -112,10 +112,10 @@ struct RowStats {
 
 __device__ __forceinline__ float exp2_of(float d) { return __builtin_amdgcn_exp2f(d); }  // results below 2^-126 are 0
 
-// T: with t.
+// largest: the thread's largest value. T: with t.
 template <bool T, typename S, int E>
-__device__ __forceinline__ RowStats segment_stats(const Segment<S, E> &x, float c, float *red) {
-  RowStats r{block_max(x.max_value(), red), 0.0f, 0.0f};
+__device__ __forceinline__ RowStats segment_stats(const Segment<S, E> &x, float largest, float c, float *red) {
+  RowStats r{block_max(largest, red), 0.0f, 0.0f};
   const float m = r.m == -INFINITY ? 0.0f : r.m;  // a segment of -inf: all terms 2^-inf = 0
   const float mc = m * c;
 #pragma unroll
@@ -142,14 +142,22 @@ __device__ __forceinline__ float logprob_of(float x, const RowStats &r, float in
   return r.s == 0.0f ? -INFINITY : fmaf(x - r.m, inv_t, -log2f(r.s) * kLn2);
 }
 
-// a and b as of one row (b the later segment).
-__device__ __forceinline__ RowStats join_stats(const RowStats &a, const RowStats &b, float c) {
-  const float m = fmaxf(a.m, b.m), n = m == -INFINITY ? 0.0f : m;
-  const float da = fmaxf((a.m - n) * c, kFloor), db = fmaxf((b.m - n) * c, kFloor);  // a segment of -inf has s = t = 0
-  const float ea = exp2_of(da), eb = exp2_of(db);
-  // A NaN among the logits is in s, and so is +inf (inf - inf); m does not show NaN.
-  RowStats r{m, a.s * ea + b.s * eb, 0.0f};
-  r.t = (a.s == 0.0f ? 0.0f : ea * (a.t + da * a.s)) + (b.s == 0.0f ? 0.0f : eb * (b.t + db * b.s));
+// The statistics of the row that the threads' segments make up, each thread's in an order that the sizes alone
+// give.
+__device__ __forceinline__ RowStats join_stats(const RowStats *stats, int segs, float c, float *red) {
+  float m = -INFINITY;
+  for (int i = threadIdx.x; i < segs; i += kThreads) m = fmaxf(m, stats[i].m);
+  RowStats r{block_max(m, red), 0.0f, 0.0f};
+  const float n = r.m == -INFINITY ? 0.0f : r.m;
+  for (int i = threadIdx.x; i < segs; i += kThreads) {
+    const RowStats a = stats[i];
+    // A NaN among the logits is in s, and so is +inf (inf - inf); m does not show NaN. A segment of -inf has s = t = 0.
+    const float d = fmaxf((a.m - n) * c, kFloor), e = exp2_of(d);
+    r.s += e * a.s;
+    r.t += e * (a.t + d * a.s);
+  }
+  r.s = block_sum(r.s, red);
+  r.t = block_sum(r.t, red);
   return r;
 }
 
@@ -168,13 +176,14 @@ __device__ __forceinline__ float key_value(uint32_t k) {
 }
 __device__ __forceinline__ uint64_t entry_key(uint32_t value, uint32_t col) { return ((uint64_t)value << 32) | ~col; }
 
-// The k-th largest of the wave's 64 values (k >= 1), bit by bit: the largest number that k lanes reach.
+// A number that at least k of the wave's 64 values reach (k >= 1): exactly k where one is that tells them apart, found bit by
+// bit (some 13 of the 32 for logits), else the k-th largest value.
 __device__ __forceinline__ uint32_t wave_kth(uint32_t v, int k) {
   uint32_t t = 0;
-#pragma unroll
-  for (int b = 31; b >= 0; --b) {
-    const uint32_t c = t | (1u << b);
-    if (__popcll(__ballot(v >= c)) >= k) t = c;
+  for (uint32_t bit = 1u << 31; bit != 0; bit >>= 1) {
+    const int n = __popcll(__ballot(v >= (t | bit)));
+    if (n >= k) t |= bit;
+    if (n == k) break;
   }
   return t;
 }
@@ -227,36 +236,37 @@ __device__ __forceinline__ void write_ranked(uint64_t *key, int n, int k, uint64
 
 // The k largest entries of a segment, in order, to out (LDS or memory): a bound from the lanes' best entries, which is
 // a whole key, so that equal values do not all reach it; what reaches it is gathered in LDS and ranked. Where that is too
-// much (large values side by side in few lanes), the best is looked for k times.
+// much (large values side by side in few lanes), and among NaN or +inf (numbers false), the best is looked for k times.
 template <typename T, int E>
-__device__ __forceinline__ void segment_top(const Segment<T, E> &x, int left, uint32_t col0, int k, TopShared<kCandidates> &sh,
-                                            uint64_t *out) {
-  uint32_t best = 0, best_col = 0;
+__device__ __forceinline__ void segment_top(const Segment<T, E> &x, float largest, bool numbers, int left, uint32_t col0, int k,
+                                            TopShared<kCandidates> &sh, uint64_t *out) {
+  int n = kCandidates + 1;
+  if (numbers) {
+    int at = INT_MAX;  // the lane's first place with its largest value
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const int at = position<T>(e);
-    const uint32_t v = at < left ? value_key(x[e]) : 0;
-    if (v > best) best = v, best_col = at;  // a lane's columns go up with e
-  }
-  if (threadIdx.x == 0) sh.count = 0;
-  // The waves whose lanes all have an entry, or the first one.
-  const int waves = max(1, min(kWaves, left / (64 * kVec<T>)));
-  const uint64_t key = block_bound(best ? entry_key(best, col0 + best_col) : 0, k, waves, sh.bound);
-  const uint32_t value = (uint32_t)(key >> 32);
+    for (int e = E - 1; e >= 0; --e)
+      if (x[e] == largest) at = position<T>(e);
+    if (threadIdx.x == 0) sh.count = 0;
+    // The waves whose lanes all have an entry, or the first one.
+    const int waves = max(1, min(kWaves, left / (64 * kVec<T>)));
+    const uint64_t key = block_bound(at < left ? entry_key(value_key(largest), col0 + at) : 0, k, waves, sh.bound);
+    const uint32_t value = (uint32_t)(key >> 32);
+    const float bound = value ? key_value(value) : -INFINITY;  // a cut between numbers may be no number's key: NaN
+    const float least = bound == bound ? bound : -INFINITY;
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const int at = position<T>(e);
-    const uint32_t v = value_key(x[e]);
-    if (v >= value && at < left) {
-      const uint64_t c = entry_key(v, col0 + at);
-      if (c >= key) {
-        const int i = atomicAdd(&sh.count, 1);  // the places' order changes nothing: they are ranked
-        if (i < kCandidates) sh.key[i] = c;
+    for (int e = 0; e < E; ++e) {
+      if (x[e] >= least) {
+        const int i = position<T>(e);
+        const uint64_t c = entry_key(value_key(x[e]), col0 + i);
+        if (c >= key && i < left) {
+          const int to = atomicAdd(&sh.count, 1);  // the places' order changes nothing: they are ranked
+          if (to < kCandidates) sh.key[to] = c;
+        }
       }
     }
+    __syncthreads();
+    n = sh.count;
   }
-  __syncthreads();
-  const int n = sh.count;
   if (n <= kCandidates) {
     write_ranked(sh.key, n, k, out);
   } else {
@@ -291,7 +301,13 @@ __device__ __forceinline__ void join_top(const uint64_t *keys, int segs, int k, 
   int kept = 0;
   for (int s0 = 0; s0 < segs; s0 += group, keys += (long)group * k) {
     const int lists = min(group, segs - s0), depth = kThreads / lists;  // entries of each list that the threads hold
-    uint64_t key = 1;
+    constexpr int N = (kJoined + kThreads - 1) / kThreads;
+    uint64_t all[N], key = 1;  // all entries: under way while the bound is found
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int at = threadIdx.x + i * kThreads;
+      all[i] = at < lists * k ? keys[at] : 0;
+    }
     if (lists * k > kThreads) {  // otherwise all are ranked
       uint64_t mine = 0;
       const int held = depth > 0 ? lists * min(depth, k) : kThreads;
@@ -305,10 +321,9 @@ __device__ __forceinline__ void join_top(const uint64_t *keys, int segs, int k, 
     for (int i = threadIdx.x; i < kept; i += kThreads) sh.key[i] = best[i];
     if (threadIdx.x == 0) sh.count = kept;
     __syncthreads();
-    for (int i = threadIdx.x; i < lists * k; i += kThreads) {
-      const uint64_t c = keys[i];
-      if (c >= key) sh.key[atomicAdd(&sh.count, 1)] = c;  // ranked, whatever the places' order
-    }
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (all[i] >= key) sh.key[atomicAdd(&sh.count, 1)] = all[i];  // ranked, whatever the places' order
     __syncthreads();
     kept = min(sh.count, k);
     write_ranked(sh.key, sh.count, k, best);
@@ -342,19 +357,23 @@ struct Teacher {
   int at[kTeacherMax];
   float red[kWaves];
 };
-__device__ __forceinline__ bool teacher_row(const DistillDesc &p, long r, float inv_t, Teacher &sh) {
+struct Entry {
+  int64_t id;
+  float logit;
+};
+__device__ __forceinline__ Entry load_entry(const DistillDesc &p, long r) {
+  const int i = threadIdx.x;
+  return i < p.k ? Entry{p.ids[r * p.k + i], p.teacher[r * p.k + i]} : Entry{-1, 0.0f};
+}
+__device__ __forceinline__ bool teacher_row(const DistillDesc &p, const Entry &entry, float inv_t, Teacher &sh) {
   const int i = threadIdx.x;
   int at = -1;
   float z = -INFINITY;
-  if (i < p.k) {
-    const int64_t id = p.ids[r * p.k + i];
-    const float t = p.teacher[r * p.k + i];
-    if (id >= p.in.cols)
-      z = NAN;
-    else if (id >= 0)
-      z = t * inv_t, at = (int)id;
-    if (z == -INFINITY) at = -1;
-  }
+  if (entry.id >= p.in.cols)
+    z = NAN;
+  else if (entry.id >= 0)
+    z = entry.logit * inv_t, at = (int)entry.id;
+  if (z == -INFINITY) at = -1;
   const float m = block_all(z, sh.red, [](float a, float b) { return a != a || b != b ? NAN : fmaxf(a, b); });
   if (m == -INFINITY) return false;
   const float e = z == -INFINITY ? 0.0f : expf(z - m);
@@ -370,7 +389,7 @@ __device__ __forceinline__ bool teacher_row(const DistillDesc &p, long r, float 
 
 template <typename T>
 __device__ __forceinline__ void finish_distill(const DistillDesc &p, long r, const RowStats &st, float inv_t, Teacher &sh) {
-  const bool some = teacher_row(p, r, inv_t, sh);
+  const bool some = teacher_row(p, load_entry(p, r), inv_t, sh);
   const int i = threadIdx.x;
   float part = 0.0f;
   if (some && i < p.k) {
@@ -413,9 +432,10 @@ __global__ void __launch_bounds__(kThreads) segment_kernel(D p, float inv_t, int
   const int left = (int)min(p.in.cols - col0, (long)kThreads * E);
   Segment<T, E> x;
   x.load(static_cast<const T *>(p.in.x) + r * p.in.ld + col0, left);
-  const RowStats st = segment_stats<!DISTILL>(x, inv_t * kLog2e, red);
+  const float largest = x.max_value();
+  const RowStats st = segment_stats<!DISTILL>(x, largest, inv_t * kLog2e, red);
   const Work w = work_of(p.workspace, p.in.rows, segs);
-  if constexpr (TOP) segment_top(x, left, (uint32_t)col0, p.k, top, ONE ? best : w.keys + (r * segs + seg) * p.k);
+  if constexpr (TOP) segment_top(x, largest, st.s == st.s, left, (uint32_t)col0, p.k, top, ONE ? best : w.keys + (r * segs + seg) * p.k);
   if constexpr (ONE) {
     if constexpr (DISTILL)
       finish_distill<T>(p, r, st, inv_t, teacher);
@@ -431,23 +451,10 @@ __global__ void __launch_bounds__(kThreads) join_kernel(D p, float inv_t, int se
   constexpr bool DISTILL = std::is_same_v<D, DistillDesc>;
   __shared__ std::conditional_t<DISTILL, Teacher, TopShared<kJoined>> sh;
   __shared__ uint64_t best[kTopMax];
-  __shared__ RowStats part[kWaves];
+  __shared__ float red[kWaves];
   const long r = blockIdx.x;
   const Work w = work_of(p.workspace, p.in.rows, segs);
-  // Each thread its segments in order, then the threads in pairs: an order that depends on the sizes alone.
-  const float c = inv_t * kLog2e;
-  RowStats st{-INFINITY, 0.0f, 0.0f};
-  for (int i = threadIdx.x; i < segs; i += kThreads) st = join_stats(st, w.stats[r * segs + i], c);
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const RowStats b{__shfl_xor(st.m, o, 64), __shfl_xor(st.s, o, 64), __shfl_xor(st.t, o, 64)};
-    st = threadIdx.x & o ? join_stats(b, st, c) : join_stats(st, b, c);
-  }
-  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = st;
-  __syncthreads();
-  st = part[0];
-#pragma unroll
-  for (int i = 1; i < kWaves; ++i) st = join_stats(st, part[i], c);
+  const RowStats st = join_stats(w.stats + r * segs, segs, inv_t * kLog2e, red);
   if constexpr (DISTILL) {
     finish_distill<T>(p, r, st, inv_t, sh);
   } else {
@@ -505,9 +512,10 @@ __global__ void __launch_bounds__(kThreads) distill_backward_kernel(DistillDesc 
   const T *row = static_cast<const T *>(p.in.x) + r * p.in.ld + col0;
   T *out = static_cast<T *>(p.grad) + r * p.ldg + col0;
   const float gt = p.grad_loss[r] * p.in.temperature, lse = p.lse_in[r] <= kMasked ? INFINITY : p.lse_in[r];  // q = 0
+  const Entry entry = load_entry(p, r);  // before the segment: loads arrive in order
   Segment<T, E> x;
   if (gt != 0.0f) x.load(row, left);
-  const bool some = teacher_row(p, r, inv_t, sh);
+  const bool some = teacher_row(p, entry, inv_t, sh);
   const bool none = !some || gt == 0.0f;
   const float bad = some && sh.w[0] != sh.w[0] ? NAN : 0.0f;
   // The entries of this segment are put right once the segment is written; their logits are read before (grad may be
