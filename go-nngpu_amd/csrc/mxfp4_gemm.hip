@@ -9,7 +9,7 @@ namespace gn {
 namespace {
 
 // 256 rows of codes, and of fp16 activations, stay below 2^31 bytes: 32-bit offsets within a tile.
-constexpr long kMaxK = 1L << 22;
+constexpr long kMaxK = 1L << 22, kMaxRows = 1L << 25;
 
 typedef int i32x8_t __attribute__((ext_vector_type(8)));
 typedef float float16_t __attribute__((ext_vector_type(16)));
@@ -837,6 +837,8 @@ int check_mxfp4_gemm(const MxGemmDesc &d, CError *err) {
   size_t n;
   if (d.K > kMaxK) return set_error(err, -1, "mxfp4 gemm: K of %ld is too large", d.K);
   if (d.M < 0 || d.N < 0 || d.K < 0) return set_error(err, -1, "mxfp4 gemm: negative size");
+  // A launch has below 2^32 work-items; up to 512 of them take 16 columns, 256 take 64 rows.
+  if (d.M > kMaxRows || d.N > kMaxRows) return set_error(err, -1, "mxfp4 gemm: %ld x %ld is too large", d.M, d.N);
   if (!act_supported(d.act)) return set_error(err, -1, "mxfp4 gemm: unsupported activation %d", d.act);
   if (d.M == 0 || d.N == 0) return 0;
   if (!d.C) return set_error(err, -1, "mxfp4 gemm: NULL C");

@@ -430,7 +430,8 @@ int gn_mxfp4_dequantize(const void *data, const void *scales, long rows, long co
  * outputs x inputs), fp32 accumulation. A is M x K: GN_F16 (lda >= K elements from row to row, a_scales NULL; each weight
  * takes part with its exact value) or GN_MXFP4 (data and scales as above, lda is not read).
  * C and bias are fp32; bias may be NULL; beta == 0 never reads C; act and act_alpha as gn_gemm; K == 0
- * gives act(beta * C + bias); K and (with several rows) lda are at most 2^22. Asynchronous; allocates nothing and may be captured.
+ * gives act(beta * C + bias); K and (with several rows) lda are at most 2^22,
+ * M and N at most 2^25. Asynchronous; allocates nothing and may be captured.
  * Codes: -1 invalid argument, -6 launch error. */
 int gn_mxfp4_gemm(int a_dtype, long M, long N, long K, float alpha, const void *A, long lda, const void *a_scales,
                   const void *B, const void *b_scales, float beta, float *C, long ldc, const float *bias, int act,

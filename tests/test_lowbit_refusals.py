@@ -61,7 +61,8 @@ CASES = [
         ("leading", dict(ldc=4)), ("leading", dict(lda=99)), ("NULL", dict(A=None)), ("NULL", dict(B=None)), ("NULL", dict(bsc=None)),
         ("multiple", dict(B=P + 8)), ("multiple", dict(bsc=P + 2)), ("scales given", dict(asc=P)), ("NULL", dict(a=FP4)),
         ("multiple", dict(a=FP4, A=P + 8, asc=P)), ("aligned", dict(A=P + 1)), ("aligned", dict(C=P + 2)), ("aligned", dict(bias=P + 1)),
-        ("too large", dict(M=1 << 33, N=1 << 33, ldc=1 << 33))]),
+        ("too large", dict(M=1 << 33, N=1 << 33, ldc=1 << 33)), ("too large", dict(M=1, N=(1 << 25) + 1, ldc=1 << 26)),
+        ("too large", dict(M=(1 << 25) + 1, N=1, ldc=1)), ("too large", dict(M=1 << 20, N=1 << 20, ldc=1 << 20))]),
     ("gn_token_logprobs", LOGPROBS, [
         ("dtype", dict(dtype=FP4)), ("size", dict(rows=-1)), ("size", dict(cols=0)), ("size", dict(cols=1 << 31, ld=1 << 31)),
         ("temperature", dict(temp=0.0)), ("temperature", dict(temp=-1.0)), ("temperature", dict(temp=NAN)), ("temperature", dict(temp=INF)),
