@@ -757,6 +757,30 @@ void launch_half(MxParams p, hipStream_t s) {
   hipLaunchKernelGGL((mx_half_kernel<WM, WN, FM, FN, NS, WPE, DMA>), dim3((unsigned)(p.tiles_m * p.tiles_n)), dim3(WM * WN * 64), 0, s, p);
 }
 
+// More than 64 rows of 4-bit activations: the tile with which a CU's share takes the least time, the larger one of two equals.
+// A tile alone on a CU takes 0.75, 0.50, 0.35, 0.28 and 0.20 us for a stage, the first at the rate of the matrix
+// instructions, the last at the latency of its copies and barriers. Measured, us, 256 x 256 / 256 x 128 / 128 x 128 / 64 x 128 / 64 x 64:
+// 4096 -> 11008, 1024 rows 36.6 / 45.9 / 43.0 / 50.5 / 63.7, 512 rows 33.3 / 23.7 / 27.8 / 29.6 / 38.8, 200 rows 29.0 / 18.6 /
+// 15.6 / 17.5 / 19.6, 128 rows 28.0 / 18.3 / 15.3 / 11.8 / 12.3; 11008 -> 4096, 512 rows 69.9 / 47.1 / 35.1 / 28.0 / 34.2;
+// 4096 -> 4096, 65 rows 26.7 / 17.2 / 13.9 / 11.4 / 9.2.
+void launch_fp4_tiles(const MxParams &p, hipStream_t s) {
+  constexpr int kTiles[5][3] = {{256, 256, 75}, {256, 128, 50}, {128, 128, 35}, {64, 128, 28}, {64, 64, 20}};
+  int best = 0;
+  long least = 0;
+  for (int i = 0; i < 5; ++i) {
+    const long tiles = ((p.M + kTiles[i][0] - 1) / kTiles[i][0]) * ((p.N + kTiles[i][1] - 1) / kTiles[i][1]);
+    const long cost = (tiles + 255) / 256 * kTiles[i][2];  // 256 CUs
+    if (i == 0 || cost < least) best = i, least = cost;
+  }
+  switch (best) {
+    case 0: return launch_fp4<2, 4, 4, 2, 2>(p, s);
+    case 1: return launch_fp4<4, 2, 2, 2, 2>(p, s);
+    case 2: return launch_fp4<2, 2, 2, 2, 2>(p, s);
+    case 3: return launch_fp4<2, 2, 1, 2, 2>(p, s);
+    default: return launch_fp4<2, 2, 1, 1, 2>(p, s);
+  }
+}
+
 // fp16 activations, more than 64 rows. 256 x 256 tiles where there is one for each CU (8192^3: 852 us, 128 x 128 1038),
 // then 128 x 128 (512 x 4096 -> 11008: 66 us, 64 x 128 69), 64 x 128 and 64 x 64 ones while those of the size before leave CUs without
 // one: a tile alone on a CU waits for its copies (256 x 4096 -> 11008: 128 x 128 48 us, 64 x 128 40; 128 x 4096 -> 4096: 48, 33,
@@ -869,13 +893,10 @@ int launch_mxfp4_gemm(const MxGemmDesc &d, hipStream_t s, CError *err) {
   if (d.K == 0) {
     hipLaunchKernelGGL(mx_k0_kernel, dim3(grid_of(d.M * d.N, 256)), dim3(256), 0, s, p);
   } else {
-    const bool big = d.M * d.N > (1L << 24);
     if (d.M <= 64)
       launch_rows(d.a_dtype == GN_MXFP4, p, s);
-    else if (d.a_dtype == GN_MXFP4 && big)
-      launch_fp4<2, 4, 4, 2, 2>(p, s);
     else if (d.a_dtype == GN_MXFP4)
-      launch_fp4<2, 2, 2, 2, 2>(p, s);
+      launch_fp4_tiles(p, s);
     else
       launch_half_tiles(p, s);
   }
