@@ -21,7 +21,8 @@ __host__ __device__ inline unsigned block_scale(uint32_t top) {
 }
 
 // Whether every code times 2^(e - 127) is an fp16 value: 0.5 2^-23 (the smallest subnormal one) to 6 2^13.
-__host__ __device__ inline bool half_exact(unsigned e) { return e >= 104 && e <= 140; }
+constexpr unsigned kHalfLeast = 104, kHalfWidth = 36;
+__host__ __device__ inline bool half_exact(unsigned e) { return e - kHalfLeast <= kHalfWidth; }
 
 struct MxGemmDesc {
   int a_dtype;

@@ -598,10 +598,10 @@ __device__ __forceinline__ void half_tile(const MxParams &p, char *smem, int tm,
   // The step's products, row by row; each fragment of A is read anew, into the same registers, once it has been used. In fp16
   // the other step's weights are converted on the way (from row `from` on), in bf16 this one's before.
   u32x4_t w[PLAIN ? 2 : 1][FN];
-  bool fits = true;
+  unsigned worst = 0;  // above the width of half_exact's range if a scale was outside of it
   auto check = [&] {
 #pragma unroll
-    for (int j = 0; j < FN; ++j) fits &= half_exact(be[j]);
+    for (int j = 0; j < FN; ++j) worst = max(worst, be[j] - kHalfLeast);
   };
   auto weight = [&](int s, int j) {
     if constexpr (PLAIN)
@@ -609,7 +609,7 @@ __device__ __forceinline__ void half_tile(const MxParams &p, char *smem, int tm,
     else
       w[0][j] = __builtin_bit_cast(u32x4_t, bf16x8_of(bq[j][s], be[j]));
   };
-  auto multiply = [&](auto step, unsigned slot, int from) {
+  auto multiply = [&](auto step, unsigned slot, int from, auto after_first) {
     constexpr int S = decltype(step)::value;
     if constexpr (!PLAIN) {
 #pragma unroll
@@ -633,6 +633,7 @@ __device__ __forceinline__ void half_tile(const MxParams &p, char *smem, int tm,
           if (from + j * (FM - from) / FN == i) weight(1 - S, j);
       }
       __builtin_amdgcn_sched_barrier(0);
+      if (i == 0) after_first();
     }
   };
 
@@ -658,19 +659,26 @@ __device__ __forceinline__ void half_tile(const MxParams &p, char *smem, int tm,
   }
   for (int t = 0; t < ns; ++t) {
     if constexpr (CHECK) check();
-    multiply(ActCode<0>{}, sl[0], 0);
+    multiply(ActCode<0>{}, sl[0], 0, [] {});
     // All but the copies of stage t + 2 and later are done: stage t + 1 is there.
     __builtin_amdgcn_s_waitcnt(vmcnt_imm(DMA ? (NS - 2) * (CA + CB) : 0));
     __syncthreads();
-    if ((t & 7) == 0) issue_scales(t / 8 + 1);
-    if constexpr (!DMA) {
-      store_a(sl[NS - 1]);
-      load_a(t + NS);
-    }
-    issue(t + NS, sl[0]);
+    auto copies = [&] {
+      if ((t & 7) == 0) issue_scales(t / 8 + 1);
+      if constexpr (!DMA) {
+        store_a(sl[NS - 1]);
+        load_a(t + NS);
+      }
+      issue(t + NS, sl[0]);
+    };
+    // The copies once the matrix instructions have work, where there are registers for it.
+    constexpr bool kLate = FM * FN < 32;
+    if constexpr (!kLate) copies();
     // Past the last stage zeros, and scales that are not looked at.
     if constexpr (PLAIN) read_b(t + 1, sl[1]);
-    multiply(ActCode<1>{}, sl[1], FM / 2);
+    multiply(ActCode<1>{}, sl[1], FM / 2, [&] {
+      if constexpr (kLate) copies();
+    });
     if constexpr (!PLAIN) read_b(t + 1, sl[1]);
     const unsigned s = sl[0];
 #pragma unroll
@@ -680,7 +688,7 @@ __device__ __forceinline__ void half_tile(const MxParams &p, char *smem, int tm,
   __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
   // No copy is under way and all waves are done with the slots: the epilogue takes their place.
   if constexpr (CHECK) {
-    if (__builtin_amdgcn_readfirstlane(__syncthreads_or(!fits))) return;
+    if (__builtin_amdgcn_readfirstlane(__syncthreads_or(worst > kHalfWidth))) return;
   } else {
     __syncthreads();
   }
@@ -757,22 +765,30 @@ void launch_half(MxParams p, hipStream_t s) {
   hipLaunchKernelGGL((mx_half_kernel<WM, WN, FM, FN, NS, WPE, DMA>), dim3((unsigned)(p.tiles_m * p.tiles_n)), dim3(WM * WN * 64), 0, s, p);
 }
 
-// More than 64 rows of 4-bit activations: the tile with which a CU's share takes the least time, the larger one of two equals.
-// A tile alone on a CU takes 0.75, 0.50, 0.35, 0.28 and 0.20 us for a stage, the first at the rate of the matrix
-// instructions, the last at the latency of its copies and barriers. Measured, us, 256 x 256 / 256 x 128 / 128 x 128 / 64 x 128 / 64 x 64:
-// 4096 -> 11008, 1024 rows 36.6 / 45.9 / 43.0 / 50.5 / 63.7, 512 rows 33.3 / 23.7 / 27.8 / 29.6 / 38.8, 200 rows 29.0 / 18.6 /
-// 15.6 / 17.5 / 19.6, 128 rows 28.0 / 18.3 / 15.3 / 11.8 / 12.3; 11008 -> 4096, 512 rows 69.9 / 47.1 / 35.1 / 28.0 / 34.2;
-// 4096 -> 4096, 65 rows 26.7 / 17.2 / 13.9 / 11.4 / 9.2.
-void launch_fp4_tiles(const MxParams &p, hipStream_t s) {
-  constexpr int kTiles[5][3] = {{256, 256, 75}, {256, 128, 50}, {128, 128, 35}, {64, 128, 28}, {64, 64, 20}};
+// More than 64 rows: the kind of tile with which a CU's share takes the least time, the largest one of equals. alone: a stage of
+// one tile on a CU, in units of 10 ns, more: of each further one of its share.
+struct TileCost {
+  int bm, bn, alone, more;
+};
+int cheapest_tile(const MxParams &p, const TileCost (&kinds)[5]) {
   int best = 0;
   long least = 0;
   for (int i = 0; i < 5; ++i) {
-    const long tiles = ((p.M + kTiles[i][0] - 1) / kTiles[i][0]) * ((p.N + kTiles[i][1] - 1) / kTiles[i][1]);
-    const long cost = (tiles + 255) / 256 * kTiles[i][2];  // 256 CUs
+    const TileCost &k = kinds[i];
+    const long tiles = ((p.M + k.bm - 1) / k.bm) * ((p.N + k.bn - 1) / k.bn);
+    const long cost = k.alone + (tiles - 1) / 256 * k.more;  // 256 CUs
     if (i == 0 || cost < least) best = i, least = cost;
   }
-  switch (best) {
+  return best;
+}
+
+// 4-bit activations: the largest tile goes at the rate of the matrix instructions, the smallest at the latency of its copies and
+// barriers. Measured, us, 256 x 256 / 256 x 128 / 128 x 128 / 64 x 128 / 64 x 64: 4096 -> 11008, 1024 rows 36.6 / 45.9 / 43.0 /
+// 50.5 / 63.7, 512 rows 33.3 / 23.7 / 27.8 / 29.6 / 38.8, 200 rows 29.0 / 18.6 / 15.6 / 17.5 / 19.6, 128 rows 28.0 / 18.3 / 15.3 /
+// 11.8 / 12.3; 11008 -> 4096, 512 rows 69.9 / 47.1 / 35.1 / 28.0 / 34.2; 4096 -> 4096, 65 rows 26.7 / 17.2 / 13.9 / 11.4 / 9.2.
+void launch_fp4_tiles(const MxParams &p, hipStream_t s) {
+  constexpr TileCost kTiles[] = {{256, 256, 75, 75}, {256, 128, 50, 50}, {128, 128, 35, 35}, {64, 128, 28, 28}, {64, 64, 20, 20}};
+  switch (cheapest_tile(p, kTiles)) {
     case 0: return launch_fp4<2, 4, 4, 2, 2>(p, s);
     case 1: return launch_fp4<4, 2, 2, 2, 2>(p, s);
     case 2: return launch_fp4<2, 2, 2, 2, 2>(p, s);
@@ -781,22 +797,22 @@ void launch_fp4_tiles(const MxParams &p, hipStream_t s) {
   }
 }
 
-// fp16 activations, more than 64 rows. 256 x 256 tiles where there is one for each CU (8192^3: 852 us, 128 x 128 1038),
-// then 128 x 128 (512 x 4096 -> 11008: 66 us, 64 x 128 69), 64 x 128 and 64 x 64 ones while those of the size before leave CUs without
-// one: a tile alone on a CU waits for its copies (256 x 4096 -> 11008: 128 x 128 48 us, 64 x 128 40; 128 x 4096 -> 4096: 48, 33,
-// 64 x 64 27). Rows of A that are not 16-byte aligned go through registers in 128 x 64 tiles.
+// The same for fp16 activations; rows of A that are not 16-byte aligned go through registers in 128 x 64 tiles. A stage of 64
+// takes a tile alone on a CU 1.42, 0.70, 0.54, 0.37 and 0.28 us; further tiles of the three smaller kinds, which share
+// the CU with it, 0.43, 0.30 and 0.13 each. Measured, us, 256 x 256 / 128 x 192 / 128 x 128 / 64 x 128 / 64 x 64: 8192^3 848 / 1078 /
+// 971 / 1144 / 1522; 4096 -> 11008, 1024 rows 113 / 122 / 116 / 125 / 156, 512 rows 98 / 55.3 / 63.9 / 59.0 / 78.2, 128 rows 96 / 49.6 /
+// 38.5 / 28.8 / 29.9; 4096 -> 4096, 2048 rows 102 / 101 / 70.2 / 81.6 / 101, 128 rows 95 / 49.9 / 39.4 / 28.3 / 24.2.
+// Waves of 128 x 32 (64 x 64: the weights of a column converted by two waves) take 39 instead of 45 us for 128 rows 4096 -> 4096.
 void launch_half_tiles(const MxParams &p, hipStream_t s) {
-  auto tiles = [&](long bm, long bn) { return ((p.M + bm - 1) / bm) * ((p.N + bn - 1) / bn); };
-  if ((uintptr_t)p.A % 16 != 0 || p.lda % 8 != 0 || p.K % 8 != 0)
-    launch_half<2, 2, 4, 2, 3, 2, false>(p, s);
-  else if (tiles(256, 256) >= 256)
-    launch_half<2, 4, 8, 4, 3, 2, true>(p, s);
-  else if (tiles(128, 128) >= 256)
-    launch_half<2, 2, 4, 4, 3, 2, true>(p, s);
-  else if (tiles(64, 128) >= 256)
-    launch_half<1, 4, 4, 2, 4, 2, true>(p, s);
-  else
-    launch_half<1, 4, 4, 1, 4, 3, true>(p, s);
+  if ((uintptr_t)p.A % 16 != 0 || p.lda % 8 != 0 || p.K % 8 != 0) return launch_half<2, 2, 4, 2, 3, 2, false>(p, s);
+  constexpr TileCost kTiles[] = {{256, 256, 142, 142}, {128, 192, 70, 78}, {128, 128, 54, 43}, {64, 128, 37, 30}, {64, 64, 28, 13}};
+  switch (cheapest_tile(p, kTiles)) {
+    case 0: return launch_half<2, 4, 8, 4, 3, 2, true>(p, s);
+    case 1: return launch_half<2, 4, 4, 3, 4, 2, true>(p, s);
+    case 2: return launch_half<1, 4, 8, 2, 3, 2, true>(p, s);
+    case 3: return launch_half<1, 4, 4, 2, 4, 3, true>(p, s);
+    default: return launch_half<1, 4, 4, 1, 4, 3, true>(p, s);
+  }
 }
 
 template <int MF, int NF, int U>
