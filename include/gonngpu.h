@@ -457,7 +457,8 @@ int gn_token_logprobs(int dtype, const void *logits, long rows, long cols, long 
  *   grad_logits[r,j] = ( g_l (1[j = targets[r]] - p_j) - g_h p_j (ln p_j + entropy[r]) ) / temperature
  * with g_l = grad_logprob[r] (0 for a target below 0) and g_h = grad_entropy[r]. grad_logits has the
  * logits' type, ldg >= cols elements from row to row, and may be the logits themselves (ldg == ld). lse and entropy are those that
- * gn_token_logprobs gave for the same logits and temperature. targets and grad_logprob may be NULL together;
+ * gn_token_logprobs gave for the same logits and temperature; p_j = e^(logits[r,j] / temperature - lse) has a relative error of
+ * about |lse| 2^-23 from the rounding of lse. targets and grad_logprob may be NULL together;
  * so may entropy and grad_entropy. A row with an lse of -2^100 or
  * less (all columns masked, by -inf or the type's lowest value) has gradient 0; one with NaN or +inf, or with a target of cols or
  * above, NaN. Where both of a row's gradients are 0 its gradient is 0 whatever the logits hold. */
@@ -478,7 +479,7 @@ int gn_distill_forward(int dtype, const void *logits, long rows, long cols, long
                        const int64_t *ids, const float *teacher, int k, float *loss, float *lse, void *workspace,
                        size_t workspace_bytes, void *stream, CError *err);
 /* grad_logits[r,j] = grad_loss[r] temperature (q_j - sum over i with ids[r,i] = j of p_i), in the logits'
- * type; lse from gn_distill_forward (with -2^100 or less q is 0); grad_logits may be the logits themselves (ldg == ld). A row whose
+ * type; lse from gn_distill_forward (with -2^100 or less q is 0; q has the error of p in gn_token_logprobs_backward); grad_logits may be the logits themselves (ldg == ld). A row whose
  * grad_loss is 0 has gradient 0 whatever the logits hold. */
 int gn_distill_backward(int dtype, const void *logits, long rows, long cols, long ld, float temperature,
                         const int64_t *ids, const float *teacher, int k, const float *lse, const float *grad_loss,

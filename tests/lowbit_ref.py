@@ -93,9 +93,10 @@ def distill(x, ids, teacher, temperature):
         at = [i for i in range(ids.shape[1]) if ids[r, i] >= 0 and teacher[r, i] != -math.inf]
         if not at:
             continue
-        p = torch.softmax(teacher[r, at].double() / temperature, 0)
+        logp = torch.log_softmax(teacher[r, at].double() / temperature, 0)  # finite where p itself underflows
+        p = logp.exp()
         where = ids[r, at]
-        loss[r] = temperature**2 * (p * (p.log() - (z[r, where] - lse[r]))).sum()
+        loss[r] = temperature**2 * (p * (logp - (z[r, where] - lse[r]))).sum()
         grad[r] = temperature * torch.exp(z[r] - lse[r])
         grad[r].index_add_(0, where, -temperature * p)
     return loss, lse, grad

@@ -181,6 +181,31 @@ def _grad_bound(ref, x, scale, temperature, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("exponent", [-2, -7, -12, -20, -100])
+@pytest.mark.parametrize("cols", [50, 3000])
+def test_small_temperatures(dev, cols, exponent, dtype):
+    """Large logits over small temperatures: m / T is past what fp32 holds ln s beside, or past any use of it, and the
+    log-probabilities are those of the differences to the maximum, which are exact here. Each has a few half-steps of its own, and
+    ln s no more than 160."""
+    x = _logits(4, cols, torch.float32, cols, spread=20.0).round()
+    x[0] += 60000
+    x[1] -= 50000
+    x[2, cols // 2:] = x[2].amax()  # many equal ones
+    x[3, 1] = x[3, cols - 1] = 65000  # two
+    x = x.to(dtype)
+    temperature, targets = 2.0**exponent, torch.tensor([0, 1, cols - 1, 1])
+    lp, lse, h, ids, tops = _forward(dev, x.to(dev), targets.to(dev), 3, temperature)
+    # 64 bits have no room either for ln s beside m / T (2^116 has steps of 2^63): of the differences, which are exact.
+    m = x.double().amax(1)
+    r = R.logprobs(x.double() - m[:, None], targets, 3, temperature)
+    _close(lp, r[0], E * (4 * r[0].abs() + 160))
+    _close(lse, m / temperature + r[1], E * (4 * (m / temperature + r[1]).abs() + 160))
+    _close(h, r[2], E * 512 * (1 + r[2]))
+    assert torch.equal(ids.cpu(), r[3])
+    _close(tops, r[4], E * (4 * r[4].abs() + 160))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
 @pytest.mark.parametrize("rows,cols", [(1, 1), (2, 3), (5, 100), (4, 1001), (3, 8192), (2, 40003)])
 def test_logprobs_backward(dev, rows, cols, dtype):
     for temperature, masked in ((1.0, 0.0), (2.5, 0.6)):
@@ -323,6 +348,21 @@ def test_distill(dev, rows, cols, k, temperature, dtype):
     x = _logits(rows, cols, dtype, cols + k)
     _check_distill(dev, x, *_teacher(rows, cols, k, k), temperature)
     _check_distill(dev, x, *_teacher(rows, cols, k, k), temperature, in_place=True)
+
+
+@pytest.mark.parametrize("exponent", [-2, -20, -100])
+def test_distill_small_temperatures(dev, exponent):
+    """Quotients that fp32 holds only as differences to the maximum; these are exact, each ln p has two roundings of its own and 160
+    half-steps of ln s, and a term its p's 160 and a rounding."""
+    T, x = 2.0**exponent, _logits(3, 500, torch.float16, 1, spread=30.0).round() + 40000
+    ids, t = _teacher(3, 500, 6, 2)
+    t = (t * 8).round() + 1e6
+    loss = torch.empty(3, device=dev)
+    G.distill(x.to(dev), ids.to(dev), t.to(dev), loss, temperature=T)
+    t = t.double() - torch.where(ids >= 0, t, -math.inf).amax(1, keepdim=True).double()
+    x = x.double() - x.double().amax(1, keepdim=True)
+    size = T * T * ((t.abs() + torch.gather(x, 1, ids.clamp_min(0)).abs()) / T + 8).amax(1)
+    _close(loss, R.distill(x, ids, t, T)[0], E * 6 * 400 * size)
 
 
 def test_distill_absent_and_repeated_entries(dev):
