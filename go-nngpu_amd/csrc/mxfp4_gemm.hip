@@ -309,8 +309,8 @@ __device__ __forceinline__ float16_t mfma32_fp4(u32x4_t a, u32x4_t b, float16_t 
 // wave they cost one cache line to a row and stage, and with two stages of 256 in flight that bound the kernel
 // (8192^3 369 us). A step multiplies while the next one's fragments are read; before a stage's second step the next
 // stage has landed (one wait and one barrier to a stage), and the copies of the one kSlots ahead go into the slot just left.
-// 8192^3 takes 297 us (3.7 PFLOP/s): the loop goes at 4.7, at the power that the card may draw, and some 60 us are the
-// tiles' ends, where all CUs write C at once. Smaller tiles read a fragment of LDS for each matrix instruction and are
+// 8192^3 takes 297 us (3.7 PFLOP/s): the loop goes at 4.7, and some 60 us are the tiles' ends, where all CUs write C at
+// once (the matrix units are busy for half of the cycles, waves wait for 38%). Smaller tiles read a fragment of LDS for each matrix instruction and are
 // bound by that and by the barriers (512 rows, 4096 -> 11008: 23.7 us; the operations alone 7, C alone 5).
 constexpr int kSlots = 4;
 template <int WM, int WN, int FM, int FN, int WPE>
