@@ -391,6 +391,12 @@ def _expect(what, t, dtype, n):
         _refuse(f"{what}: {n} contiguous values of {dtype} are needed, got {t.dtype} {tuple(t.shape)}")
 
 
+def _expect_rows(what, t, dtype, rows, width):
+    """The same of an array of rows x width."""
+    if t.dtype is not dtype or t.dim() != 2 or t.size(0) != rows or t.numel() != rows * width or not t.is_contiguous():
+        _refuse(f"{what}: {rows} x {width} contiguous values of {dtype} are needed, got {t.dtype} {tuple(t.shape)}")
+
+
 def _matrix(what, t):
     """(GN_F32 or GN_F16, rows, cols, elements from row to row) of a matrix whose rows are dense."""
     T = _types()
@@ -411,9 +417,9 @@ def _matrix(what, t):
 
 def _mxfp4_matrix(what, data, scales, rows, cols):
     """Checks the two arrays of a stored MXFP4 matrix."""
-    u8, groups = _types().uint8, rows * (-(-cols // 128))
-    _expect(what, data, u8, 64 * groups)
-    _expect(what, scales, u8, 4 * groups)
+    u8, groups = _types().uint8, -(-cols // 128)
+    _expect_rows(what, data, u8, rows, 64 * groups)
+    _expect_rows(what, scales, u8, rows, 4 * groups)
 
 
 def _width(t):
@@ -508,8 +514,8 @@ def token_logprobs(logits, targets, logprob, *, lse=None, entropy=None, top_ids=
     k = 0
     if top_ids is not None:
         k = _width(top_ids)
-        _expect("token_logprobs: top_ids", top_ids, T.int64, rows * k)
-        _expect("token_logprobs: top_logprobs", top_logprobs, T.float32, rows * k)
+        _expect_rows("token_logprobs: top_ids", top_ids, T.int64, rows, k)
+        _expect_rows("token_logprobs: top_logprobs", top_logprobs, T.float32, rows, k)
     if targets is not None:
         _expect("token_logprobs: targets", targets, T.int64, rows)
     for what, t in (("logprob", logprob), ("lse", lse), ("entropy", entropy)):
@@ -551,8 +557,8 @@ def distill(logits, ids, teacher, loss, *, lse=None, temperature=1.0, stream_ptr
     T = _types()
     dt, rows, cols, ld = _matrix("distill", logits)
     k = _width(ids)
-    _expect("distill: ids", ids, T.int64, rows * k)
-    _expect("distill: teacher", teacher, T.float32, rows * k)
+    _expect_rows("distill: ids", ids, T.int64, rows, k)
+    _expect_rows("distill: teacher", teacher, T.float32, rows, k)
     for what, t in (("loss", loss), ("lse", lse)):
         if t is not None:
             _expect("distill: " + what, t, T.float32, rows)
@@ -570,8 +576,8 @@ def distill_backward(logits, ids, teacher, lse, grad_loss, grad_logits, *, tempe
     if (dg, grows, gcols) != (dt, rows, cols):
         _refuse("distill_backward: grad_logits has the type and shape of logits")
     k = _width(ids)
-    _expect("distill_backward: ids", ids, T.int64, rows * k)
-    _expect("distill_backward: teacher", teacher, T.float32, rows * k)
+    _expect_rows("distill_backward: ids", ids, T.int64, rows, k)
+    _expect_rows("distill_backward: teacher", teacher, T.float32, rows, k)
     _expect("distill_backward: lse", lse, T.float32, rows)
     _expect("distill_backward: grad_loss", grad_loss, T.float32, rows)
     device = _device_of(logits, ids, teacher, lse, grad_loss, grad_logits)

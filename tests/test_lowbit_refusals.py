@@ -127,6 +127,9 @@ BINDING = [
     ("rows of A", lambda: G.mxfp4_gemm(_t(4, 8, dtype=H), _pair(3, 8), _t(2, 3))),
     ("gemm: B", lambda: G.mxfp4_gemm(_t(2, 8, dtype=H), _pair(4, 8), _t(2, 3))),
     ("gemm: B", lambda: G.mxfp4_gemm(_pair(2, 129), _pair(3, 128), _t(2, 3), K=129)),
+    # as many values, other rows
+    ("gemm: A", lambda: G.mxfp4_gemm(_pair(3, 256), _pair(3, 128), _t(6, 3), K=128)),
+    ("gemm: B", lambda: G.mxfp4_gemm(_t(2, 128, dtype=H), _pair(3, 256), _t(2, 6))),
     ("bias", lambda: G.mxfp4_gemm(_t(2, 8, dtype=H), _pair(3, 8), _t(2, 3), bias=_t(2))),
     ("together", lambda: G.token_logprobs(_t(2, 8), _t(2, dtype=I64), None)),
     ("together", lambda: G.token_logprobs(_t(2, 8), None, None, top_ids=_t(2, 3, dtype=I64))),
@@ -138,6 +141,7 @@ BINDING = [
     ("together", lambda: G.token_logprobs_backward(_t(2, 8), None, _t(2), None, _t(2, 8), entropy=_t(2))),
     ("ids", lambda: G.distill(_t(2, 8), _t(2, 3), _t(2, 3), _t(2))),
     ("teacher", lambda: G.distill(_t(2, 8), _t(2, 3, dtype=I64), _t(2, 4), _t(2))),
+    ("teacher", lambda: G.distill(_t(2, 8), _t(2, 3, dtype=I64), _t(3, 2), _t(2))),
     ("loss", lambda: G.distill(_t(2, 8), _t(2, 3, dtype=I64), _t(2, 3), _t(3))),
     ("type and shape", lambda: G.distill_backward(_t(2, 8), _t(2, 3, dtype=I64), _t(2, 3), _t(2), _t(2), _t(2, 9))),
     ("grad_loss", lambda: G.distill_backward(_t(2, 8), _t(2, 3, dtype=I64), _t(2, 3), _t(2), _t(2, dtype=H), _t(2, 8))),
