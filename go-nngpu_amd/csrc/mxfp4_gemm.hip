@@ -474,7 +474,7 @@ mx_fp4_kernel(MxParams p) {
 // wave's read of 16 rows is 512 consecutive ones) and lie in one block. A row's scales for 8 stages are 16 bytes in LDS. The
 // scales are applied as in the few-rows kernel: in fp16 where all of the wave's allow it, else in bf16.
 // 8192^3 takes 820 us (1.34 PFLOP/s, the rate of a large bf16 library product on this card: its power); smaller products wait for LDS and
-// the barriers between stages (128 x 128 tiles without their matrix instructions take 85% of their time, without their copies 75%).
+// the barriers between stages (128 x 128 tiles without their matrix instructions took 85% of their time, without their copies 75%).
 // DMA: A is copied to LDS by dma16 (16-byte aligned rows, K a multiple of 8); otherwise through registers, its tail masked.
 template <int WM, int WN, int FM, int FN, int NS>
 struct HalfTile {
@@ -818,15 +818,15 @@ void launch_fp4_tiles(const MxParams &p, hipStream_t s) {
   }
 }
 
-// The same for fp16 activations; rows of A that are not 16-byte aligned go through registers in 128 x 64 tiles. A stage of 64
-// takes a tile alone on a CU 1.42, 0.70, 0.54, 0.37 and 0.28 us; further tiles of the three smaller kinds, which share
-// the CU with it, 0.43, 0.30 and 0.13 each. Measured, us, 256 x 256 / 128 x 192 / 128 x 128 / 64 x 128 / 64 x 64: 8192^3 848 / 1078 /
-// 971 / 1144 / 1522; 4096 -> 11008, 1024 rows 113 / 122 / 116 / 125 / 156, 512 rows 98 / 55.3 / 63.9 / 59.0 / 78.2, 128 rows 96 / 49.6 /
-// 38.5 / 28.8 / 29.9; 4096 -> 4096, 2048 rows 102 / 101 / 70.2 / 81.6 / 101, 128 rows 95 / 49.9 / 39.4 / 28.3 / 24.2.
-// Waves of 128 x 32 (64 x 64: the weights of a column converted by two waves) take 39 instead of 45 us for 128 rows 4096 -> 4096.
+// The same for fp16 activations; rows of A that are not 16-byte aligned go through registers in 128 x 64 tiles. Two tiles of the
+// three smaller kinds share a CU and its time. Measured, us, 256 x 256 / 128 x 192 / 128 x 128 / 64 x 128 / 64 x 64: 8192^3 825 / 1001 /
+// 925 / 1073 / 1401; 4096 -> 11008, 1024 rows 111 / 115 / 105 / 114 / 143, 512 rows 98 / 52.6 / 62.8 / 55.6 / 70.8, 256 rows 97 / 46.2 /
+// 38.4 / 36.7 / 37.0, 128 rows 96 / 46.0 / 37.6 / 24.6 / 25.7; 4096 -> 4096, 2048 rows 102 / 95 / 67.3 / 74.0 / 90.6, 128 rows 95 /
+// 45.6 / 37.6 / 23.5 / 19.8. Waves of 128 x 32 (64 x 64: the weights of a column converted by two waves) took 39 instead of 45 us
+// for the 128 x 128 tiles of 128 rows 4096 -> 4096.
 void launch_half_tiles(const MxParams &p, hipStream_t s) {
   if ((uintptr_t)p.A % 16 != 0 || p.lda % 8 != 0 || p.K % 8 != 0) return launch_half<2, 2, 4, 2, 3, 2, false>(p, s);
-  constexpr TileCost kTiles[] = {{256, 256, 142, 142}, {128, 192, 70, 78}, {128, 128, 54, 43}, {64, 128, 37, 30}, {64, 64, 28, 13}};
+  constexpr TileCost kTiles[] = {{256, 256, 142, 142}, {128, 192, 64, 71}, {128, 128, 55, 38}, {64, 128, 30, 24}, {64, 64, 24, 14}};
   switch (cheapest_tile(p, kTiles)) {
     case 0: return launch_half<2, 4, 8, 4, 3, 2, true>(p, s);
     case 1: return launch_half<2, 4, 4, 3, 4, 2, true>(p, s);

@@ -133,7 +133,8 @@ def _bounded(y, a, w, K, more=0.0, alpha=1.0, slope=1.0):
 SIZES = [(1, 1, 1), (1, 16, 32), (1, 300, 4096), (2, 33, 100), (3, 128, 129), (5, 77, 1000), (16, 1000, 512), (17, 64, 640),
          (27, 500, 2027), (33, 257, 384), (64, 130, 96), (65, 129, 257), (100, 260, 1024), (128, 128, 128), (129, 256, 256),
          (200, 300, 515), (256, 512, 768), (300, 700, 1300), (513, 300, 260), (520, 1030, 4096),
-         (100, 9000, 200), (200, 9000, 130), (300, 11000, 260), (1000, 11000, 140)]  # with 4-bit activations: each tile
+         (100, 9000, 200), (200, 9000, 130), (300, 11000, 260), (1000, 11000, 140),
+         (400, 11000, 328), (3900, 4000, 200)]  # these: each tile of both kinds
 
 
 @pytest.mark.parametrize("M,N,K", SIZES)
@@ -169,7 +170,8 @@ def test_product_scales_over_the_whole_range(dev, M, N, K, fp4):
     _bounded(y.cpu(), a, R.values(*w, K), K)
 
 
-@pytest.mark.parametrize("M,N,K", [(1, 40, 256), (20, 600, 384), (70, 200, 512), (270, 300, 128), (3000, 5700, 64)])
+@pytest.mark.parametrize("M,N,K", [(1, 40, 256), (20, 600, 384), (70, 200, 512), (270, 300, 128), (140, 9000, 64), (400, 11000, 64),
+                                   (1000, 11000, 64), (3000, 5700, 64), (3900, 4000, 64)])
 @pytest.mark.parametrize("lo,hi", [(104, 114), (114, 141), (137, 145), (100, 108)])
 def test_product_scales_at_the_ends_of_fp16(dev, M, N, K, lo, hi):
     """Scales whose weights are all fp16 numbers, the subnormal ones included, and scales around both ends of that range."""
