@@ -145,7 +145,9 @@ __device__ __forceinline__ RowStats segment_stats(const Segment<S, E> &x, float 
   }
   return r;
 }
-__device__ __forceinline__ float lse_of(const RowStats &r, float inv_t) { return r.s == 0.0f ? -INFINITY : fmaf(r.m, inv_t, log2f(r.s) * kLn2); }
+__device__ __forceinline__ float lse_of(const RowStats &r, float inv_t) {
+  return r.s == 0.0f ? -INFINITY : fmaf(r.m, inv_t, log2f(r.s) * kLn2);
+}
 __device__ __forceinline__ float entropy_of(const RowStats &r) { return r.s == 0.0f ? 0.0f : (log2f(r.s) - r.t / r.s) * kLn2; }
 // Of x, from its distance to the maximum: lse may be too large to hold ln s beside it.
 __device__ __forceinline__ float logprob_of(float x, const RowStats &r, float inv_t) {

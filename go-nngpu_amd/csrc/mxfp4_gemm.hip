@@ -80,9 +80,9 @@ __device__ __forceinline__ float finish(const MxParams &p, float acc, long m, lo
 }
 
 // ------------------------------------------------------------------ few rows
-// Up to 64 rows: bound by the stream of B (1 row 4096 -> 11008: 24 MB in 9.2 us with the launch). A workgroup owns some columns for all rows; its waves cut K among them, whole
-// groups each, and the partial sums meet in LDS. Lane (r, g) = (lane % 16, lane / 16) takes block g of row r's group, 16
-// consecutive bytes, so a wave reads whole 64-byte pieces of 16 rows of B, straight into registers.
+// Up to 64 rows: bound by the stream of B (1 row 4096 -> 11008: 24 MB in 9.2 us with the launch). A workgroup owns some
+// columns for all rows; its waves cut K among them, whole groups each, and the partial sums meet in LDS. Lane (r, g) =
+// (lane % 16, lane / 16) takes block g of row r's group, 16 consecutive bytes, so a wave reads whole 64-byte pieces of 16 rows of B, straight into registers.
 
 // Adds the waves' partial sums and writes C: `part` holds [wk][blocks][64] of them, each block 16 x 16, block j MF + i the
 // rows m0 + 16 i .. and the columns n0 + 16 j ... Lane (r, g) of a block has rows 4 g .. 4 g + 3 of column r.
@@ -310,8 +310,8 @@ __device__ __forceinline__ float16_t mfma32_fp4(u32x4_t a, u32x4_t b, float16_t 
 // (8192^3 369 us). A step multiplies while the next one's fragments are read; before a stage's second step the next
 // stage has landed (one wait and one barrier to a stage), and the copies of the one kSlots ahead go into the slot just left.
 // 8192^3 takes 297 us (3.7 PFLOP/s): the loop goes at 4.7, and some 60 us are the tiles' ends, where all CUs write C at
-// once (the matrix units are busy for half of the cycles, waves wait for 38%). Smaller tiles read a fragment of LDS for each matrix instruction and are
-// bound by that and by the barriers (512 rows, 4096 -> 11008: 23.7 us; the operations alone 7, C alone 5).
+// once (the matrix units are busy for half of the cycles, waves wait for 38%). Smaller tiles read a fragment of LDS for each
+// matrix instruction and are bound by that and by the barriers (512 rows, 4096 -> 11008: 23.7 us; the operations alone 7, C alone 5).
 constexpr int kSlots = 4;
 template <int WM, int WN, int FM, int FN, int WPE>
 __global__ void __launch_bounds__(WM * WN * 64) __attribute__((amdgpu_waves_per_eu(WPE, WPE)))

@@ -479,8 +479,8 @@ int gn_distill_forward(int dtype, const void *logits, long rows, long cols, long
                        const int64_t *ids, const float *teacher, int k, float *loss, float *lse, void *workspace,
                        size_t workspace_bytes, void *stream, CError *err);
 /* grad_logits[r,j] = grad_loss[r] temperature (q_j - sum over i with ids[r,i] = j of p_i), in the logits'
- * type; lse from gn_distill_forward (with -2^100 or less q is 0; q has the error of p in gn_token_logprobs_backward); grad_logits may be the logits themselves (ldg == ld). A row whose
- * grad_loss is 0 has gradient 0 whatever the logits hold. */
+ * type; lse from gn_distill_forward (with -2^100 or less q is 0; q has the error of p in gn_token_logprobs_backward);
+ * grad_logits may be the logits themselves (ldg == ld). A row whose grad_loss is 0 has gradient 0 whatever the logits hold. */
 int gn_distill_backward(int dtype, const void *logits, long rows, long cols, long ld, float temperature,
                         const int64_t *ids, const float *teacher, int k, const float *lse, const float *grad_loss,
                         void *grad_logits, long ldg, void *stream, CError *err);

@@ -130,7 +130,8 @@ def _bounded(y, a, w, K, more=0.0, alpha=1.0, slope=1.0):
     return ref
 
 
-SIZES = [(1, 1, 1), (1, 16, 32), (1, 300, 4096), (2, 33, 100), (3, 128, 129), (5, 77, 1000), (16, 1000, 512), (17, 64, 640),
+SIZES = [(1, 1, 1), (2, 3, 9), (70, 90, 1), (80, 100, 8), (100, 70, 33), (65, 1, 128), (300, 1, 264),
+         (1, 16, 32), (1, 300, 4096), (2, 33, 100), (3, 128, 129), (5, 77, 1000), (16, 1000, 512), (17, 64, 640),
          (27, 500, 2027), (33, 257, 384), (64, 130, 96), (65, 129, 257), (100, 260, 1024), (128, 128, 128), (129, 256, 256),
          (200, 300, 515), (256, 512, 768), (300, 700, 1300), (513, 300, 260), (520, 1030, 4096),
          (100, 9000, 200), (200, 9000, 130), (300, 11000, 260), (1000, 11000, 140),
