@@ -8,6 +8,7 @@ GonngpuUnavailable; there is no CPU fallback.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 import re
 import threading
@@ -190,7 +191,8 @@ def call(name, *args):
     err = getattr(_errors, "err", None)
     if err is None:
         err = _errors.err = CError()
-    rc = getattr(L, name)(*args, ctypes.byref(err))
+        _errors.ref = ctypes.byref(err)
+    rc = getattr(L, name)(*args, _errors.ref)
     _check(rc, err)
     return rc
 
@@ -489,17 +491,24 @@ def mxfp4_gemm(A, B, C, *, alpha=1.0, beta=0.0, bias=None, act=ACT_NONE, act_alp
                  B[1].data_ptr(), beta, C.data_ptr(), ldc, _ptr(bias), act, act_alpha)
 
 
-def _logits_workspace(rows, cols, k, device, stream_ptr):
+@functools.lru_cache(maxsize=256)
+def _logits_workspace_bytes(rows, cols, k):
+    return load().gn_logits_workspace(rows, cols, k)
+
+
+def _logits_workspace(logits, rows, cols, k, device, stream_ptr):
     """Scratch for one call, from torch's allocator (which keeps what a captured graph uses), of the pool of the stream
-    that the call runs on: a block of another stream's pool may still be in use there."""
+    that the call runs on: a block of another stream's pool may still be in use there. Asked for in the logits' type (the
+    bytes are a multiple of 8): naming a type and a device takes 1.3 us more."""
     T = _types()
-    n = load().gn_logits_workspace(rows, cols, k)
+    n = _logits_workspace_bytes(rows, cols, k)
     if n == 0:
         return None, 0
+    size = n // (4 if logits.dtype is T.float32 else 2)
     if stream_ptr is None or stream_ptr == _current_stream(device):
-        return T.empty((n,), dtype=T.uint8, device=T.device("cuda", device)), n
+        return logits.new_empty((size,)), n
     with T.cuda.stream(T.cuda.ExternalStream(stream_ptr or stream(), device=device)):
-        return T.empty((n,), dtype=T.uint8, device=T.device("cuda", device)), n
+        return logits.new_empty((size,)), n
 
 
 def token_logprobs(logits, targets, logprob, *, lse=None, entropy=None, top_ids=None, top_logprobs=None,
@@ -522,7 +531,7 @@ def token_logprobs(logits, targets, logprob, *, lse=None, entropy=None, top_ids=
         if t is not None:
             _expect("token_logprobs: " + what, t, T.float32, rows)
     device = _device_of(logits, targets, logprob, lse, entropy, top_ids, top_logprobs)
-    ws, n = _logits_workspace(rows, cols, k, device, stream_ptr)
+    ws, n = _logits_workspace(logits, rows, cols, k, device, stream_ptr)
     _dispatch_on(device, stream_ptr, "gn_token_logprobs", dt, logits.data_ptr(), rows, cols, ld, temperature,
                  _ptr(targets), _ptr(logprob), _ptr(lse), _ptr(entropy), k, _ptr(top_ids), _ptr(top_logprobs),
                  _ptr(ws), n)
@@ -563,7 +572,7 @@ def distill(logits, ids, teacher, loss, *, lse=None, temperature=1.0, stream_ptr
         if t is not None:
             _expect("distill: " + what, t, T.float32, rows)
     device = _device_of(logits, ids, teacher, loss, lse)
-    ws, n = _logits_workspace(rows, cols, 0, device, stream_ptr)
+    ws, n = _logits_workspace(logits, rows, cols, 0, device, stream_ptr)
     _dispatch_on(device, stream_ptr, "gn_distill_forward", dt, logits.data_ptr(), rows, cols, ld, temperature, ids.data_ptr(),
                  teacher.data_ptr(), k, loss.data_ptr(), _ptr(lse), _ptr(ws), n)
 
