@@ -82,7 +82,8 @@ __device__ __forceinline__ float finish(const MxParams &p, float acc, long m, lo
 // ------------------------------------------------------------------ few rows
 // Up to 64 rows: bound by the stream of B (1 row 4096 -> 11008: 24 MB in 9.2 us with the launch). A workgroup owns some
 // columns for all rows; its waves cut K among them, whole groups each, and the partial sums meet in LDS. Lane (r, g) =
-// (lane % 16, lane / 16) takes block g of row r's group, 16 consecutive bytes, so a wave reads whole 64-byte pieces of 16 rows of B, straight into registers.
+// (lane % 16, lane / 16) takes block g of row r's group, 16 consecutive bytes, so a wave reads whole 64-byte pieces of 16
+// rows of B, straight into registers.
 
 // Adds the waves' partial sums and writes C: `part` holds [wk][blocks][64] of them, each block 16 x 16, block j MF + i the
 // rows m0 + 16 i .. and the columns n0 + 16 j ... Lane (r, g) of a block has rows 4 g .. 4 g + 3 of column r.
