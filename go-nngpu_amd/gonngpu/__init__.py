@@ -498,16 +498,20 @@ def _logits_workspace_bytes(rows, cols, k):
 
 def _logits_workspace(logits, rows, cols, k, device, stream_ptr):
     """Scratch for one call, from torch's allocator (which keeps what a captured graph uses), of the pool of the stream
-    that the call runs on: a block of another stream's pool may still be in use there. Asked for in the logits' type (the
-    bytes are a multiple of 8): naming a type and a device takes 1.3 us more."""
+    that the call runs on: a block of another stream's pool may still be in use there. A handle of 0 asked for is the library's
+    stream, whereas torch's default stream, whose handle is 0 too, is None asked for (the call is then waited for). Asked
+    for in the logits' type (the bytes are a multiple of 8): naming a type and a device takes 1.3 us more."""
     T = _types()
     n = _logits_workspace_bytes(rows, cols, k)
     if n == 0:
         return None, 0
     size = n // (4 if logits.dtype is T.float32 else 2)
-    if stream_ptr is None or stream_ptr == _current_stream(device):
+    if stream_ptr is None:
         return logits.new_empty((size,)), n
-    with T.cuda.stream(T.cuda.ExternalStream(stream_ptr or stream(), device=device)):
+    stream_ptr = stream_ptr or stream()
+    if stream_ptr == _current_stream(device):
+        return logits.new_empty((size,)), n
+    with T.cuda.stream(T.cuda.ExternalStream(stream_ptr, device=device)):
         return logits.new_empty((size,)), n
 
 
