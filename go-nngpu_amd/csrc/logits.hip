@@ -176,14 +176,16 @@ __device__ __forceinline__ RowStats join_stats(const RowStats *stats, int segs, 
 // ------------------------------------------------------------------ the top alternatives
 // Their order is the larger value first, then the lower column. A float's bits as an unsigned number that is ordered as
 // the values are (NaN above infinity, -0 as 0), and with the column below it a key of its own for each entry. 0: no entry
-// (of a float, only a negative NaN would have it).
+// (of a float, only a negative NaN would have it). NaN's is not the largest word: with column 0's complement, which is, the key
+// would be the one that the search for the best starts below.
+constexpr uint32_t kNanKey = 0xfffffffeu;
 __device__ __forceinline__ uint32_t value_key(float x) {
   const uint32_t b = __float_as_uint(x + 0.0f);
-  if ((b & 0x7fffffffu) > 0x7f800000u) return 0xffffffffu;
+  if ((b & 0x7fffffffu) > 0x7f800000u) return kNanKey;
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float key_value(uint32_t k) {
-  if (k == 0xffffffffu) return NAN;
+  if (k == kNanKey) return NAN;
   return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
 __device__ __forceinline__ uint64_t entry_key(uint32_t value, uint32_t col) { return ((uint64_t)value << 32) | ~col; }

@@ -521,3 +521,18 @@ def test_offsets_past_32_bits(dev):
     bound = _grad_bound(ref, xs, scale, 1.0, torch.float16)
     bound.scatter_add_(1, tid.cpu()[pick], torch.full((5, 4), 2048.0 * 400 * E, dtype=torch.float64))
     _close(x[pick.to(dev)], ref, bound)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("cols", [1, 2, 64, 5000, 33000])
+def test_nan_in_the_first_column(dev, cols, dtype):
+    """NaN is the largest value in column 0 as in any other: alone, among numbers, beside other NaN, and where all are NaN. Every
+    column named is one of the row's."""
+    x = _logits(5, cols, dtype, 23)
+    x[0, 0] = math.nan
+    x[1] = math.nan
+    x[2, 0] = x[2, cols // 2] = x[2, cols - 1] = math.nan
+    x[3, 0], x[3, cols - 1] = -math.nan, math.inf
+    targets = torch.tensor([0, cols - 1, 0, cols // 2, 0])
+    for k in {1, min(cols, 5), min(cols, 64)}:
+        _check_forward(dev, x, targets, k, 1.0)
