@@ -559,8 +559,9 @@ int check_logits(const char *what, const LogitsDesc &d, CError *err) {
   if (d.dtype != GN_F32 && d.dtype != GN_F16) return set_error(err, -1, "%s: unsupported dtype %d", what, d.dtype);
   if (d.rows < 0 || d.cols < 1 || d.cols > INT_MAX)
     return set_error(err, -1, "%s: invalid size %ld x %ld", what, d.rows, d.cols);
-  if (!(d.temperature > 0.0f) || !(1.0f / d.temperature > 0.0f) || !(1.0f / d.temperature < INFINITY))
-    return set_error(err, -1, "%s: a temperature above 0 and finite, with a finite reciprocal, is needed", what);
+  // The kernels multiply by c = log2(e) / T, and 0 times an infinite one would be NaN.
+  if (!(d.temperature > 0.0f) || !(1.0f / d.temperature > 0.0f) || !(1.0f / d.temperature * kLog2e < INFINITY))
+    return set_error(err, -1, "%s: a temperature above 0 and finite, with a finite log2(e) / temperature, is needed", what);
   if (d.ld < d.cols) return set_error(err, -1, "%s: leading dimension %ld smaller than row length %ld", what, d.ld, d.cols);
   // A workgroup to 2048 columns and more of a row, below 2^24 of them (2^32 threads).
   if (!matrix_bytes(d.rows, d.ld, 4, &n) || n > ((size_t)1 << 62) || d.rows >= (1L << 24) / ((d.cols + 8191) / 8192))

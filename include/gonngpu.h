@@ -438,7 +438,8 @@ int gn_mxfp4_gemm(int a_dtype, long M, long N, long K, float alpha, const void *
                   float act_alpha, void *stream, CError *err);
 
 /* Rows of logits (GN_F32 or GN_F16, rows x cols, cols >= 1, ld >= cols elements from row to row), z = x / temperature in
- * fp32 (x times the temperature's fp32 reciprocal), temperature finite and above 0:
+ * fp32 (x times the temperature's fp32 reciprocal), temperature finite and above 0, with a finite log2(e) / temperature in
+ * fp32 (from 4.3e-39 up):
  *   lse[r] = ln sum_j e^z[r,j]      logprob[r] = z[r, targets[r]] - lse[r]
  *   entropy[r] = - sum_j p_j ln p_j, p = e^(z - lse)
  *   top_ids[r, 0..k), top_logprobs[r, 0..k): the k largest logits' columns and z - lse, largest first, the

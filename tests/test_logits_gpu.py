@@ -536,3 +536,15 @@ def test_nan_in_the_first_column(dev, cols, dtype):
     targets = torch.tensor([0, cols - 1, 0, cols // 2, 0])
     for k in {1, min(cols, 5), min(cols, 64)}:
         _check_forward(dev, x, targets, k, 1.0)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_smallest_and_largest_temperatures(dev, dtype):
+    """The ends of what is accepted: one column is left at the smallest, all are equally likely at the largest."""
+    x = torch.tensor([[-3.0, 2.0, -5.0, 1.5, -math.inf], [-8.0, -4.0, -6.0, -4.5, -5.0]]).to(dtype)
+    lp, lse, h, ids, tops = _forward(dev, x.to(dev), torch.tensor([1, 1], device=dev), 2, 4.3e-39)
+    assert lp.tolist() == [0.0, 0.0] and h.tolist() == [0.0, 0.0] and ids.tolist() == [[1, 3], [1, 3]]
+    assert tops[:, 0].tolist() == [0.0, 0.0] and bool((tops[:, 1] < -1e37).all())
+    lp, lse, h, ids, tops = _forward(dev, x.to(dev), torch.tensor([1, 1], device=dev), 2, 3.4e38)
+    for r, n in enumerate((4, 5)):
+        assert abs(lp[r].item() + math.log(n)) <= 32 * E and abs(h[r].item() - math.log(n)) <= 64 * E

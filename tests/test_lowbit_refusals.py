@@ -154,3 +154,11 @@ def test_binding_refuses(i):
     word, call = BINDING[i]
     with pytest.raises(G.GonngpuError, match=word):
         call()
+
+
+@pytest.mark.parametrize("name,good", [("gn_token_logprobs", LOGPROBS), ("gn_token_logprobs_backward", LOGPROBS_GRAD),
+                                       ("gn_distill_forward", DISTILL), ("gn_distill_backward", DISTILL_GRAD)])
+@pytest.mark.parametrize("temperature", [1e-45, 2.9e-39, 2.95e-39, 3.5e-39, 4.23e-39])
+def test_temperature_whose_exponents_would_be_infinite(name, good, temperature):
+    """The reciprocal may be finite, but not its product with log2(e), which the exponents are multiplied with."""
+    _refused("temperature", name, *{**good, "temp": temperature}.values())
