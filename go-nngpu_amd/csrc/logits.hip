@@ -410,9 +410,12 @@ __device__ __forceinline__ void finish_distill(const DistillDesc &p, long r, con
   if (some && i < p.k) {
     if (sh.w[i] != sh.w[i]) {
       part = NAN;
-    } else if (sh.at[i] >= 0 && sh.w[i] > 0.0f) {
-      const float lq = logprob_of((float)(static_cast<const T *>(p.in.x) + r * p.in.ld)[sh.at[i]], st, inv_t);
-      part = sh.w[i] * (sh.lw[i] - lq);  // +inf where lq is -inf
+    } else if (sh.at[i] >= 0) {
+      const float x = (float)(static_cast<const T *>(p.in.x) + r * p.in.ld)[sh.at[i]];
+      if (sh.w[i] > 0.0f)
+        part = sh.w[i] * (sh.lw[i] - logprob_of(x, st, inv_t));  // +inf where x is -inf
+      else if (x == -INFINITY)
+        part = INFINITY;  // p is above 0, if below what fp32 holds
     }
   }
   part = block_sum(part, sh.red);

@@ -474,7 +474,7 @@ int gn_token_logprobs_backward(int dtype, const void *logits, long rows, long co
  *   lse[r] = ln sum_j e^(logits[r,j] / temperature).
  * An entry whose id is below 0 or whose teacher logit is -inf is absent; a row of absent entries has loss 0 and gradient 0. An id
  * may occur more than once. An id of cols or above, a NaN or +inf teacher logit, and a NaN or +inf logit
- * make the row's loss NaN (its gradient too). Where a present id's logit is -inf the loss is +inf. lse may be NULL.
+ * make the row's loss NaN (its gradient too). Where a present id's logit is -inf the loss is +inf, however small its p. lse may be NULL.
  * workspace: gn_logits_workspace(rows, cols, 0) bytes, as for gn_token_logprobs. */
 int gn_distill_forward(int dtype, const void *logits, long rows, long cols, long ld, float temperature,
                        const int64_t *ids, const float *teacher, int k, float *loss, float *lse, void *workspace,

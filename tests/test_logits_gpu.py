@@ -548,3 +548,22 @@ def test_smallest_and_largest_temperatures(dev, dtype):
     lp, lse, h, ids, tops = _forward(dev, x.to(dev), torch.tensor([1, 1], device=dev), 2, 3.4e38)
     for r, n in enumerate((4, 5)):
         assert abs(lp[r].item() + math.log(n)) <= 32 * E and abs(h[r].item() - math.log(n)) <= 64 * E
+
+
+def test_infinite_loss_where_the_teacher_probability_underflows(dev):
+    """A present entry whose logit the student rules out: +inf however small p is."""
+    for cols in (40, 30000):
+        for dtype in (torch.float32, torch.float16):
+            x = _logits(4, cols, dtype, 24)
+            ids, t = _teacher(4, cols, 3, 25)
+            t[:, 0] = 0.0
+            t[:3, 1] = torch.tensor([-200.0, -3e38, -100.0])
+            x[0, ids[0, 1]] = x[1, ids[1, 1]] = x[2, ids[2, 1]] = -math.inf
+            t[2, 1] = -math.inf  # absent: not looked at
+            t[3, 1] = -200.0  # ruled out by nobody
+            loss = torch.empty(4, device=dev)
+            G.distill(x.to(dev), ids.to(dev), t.to(dev), loss)
+            loss = loss.cpu()
+            assert loss[0] == math.inf and loss[1] == math.inf
+            r = R.distill(x[2:], ids[2:], t[2:], 1.0)[0]
+            assert bool(((loss[2:].double() - r).abs() <= E * 2000 * (1 + r.abs())).all())
