@@ -43,25 +43,30 @@ __device__ __forceinline__ half8_t half8_of(uint32_t w, float unit) {
   return half8_t{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-// Where a scale would take the weights out of fp16's normal range, the products go through bf16, whose range is
-// fp32's: a code times any 2^(E - 127) is a bf16 number (down to 2^-128, a subnormal one), and an fp16 number is exactly
-// the sum of two. Twice the matrix instructions, the same accumulators, every product still exact.
+// Where a scale would take the weights out of fp16's range, the products go through bf16, whose range is fp32's, and an fp16
+// number is exactly the sum of two. A code times 2^(E - 127) is a bf16 number for E up to 252; the weights are taken as a quarter
+// and the activations (the products' other side, 2^18 at most) four times as large, which serves E up to 254. Twice the
+// matrix instructions, the same accumulators, every product still exact.
+// A quarter's exponent is below the conversion's range for E of 0 and 1. Such a value is a multiple of 2^-133 below 2^-125, whose
+// bits in bf16 are that multiple; the bits of the multiples of 2^-24 in fp16 are the same, and its conversion reaches them.
 __device__ __forceinline__ bf16x8_t bf16x8_of(uint32_t w, unsigned e) {
-  const float unit = __uint_as_float(e << 23);
-  const bf16x2_t a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, unit, 0);
-  const bf16x2_t b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, unit, 1);
-  const bf16x2_t c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, unit, 2);
-  const bf16x2_t d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, unit, 3);
-  const bf16x8_t v = {a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+  const bool least = e < 2;
+  const float unit = __uint_as_float((least ? e + 107 : e - 2) << 23);  // least: code 2^(E + 4) 2^-24
+  u32x4_t v;
+  auto pair = [&](bf16x2_t a, half2_t b) { return least ? __builtin_bit_cast(uint32_t, b) : __builtin_bit_cast(uint32_t, a); };
+  v[0] = pair(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, unit, 0), __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, unit, 0));
+  v[1] = pair(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, unit, 1), __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, unit, 1));
+  v[2] = pair(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, unit, 2), __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, unit, 2));
+  v[3] = pair(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, unit, 3), __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, unit, 3));
   const u32x4_t nan = {0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u};
-  return e == 255 ? __builtin_bit_cast(bf16x8_t, nan) : v;
+  return __builtin_bit_cast(bf16x8_t, e == 255 ? nan : v);
 }
-// c + A B^T of an fp16 A, as its upper 8 bits and the rest (0 for infinities and NaN).
+// c + A B^T of an fp16 A, as the upper 8 bits of 4 A and the rest (0 for infinities and NaN), and of quarters in B.
 __device__ __forceinline__ float4_t mfma_halves_bf16(half8_t a, bf16x8_t b, float4_t c) {
   u32x4_t hi, lo;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float x = (float)a[2 * i], y = (float)a[2 * i + 1];
+    const float x = 4.0f * (float)a[2 * i], y = 4.0f * (float)a[2 * i + 1];
     const uint32_t xh = __float_as_uint(x) & 0xffff0000u, yh = __float_as_uint(y) & 0xffff0000u;
     const float xl = copysignf(fmaxf(fabsf(x - __uint_as_float(xh)), 0.0f), x);  // NaN to 0
     const float yl = copysignf(fmaxf(fabsf(y - __uint_as_float(yh)), 0.0f), y);

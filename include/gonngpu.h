@@ -422,13 +422,14 @@ int gn_mxfp4_size(long rows, long cols, size_t *data_bytes, size_t *scale_bytes,
  * Codes: -1 invalid argument, -6 launch error. */
 int gn_mxfp4_quantize(int dtype, const void *x, long rows, long cols, long ldx, void *data, void *scales,
                       void *stream, CError *err);
-/* The values that a stored matrix stands for, to GN_F32 (exact) or GN_F16 (rounded to nearest even)
+/* The values that a stored matrix stands for, to GN_F32 (exact; infinity for those past its range, which gn_mxfp4_quantize
+ * does not write: scale bytes 253 and 254) or GN_F16 (rounded to nearest even)
  * rows x cols, ldo >= cols elements from row to row; out[r, j] past cols is not written. */
 int gn_mxfp4_dequantize(const void *data, const void *scales, long rows, long cols, int dtype, void *out, long ldo,
                         void *stream, CError *err);
 /* C[M,N] = act( alpha * A * B^T + beta * C + bias[n] ), B an N x K matrix in MXFP4 (a linear layer's weights,
  * outputs x inputs), fp32 accumulation. A is M x K: GN_F16 (lda >= K elements from row to row, a_scales NULL; each weight
- * takes part with its exact value) or GN_MXFP4 (data and scales as above, lda is not read).
+ * takes part with its exact value, also one past fp32's range) or GN_MXFP4 (data and scales as above, lda is not read).
  * C and bias are fp32; bias may be NULL; beta == 0 never reads C; act and act_alpha as gn_gemm; K == 0
  * gives act(beta * C + bias); K and (with several rows) lda are at most 2^22,
  * M and N at most 2^25. Asynchronous; allocates nothing and may be captured.

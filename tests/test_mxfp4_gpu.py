@@ -348,3 +348,38 @@ def test_offsets_past_32_bits(dev):
     G.mxfp4_gemm(aq, bd, y, K=K)
     _bounded(y[pick][:, cols_at].cpu(), R.values(aq[0][pick].cpu(), aq[1][pick].cpu(), K), bv, K)
     assert bool(torch.isfinite(y[-1]).all())
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 40, 32), (3, 40, 20), (12, 40, 32), (27, 60, 32), (50, 64, 31), (70, 200, 32), (90, 140, 29),
+                                   (140, 9000, 32), (400, 11000, 32), (1000, 11000, 32), (3900, 4000, 32)])
+@pytest.mark.parametrize("codes", [(0, 1, 2, 3, 5, 20), (104, 103, 140, 141), (254, 253, 252, 251, 250, 230)])
+@pytest.mark.parametrize("fp4", [False, True])
+def test_product_of_single_scale_rows_at_both_ends(dev, M, N, K, codes, fp4):
+    """Every row of the weights has one scale, among them the smallest and the largest that a stored matrix may have. All values
+    are of one sign in a row, and the activations such that every product is a normal fp32 number: the bound is
+    relative throughout, and weights flushed to 0 or to infinity do not pass it."""
+    g = torch.Generator().manual_seed(M + codes[0])
+    code = torch.randint(0, 8, (N, 128), generator=g) + 8 * (torch.arange(N) % 3 == 0)[:, None]
+    code[:, K:] = 0
+    w = ((code[:, 0::2] + 16 * code[:, 1::2]).to(torch.uint8),
+         torch.tensor(codes, dtype=torch.uint8)[torch.arange(N) % len(codes)][:, None].repeat(1, 4))
+    wv = R.values(*w, K)
+    low, high = codes[0] == 0, codes[0] == 254
+    # the largest outputs are below 32 * 6 * 2^127 * 2^-9, the smallest products above 2^-128 * 2^10
+    span = (2.0**10, 2.0**15) if low else (2.0**-13, 2.0**-9) if high else (2.0**-3, 2.0**3)
+    if fp4:
+        x = _weights(M, K, M + 1)
+        x[0].bitwise_and_(0x77)
+        x[1].fill_(127 + (11 if low else -14 if high else 0))
+        a = R.values(*x, K)
+        xd = tuple(t.to(dev) for t in x)
+    else:
+        x = (span[0] * torch.exp2(torch.rand((M, K), generator=g) * math.log2(span[1] / span[0]))).half()
+        x[:, ::2] = torch.exp2(torch.floor(torch.log2(x[:, ::2].float()))).half()  # every other one a power of two
+        a, xd = x.double(), x.to(dev)
+    y = torch.full((M, N), math.nan, device=dev)
+    G.mxfp4_gemm(xd, tuple(t.to(dev) for t in w), y, K=K)
+    ref = a @ wv.t()
+    bound = STEP * (K + 8) * (a.abs() @ wv.abs().t())
+    assert bool(((y.cpu().double() - ref).abs() <= bound).all()), [
+        (c, bool(((y.cpu().double() - ref).abs() <= bound)[:, i::len(codes)].all())) for i, c in enumerate(codes)]
