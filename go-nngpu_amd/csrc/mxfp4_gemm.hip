@@ -66,7 +66,7 @@ __device__ __forceinline__ float4_t mfma_halves_bf16(half8_t a, bf16x8_t b, floa
   u32x4_t hi, lo;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float x = 4.0f * (float)a[2 * i], y = 4.0f * (float)a[2 * i + 1];
+    const float x = fmaf((float)a[2 * i], 4.0f, 0.0f), y = fmaf((float)a[2 * i + 1], 4.0f, 0.0f);  // one instruction each
     const uint32_t xh = __float_as_uint(x) & 0xffff0000u, yh = __float_as_uint(y) & 0xffff0000u;
     const float xl = copysignf(fmaxf(fabsf(x - __uint_as_float(xh)), 0.0f), x);  // NaN to 0
     const float yl = copysignf(fmaxf(fabsf(y - __uint_as_float(yh)), 0.0f), y);
