@@ -459,10 +459,10 @@ int gn_token_logprobs(int dtype, const void *logits, long rows, long cols, long 
  *   grad_logits[r,j] = ( g_l (1[j = targets[r]] - p_j) - g_h p_j (ln p_j + entropy[r]) ) / temperature
  * with g_l = grad_logprob[r] (0 for a target below 0) and g_h = grad_entropy[r]. grad_logits has the
  * logits' type, ldg >= cols elements from row to row, and may be the logits themselves (ldg == ld). lse and entropy are those that
- * gn_token_logprobs gave for the same logits and temperature; p_j = e^(logits[r,j] / temperature - lse) has a relative error of
- * about |lse| 2^-23 from the rounding of lse. targets and grad_logprob may be NULL together;
- * so may entropy and grad_entropy. A row with an lse of -2^100 or
- * less (all columns masked, by -inf or the type's lowest value) has gradient 0; one with NaN or +inf, or with a target of cols or
+ * gn_token_logprobs gave for the same logits and temperature; p_j = e^(logits[r,j] / temperature - lse), as precise as the
+ * log-probabilities also where lse is large (from 512 on either side of 0 the row is read twice). targets and grad_logprob may be
+ * NULL together; so may entropy and grad_entropy. A row of masked columns only (its largest logit -2^100 or less, its lse -512
+ * or less: -inf or the type's lowest value) has gradient 0; one with NaN or +inf, or with a target of cols or
  * above, NaN. Where both of a row's gradients are 0 its gradient is 0 whatever the logits hold. */
 int gn_token_logprobs_backward(int dtype, const void *logits, long rows, long cols, long ld, float temperature,
                                const int64_t *targets, const float *lse, const float *entropy,
@@ -475,13 +475,14 @@ int gn_token_logprobs_backward(int dtype, const void *logits, long rows, long co
  *   lse[r] = ln sum_j e^(logits[r,j] / temperature).
  * An entry whose id is below 0 or whose teacher logit is -inf is absent; a row of absent entries has loss 0 and gradient 0. An id
  * may occur more than once. An id of cols or above, a NaN or +inf teacher logit, and a NaN or +inf logit
- * make the row's loss NaN (its gradient too). Where a present id's logit is -inf the loss is +inf, however small its p. lse may be NULL.
+ * make the row's loss NaN (its gradient too). Where a present id's logit is -inf the loss is +inf, however small its p.
+ * lse may be NULL.
  * workspace: gn_logits_workspace(rows, cols, 0) bytes, as for gn_token_logprobs. */
 int gn_distill_forward(int dtype, const void *logits, long rows, long cols, long ld, float temperature,
                        const int64_t *ids, const float *teacher, int k, float *loss, float *lse, void *workspace,
                        size_t workspace_bytes, void *stream, CError *err);
 /* grad_logits[r,j] = grad_loss[r] temperature (q_j - sum over i with ids[r,i] = j of p_i), in the logits'
- * type; lse from gn_distill_forward (with -2^100 or less q is 0; q has the error of p in gn_token_logprobs_backward);
+ * type; lse from gn_distill_forward; q as p in gn_token_logprobs_backward, 0 in a row of masked columns only;
  * grad_logits may be the logits themselves (ldg == ld). A row whose grad_loss is 0 has gradient 0 whatever the logits hold. */
 int gn_distill_backward(int dtype, const void *logits, long rows, long cols, long ld, float temperature,
                         const int64_t *ids, const float *teacher, int k, const float *lse, const float *grad_loss,

@@ -567,3 +567,98 @@ def test_infinite_loss_where_the_teacher_probability_underflows(dev):
             assert loss[0] == math.inf and loss[1] == math.inf
             r = R.distill(x[2:], ids[2:], t[2:], 1.0)[0]
             assert bool(((loss[2:].double() - r).abs() <= E * 2000 * (1 + r.abs())).all())
+
+
+def _far_rows(rows, cols, dtype, seed):
+    """Integers (so that differences to the maximum are exact) far from 0, on both sides of it."""
+    x = _logits(rows, cols, torch.float32, seed, spread=20.0).round()
+    x += torch.where(torch.arange(rows) % 2 == 0, 40000.0, -40000.0)[:, None]
+    x[rows // 2, cols // 2:] = x[rows // 2].amax()  # many equal ones
+    if cols > 10:
+        x[:, 3:cols:7] = -math.inf
+    return x.to(dtype)
+
+
+def _far_bound(ref, x, scale, temperature, dtype):
+    """p = 2^((x - m) c - log2 s) from the exact x - m: half-steps of c, of the product and of the subtraction (4 |z|), of ln s
+    (160) and of the forward's entropy (512), and a few of the exponential's and the products'; p below 2^-126 is 0."""
+    z = x / temperature
+    lse = torch.logsumexp(z, 1, keepdim=True)
+    lp = torch.where(torch.isneginf(z), 0.0, z - lse)
+    p = torch.exp(z - lse)
+    out = torch.finfo(dtype).eps / 2 * ref.abs() + (2.0**-25 if dtype == torch.float16 else 1e-44)
+    return scale * (p * E * (800 + 4 * lp.abs()) * (1 + lp.abs()) + 2.0**-126 * 100) + 8 * E * ref.abs() + out
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("exponent", [0, -2, -7, -12, -20, -100, -115, 3])
+@pytest.mark.parametrize("rows,cols", [(2, 1), (4, 50), (3, 3000), (2, 70001), (600, 9000)])
+def test_gradients_of_rows_far_from_zero(dev, rows, cols, exponent, dtype):
+    """Large logits, small temperatures: lse has no room for ln s (at the last temperature it is infinite), and the gradients are
+    those of the differences to the maximum, as the log-probabilities are. Both operators, in place too."""
+    _say("far gradients", rows, cols, exponent, dtype)
+    if rows == 600 and exponent not in (-7, -100):
+        return
+    x, temperature = _far_rows(rows, cols, dtype, cols + rows), 2.0**exponent
+    d = x.double() - x.double().amax(1, keepdim=True)
+    best = d.argmax(1)
+    targets = torch.where(torch.arange(rows) % 3 == 1, (best + cols // 2) % cols, best)
+    targets[-1] = -1
+    g = torch.Generator().manual_seed(27)
+    gl, gh = torch.randn(rows, generator=g) * temperature, torch.randn(rows, generator=g) * temperature
+    xd, td = x.to(dev), targets.to(dev)
+    lp, lse, h, _, _ = _forward(dev, xd, td, 0, temperature)
+    assert bool((lse.abs() >= 4000).all())
+    r = R.logprobs_grad(d, targets, gl, gh, temperature)
+    scale = ((gl.abs() + gh.abs()).double() * (1 + R.logprobs(d, targets, 0, temperature)[2]) / temperature)[:, None] if rows < 600 else \
+        ((gl.abs() + gh.abs()).double() * 11 / temperature)[:, None]  # an entropy of at most ln 9000
+    bound = _far_bound(r, d, scale, temperature, dtype)
+    at = torch.zeros_like(bound).scatter_(1, targets.clamp_min(0)[:, None], 1.0)
+    bound += 16 * E * at * (gl.abs().double() / temperature)[:, None]
+    dx = torch.full((rows, cols), 9.0, dtype=dtype, device=dev)
+    G.token_logprobs_backward(xd, td, lse, gl.to(dev), dx, entropy=h, grad_entropy=gh.to(dev), temperature=temperature)
+    _close(dx, r, bound)
+    mine = xd.clone()
+    G.token_logprobs_backward(mine, td, lse, gl.to(dev), mine, entropy=h, grad_entropy=gh.to(dev), temperature=temperature)
+    assert torch.equal(mine, dx)
+
+    k = min(cols, 5)
+    ids = torch.stack([torch.randperm(cols, generator=g)[:k] for _ in range(rows)])
+    ids[0, k - 1] = -1 if k > 1 else 0
+    t = (torch.randn((rows, k), generator=g) * 2 * temperature).clamp(-1e30, 1e30)
+    loss, gd = torch.empty(rows, device=dev), torch.linspace(-1.5, 2, rows) / temperature
+    G.distill(xd, ids.to(dev), t.to(dev), loss, lse=lse, temperature=temperature)
+    r = R.distill(d, ids, t, temperature)[2] * gd.double()[:, None]
+    scale = (gd.abs().double() * temperature)[:, None]
+    bound = _far_bound(r, d, scale, temperature, dtype)
+    bound += 400 * E * scale * torch.zeros_like(bound).scatter_(1, ids.clamp_min(0), 1.0)
+    G.distill_backward(xd, ids.to(dev), t.to(dev), lse, gd.to(dev), dx, temperature=temperature)
+    _close(dx, r, bound)
+    G.distill_backward(xd, ids.to(dev), t.to(dev), lse, gd.to(dev), xd, temperature=temperature)
+    assert torch.equal(xd, dx)
+
+
+def test_gradients_of_masked_rows_at_any_temperature(dev):
+    """Rows of nothing but -inf or fp32's lowest value have gradient 0 (distillation: q = 0) whatever the temperature; NaN and +inf
+    stay NaN, a row whose gradients are 0 is 0."""
+    low = torch.finfo(torch.float32).min
+    for cols in (60, 20000):
+        x = torch.full((5, cols), low)
+        x[1] = -math.inf
+        x[2] = 40000.0
+        x[2, 1] = math.nan
+        x[3, 1] = math.inf
+        x[4] = math.nan
+        for temperature in (1.0, 1e-6, 1e10, 1e30):
+            t = torch.tensor([3, 1, 2, 1, 0], device=dev)
+            lp, lse, h, _, _ = _forward(dev, x.to(dev), t, 0, temperature)
+            g = torch.tensor([1.0, 1, 1, 1, 0], device=dev)
+            dx = torch.empty((5, cols), device=dev)
+            G.token_logprobs_backward(x.to(dev), t, lse, g, dx, temperature=temperature)
+            assert bool((dx[:2] == 0).all()) and bool(torch.isnan(dx[2:4]).all()) and bool((dx[4] == 0).all())
+            ids, teacher = torch.tensor([[1, 2]] * 5, device=dev), torch.zeros((5, 2), device=dev)
+            G.distill_backward(x.to(dev), ids, teacher, lse, g / temperature, dx, temperature=temperature)
+            want = torch.zeros(cols)
+            want[1:3] = -0.5
+            dx = dx.cpu()
+            assert bool(((dx[:2] - want).abs() <= 4 * E).all()) and bool(torch.isnan(dx[2:4]).all()) and bool((dx[4] == 0).all())
