@@ -828,6 +828,11 @@ void *gn_stream(void) {
   return ctx ? (void *)ctx->stream : nullptr;
 }
 
+int gn_device(void) {
+  gn::Context *ctx = gn::context(nullptr);
+  return ctx ? ctx->device : -1;
+}
+
 void *gn_buffer_device_ptr(GPUPtr buf) {
   Buffer *b = gn::as_buffer(buf);
   return b ? b->dptr : nullptr;

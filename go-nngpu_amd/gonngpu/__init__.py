@@ -71,6 +71,7 @@ SIGNATURES = {
     "gn_version": (ctypes.c_char_p, []),
     "gn_init": (_I, [_ERR]),
     "gn_stream": (_VP, []),
+    "gn_device": (_I, []),
     "gn_buffer_device_ptr": (_VP, [_VP]),
     "gn_buffer_bytes": (_L, [_VP]),
     "gn_memory_stats": (None, [ctypes.POINTER(_L), ctypes.POINTER(_L), ctypes.POINTER(_L)]),
@@ -215,6 +216,11 @@ def init():
 
 def stream():
     return load().gn_stream()
+
+
+def library_device():
+    """Number of the GPU that the library's stream is on."""
+    return load().gn_device()
 
 
 def memory_stats():
@@ -430,10 +436,15 @@ def _width(t):
 
 
 def _dispatch_on(device, stream_ptr, name, *args):
-    """_dispatch for arguments whose device is known to be the current one."""
-    if stream_ptr is None:
+    """_dispatch for arguments whose device is known to be the current one. The library's own stream is on one device only:
+    it does not stand in for the default stream of another."""
+    ordered = stream_ptr is None
+    if ordered:
         stream_ptr = _current_stream(device)
-        if not stream_ptr:
+    if not stream_ptr:
+        if device != library_device():
+            _refuse(f"the library's stream is on GPU {library_device()}, the tensors are on GPU {device}: a stream of theirs is needed")
+        if ordered:
             return _run_ordered(name, *args)
     return call(name, *args, stream_ptr)
 

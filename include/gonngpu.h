@@ -280,8 +280,10 @@ int gn_csr_indices_changed(GPUPtr valuesPtr);
 const char *gn_version(void);
 /* Initialises the device context once (thread-safe). 0 on success. */
 int gn_init(CError *err);
-/* The library's stream (a hipStream_t, returned as void*). */
+/* The library's stream (a hipStream_t, returned as void*), and the device that it is on: the one that was current when the
+ * context was initialised (-1 without one). */
 void *gn_stream(void);
+int gn_device(void);
 /* Device pointer of a GPUPtr handle (NULL for an invalid handle), and its size. */
 void *gn_buffer_device_ptr(GPUPtr buf);
 long gn_buffer_bytes(GPUPtr buf);

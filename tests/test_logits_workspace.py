@@ -79,3 +79,25 @@ def test_library_stream_with_the_default_stream_current(dev, monkeypatch, distil
     torch.cuda.synchronize()
     for a, b in zip((lp, lse, ids, tops), want):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("current,asked,where", [
+    (DEFAULT, None, 0), (DEFAULT, 0, 0), (MINE, 0, 0), (MINE, None, 1), (DEFAULT, MINE, 1)])
+def test_library_stream_on_another_gpu(monkeypatch, current, asked, where):
+    """A call that would run on the library's stream is refused for tensors of another GPU than that stream's; a stream of theirs is
+    used as it is."""
+    ran = []
+    monkeypatch.setattr(G, "_current_stream", lambda device=None: current)
+    monkeypatch.setattr(G, "library_device", lambda: 0, raising=False)
+    monkeypatch.setattr(G, "call", lambda name, *args: ran.append(args[-1]))
+    monkeypatch.setattr(G, "_run_ordered", lambda name, *args: ran.append("ordered"))
+    G._dispatch_on(0, asked, "gn_mxfp4_quantize", 5)
+    assert ran == ["ordered" if current == DEFAULT and asked is None else asked if asked is not None else current]
+    ran.clear()
+    if where == 1:
+        G._dispatch_on(1, asked, "gn_mxfp4_quantize", 5)
+        assert ran == [asked or current]
+    else:
+        with pytest.raises(G.GonngpuError, match="library's stream is on GPU 0"):
+            G._dispatch_on(1, asked, "gn_mxfp4_quantize", 5)
+        assert ran == []
