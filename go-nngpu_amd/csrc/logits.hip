@@ -10,8 +10,9 @@
 // first exponential, and the top alternatives are looked for in registers. Rows of several segments leave (m, s, t) and the
 // segment's best k in the workspace, and a second kernel, one workgroup to a row, joins them in segment order.
 // Measured (a large copy 4.6, reads alone 5.4 TB/s): 4096 rows of 32768 in fp32 103 us forward (5.2 TB/s), 180 with 20
-// alternatives, 191 backward (5.6); distillation of 2048 rows of 65536 in fp16 54 us forward, 96 backward (5.6). One row of 131072
-// takes 5.8 us, with 20 alternatives 12.8: there the latencies of two launches and their reductions.
+// alternatives (141 registers against 92 leave 3 waves to a SIMD instead of 5, for the loads as for the search), 191 backward (5.6);
+// distillation of 2048 rows of 65536 in fp16 54 us forward, 96 backward (5.6). One row of 131072 takes 5.8 us, the
+// latencies of two launches and their reductions, and with 20 alternatives 12.8: those of the two searches too.
 #include <algorithm>
 #include <climits>
 #include <type_traits>
@@ -663,7 +664,11 @@ int launched(const char *what, CError *err) {
 }
 
 // Values of a row to a thread: 32, 8192 logits to a workgroup, or 8 where that leaves CUs without one (one row of
-// 131072, 20 alternatives: 16 workgroups of 8192 take 8.4 us and their join 7.4, 64 of 2048 6.2 and 7.1).
+// 131072, 20 alternatives: 16 workgroups of 8192 take 8.4 us and their join 7.4, 64 of 2048 6.2 and 7.1). Calls with 8 against 32, us
+// (forward, with 20 alternatives, gradient; logits in the Infinity Cache): 1 x 131072 fp32 5.5 / 6.0, 12.6 / 15.7, 2.3 / 3.4; 16 x 131072
+// 6.5 / 6.5, 14.4 / 16.2, 4.0 / 4.6; 32 x 131072, at the border, 7.5 / 7.1, 18.0 / 16.9, 5.4 / 6.8; 64 x 50257 fp16 7.3 / 7.5,
+// 16.6 / 16.2, 4.6 / 5.6; 512 x 4096 fp32 6.9 / 4.6, 12.6 / 9.1, 4.0 / 5.5. Below the border rows of one segment of 8192 lose their join
+// with 32 (256 x 8192 6.6 / 3.8, 12.8 / 8.9, 4.0 / 4.6): forward and gradient share the rule all the same.
 struct Split {
   int per, segs;
 };

@@ -85,10 +85,10 @@ __device__ __forceinline__ float finish(const MxParams &p, float acc, long m, lo
 }
 
 // ------------------------------------------------------------------ few rows
-// Up to 64 rows: bound by the stream of B (1 row 4096 -> 11008: 24 MB in 9.2 us with the launch). A workgroup owns some
-// columns for all rows; its waves cut K among them, whole groups each, and the partial sums meet in LDS. Lane (r, g) =
-// (lane % 16, lane / 16) takes block g of row r's group, 16 consecutive bytes, so a wave reads whole 64-byte pieces of 16
-// rows of B, straight into registers.
+// Up to 64 rows: B is read once (1 row 4096 -> 11008: 24 MB, 4.4 us at the rate of reads, in 9.0 us with the launch), and the time
+// is that of the loads' latencies, which only in part pass side by side (below). A workgroup owns some columns for all rows;
+// its waves cut K among them, whole groups each, and the partial sums meet in LDS. Lane (r, g) = (lane % 16, lane / 16) takes
+// block g of row r's group, 16 consecutive bytes, so a wave reads whole 64-byte pieces of 16 rows of B, straight into registers.
 
 // Adds the waves' partial sums and writes C: `part` holds [wk][blocks][64] of them, each block 16 x 16, block j MF + i the
 // rows m0 + 16 i .. and the columns n0 + 16 j ... Lane (r, g) of a block has rows 4 g .. 4 g + 3 of column r.
@@ -107,7 +107,9 @@ __device__ __forceinline__ void join_rows(const MxParams &p, const float4_t *par
   }
 }
 
-// Both sides in 4 bits: U groups of NF columns' and MF rows' fragments in flight.
+// Both sides in 4 bits, U groups of NF columns' and MF rows' fragments to a turn. In <1, 1, 4> a turn's loads leave together; of
+// the other forms' the compiler moves some to their use, in <2, 4, 2> a column's codes and scales after the first one's, each with
+// a wait of its own (16, 32 and 64 rows of 4096 -> 11008 12.2, 16.2 and 19.1 us, the bytes 5 to 6).
 template <int MF, int NF, int U>
 __global__ void __launch_bounds__(512) mx_fp4_rows_kernel(MxParams p) {
   extern __shared__ float4_t part[];  // [waves][MF * NF][64]
@@ -159,7 +161,9 @@ __global__ void __launch_bounds__(512) mx_fp4_rows_kernel(MxParams p) {
 
 // fp16 activations. K goes in slabs of KS = 128 U WK values, a slab of all rows staged in LDS (through registers: A needs no
 // alignment and its tail is masked on the way); WK x WN waves, wave (wk, wn) takes the slab's groups wk U .. wk U + U - 1 and
-// NF blocks of columns. The next slab's A and B are on their way while one is multiplied. The lane's 32 weights become
+// NF blocks of columns. The next slab's A and B are asked for before one is multiplied; on their way meanwhile they are for every
+// other slab only: behind the branches for A's tail the compiler has no count of the loads, and for the rest it waits for all of
+// them before the products (with 17 rows and more for A's chunks one after the other, too). The lane's 32 weights become
 // four fragments of v_mfma_f32_16x16x32_f16 whose k are 8 j .. 8 j + 7 of each lane's own block, and A's lanes read the same.
 // Where the scales of a wave's blocks all keep the weights normal fp16 numbers (half_exact; weights of ordinary size do) the
 // conversion applies them, exactly; otherwise both sides go through bf16.
@@ -477,8 +481,11 @@ mx_fp4_kernel(MxParams p) {
 // C = A B^T on v_mfma_f32_16x16x32_f16, the weights converted in registers. WM x WN waves, each FM x FN blocks of 16 x 16;
 // K in stages of 64, NS of them in LDS: 128 bytes of A to a row (ring_plan.h's plan and swizzle) and 32 of codes. Lane (r,
 // g) takes k = 16 g .. 16 g + 15 of the stage on both sides, 8 in each of two steps, so its 16 codes are 8 consecutive bytes (a
-// wave's read of 16 rows is 512 consecutive ones) and lie in one block. A row's scales for 8 stages are 16 bytes in LDS. The
-// scales are applied as in the few-rows kernel: in fp16 where all of the wave's allow it, else in bf16.
+// wave's read of 16 rows is 512 consecutive ones) and lie in one block. A row's scales for 8 stages are 16 bytes in LDS. A tile's
+// weights are applied in fp16 where all of its columns' scales allow it over the whole of K, else in bf16, at 3.4 times the time
+// and, but for the 256 x 256 tile, after a pass in fp16 that is thrown away: with one block in 32 rows of B out of
+// range, as a pruned layer may have them (a largest weight below 2^-21), 128 rows 4096 -> 11008 105 us instead of 24, 512 rows 203
+// instead of 52, 8192^3 2.81 ms instead of 0.83. (In the few-rows kernel a wave decides for each of its slabs: 64 rows 29 instead of 26 us.)
 // 8192^3 takes 820 us (1.34 PFLOP/s, the rate of a large bf16 library product on this card: its power); smaller products wait for LDS and
 // the barriers between stages (128 x 128 tiles without their matrix instructions took 85% of their time, without their copies 75%).
 // DMA: A is copied to LDS by dma16 (16-byte aligned rows, K a multiple of 8); otherwise through registers, its tail masked.
@@ -824,7 +831,9 @@ void launch_fp4_tiles(const MxParams &p, hipStream_t s) {
   }
 }
 
-// The same for fp16 activations; rows of A that are not 16-byte aligned go through registers in 128 x 64 tiles. Two tiles of the
+// The same for fp16 activations; rows of A that are not 16-byte aligned go through registers in 128 x 64 tiles, with a wait for all
+// copies in each stage (K of 4097 against 4096, 512 rows -> 11008: 125 against 55 us, 2048 rows -> 4096 130 / 68; 8192 x 8193 -> 8192
+// 1.86 / 0.83 ms): a copy with aligned rows would need memory that this call, which allocates nothing, does not have. Two tiles of the
 // three smaller kinds share a CU and its time. Measured, us, 256 x 256 / 128 x 192 / 128 x 128 / 64 x 128 / 64 x 64: 8192^3 825 / 1001 /
 // 925 / 1073 / 1401; 4096 -> 11008, 1024 rows 111 / 115 / 105 / 114 / 143, 512 rows 98 / 52.6 / 62.8 / 55.6 / 70.8, 256 rows 97 / 46.2 /
 // 38.4 / 36.7 / 37.0, 128 rows 96 / 46.0 / 37.6 / 24.6 / 25.7; 4096 -> 4096, 2048 rows 102 / 95 / 67.3 / 74.0 / 90.6, 128 rows 95 /
@@ -863,7 +872,9 @@ void launch_half_rows(const MxParams &p, hipStream_t s) {
 // against narrow form: 4-bit A, 4096 -> 11008, 16 rows 12.7 / 14.4, 32 rows 14.7 / 17.8, 64 rows 19.7 / 24.8; 8 rows
 // 4096 -> 4096 11.8 / 6.1, 40 rows 1000 -> 1000 7.5 / 4.8. fp16 A, 1 row 4096 -> 11008 9.2 / 10.6, 11008 -> 4096
 // 11.0 / 9.6; 16 rows 4096 -> 11008 13.3 / 21.3, 8192 -> 1024 15.5 / 10.7; 64 rows 4096 -> 11008 26.6 / 39.4,
-// 4096 -> 4096 25.5 / 19.8.
+// 4096 -> 4096 25.5 / 19.8. Next to the border (weights in the Infinity Cache): 4096 -> 6144, 64 rows 4-bit A 18.7 / 17.0, fp16 A
+// 24.0 / 18.4; 4096 -> 8192 19.0 / 17.3 and 25.6 / 20.7, 8 rows 11.6 / 8.6 and 10.4 / 8.7, but 1024 -> 8192 in fp16, 8 rows 4.2 / 6.0;
+// 4096 -> 16384, 64 rows 19.4 / 31.5 and 26.9 / 39.1. For 8192 columns themselves the narrow forms are the faster ones with much K.
 void launch_rows(bool fp4, const MxParams &p, hipStream_t s) {
   const bool wide = p.N >= 8192;
   if (fp4) {
@@ -936,6 +947,10 @@ int launch_mxfp4_gemm(const MxGemmDesc &d, hipStream_t s, CError *err) {
   if (d.K == 0) {
     hipLaunchKernelGGL(mx_k0_kernel, dim3(grid_of(d.M * d.N, 256)), dim3(256), 0, s, p);
   } else {
+    // The few-rows kernels against tiles, us, weights in the Infinity Cache. fp16 A: 4096 -> 4096, 16 rows 7.7 / 18.1, 64 rows
+    // 18.2 / 18.6; 11008 -> 4096, 64 rows 43.8 / 42.7; 4096 -> 11008, 32 rows 16.7 / 18.4, 64 rows 25.9 / 19.2. 4-bit A: 4096 -> 4096, 16
+    // rows 6.4 / 8.1, 64 rows 10.1 / 8.6; 11008 -> 4096, 64 rows 15.9 / 17.3; 4096 -> 11008, 1 row 8.7 / 8.1, 64 rows 19.1 / 8.8. The border
+    // fits where a tile to a CU does not go round; with many columns tiles would win below it, in 4 bits at any number of rows.
     if (d.M <= 64)
       launch_rows(d.a_dtype == GN_MXFP4, p, s);
     else if (d.a_dtype == GN_MXFP4)
