@@ -461,11 +461,11 @@ int gn_token_logprobs(int dtype, const void *logits, long rows, long cols, long 
  *   grad_logits[r,j] = ( g_l (1[j = targets[r]] - p_j) - g_h p_j (ln p_j + entropy[r]) ) / temperature
  * with g_l = grad_logprob[r] (0 for a target below 0) and g_h = grad_entropy[r]. grad_logits has the
  * logits' type, ldg >= cols elements from row to row, and may be the logits themselves (ldg == ld). lse and entropy are those that
- * gn_token_logprobs gave for the same logits and temperature; p_j = e^(logits[r,j] / temperature - lse), as precise as the
- * log-probabilities also where lse is large (from 512 on either side of 0 the row is read twice). targets and grad_logprob may be
- * NULL together; so may entropy and grad_entropy. A row of masked columns only (its largest logit -2^100 or less, its lse -512
- * or less: -inf or the type's lowest value) has gradient 0; one with NaN or +inf, or with a target of cols or
- * above, NaN. Where both of a row's gradients are 0 its gradient is 0 whatever the logits hold. */
+ * gn_token_logprobs gave for the same logits and temperature; p_j = e^(logits[r,j] / temperature - lse), off by what
+ * rounding lse lost, at most 2^-16 of it: from an |lse| of 512 on the row is read twice, and p as precise as from its
+ * log-probability. targets and grad_logprob may be NULL together; so may entropy and grad_entropy. A row of masked columns only
+ * (its largest logit -2^100 or less, its lse -512 or less: -inf or the type's lowest value) has gradient 0; one with NaN or +inf,
+ * or with a target of cols or above, NaN. Where both of a row's gradients are 0 its gradient is 0 whatever the logits hold. */
 int gn_token_logprobs_backward(int dtype, const void *logits, long rows, long cols, long ld, float temperature,
                                const int64_t *targets, const float *lse, const float *entropy,
                                const float *grad_logprob, const float *grad_entropy, void *grad_logits, long ldg,

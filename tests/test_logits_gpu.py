@@ -662,3 +662,69 @@ def test_gradients_of_masked_rows_at_any_temperature(dev):
             want[1:3] = -0.5
             dx = dx.cpu()
             assert bool(((dx[:2] - want).abs() <= 4 * E).all()) and bool(torch.isnan(dx[2:4]).all()) and bool((dx[4] == 0).all())
+
+
+@pytest.mark.parametrize("cols", [300, 21000])
+def test_far_rows_strided_repeated_and_captured(dev, cols):
+    """Far rows and near ones side by side in a strided view at odd addresses, into one of another stride; repeated and absent
+    entries; rows without a gradient; the same from a graph, replayed with other rows far."""
+    rows, T = 20, 0.5
+    g = torch.Generator().manual_seed(30)
+    for dtype in (torch.float32, torch.float16):
+        base, out = torch.zeros((2 * rows, cols + 7), dtype=dtype, device=dev), torch.full((rows, cols + 3), 7.0, dtype=dtype, device=dev)
+        xd, dx = base[::2, 3:3 + cols], out[:, 1:1 + cols]
+        ids = torch.randint(0, cols, (rows, 6), generator=g)
+        ids[:, 4] = ids[:, 2]
+        ids[1] = -1
+        ids[2, 0] = -7
+        t, gd = torch.randn((rows, 6), generator=g), torch.randn(rows, generator=g)
+        gd[[3, 4]] = 0.0
+        targets = torch.randint(0, cols, (rows,), generator=g)
+        targets[5] = -1
+        new = lambda: torch.empty(rows, device=dev)  # noqa: E731
+        lse, lp, loss, l1, l2 = new(), new(), new(), torch.empty_like(dx), torch.empty_like(dx)
+        td, idd, tld, gdd = targets.to(dev), ids.to(dev), t.to(dev), gd.to(dev)
+
+        def step():
+            G.token_logprobs(xd, td, lp, lse=lse, temperature=T)
+            G.token_logprobs_backward(xd, td, lse, gdd, dx, temperature=T)
+            l1.copy_(dx)
+            G.distill(xd, idd, tld, loss, lse=lse, temperature=T)
+            G.distill_backward(xd, idd, tld, lse, gdd, dx, temperature=T)
+            l2.copy_(dx)
+
+        def check(x):
+            d = x.double() - x.double().amax(1, keepdim=True)
+            none = torch.zeros(rows)
+            scale = (gd.abs().double() / T)[:, None]
+            hot = torch.zeros((rows, cols), dtype=torch.float64).scatter_(1, targets.clamp_min(0)[:, None], 1.0)
+            r = R.logprobs_grad(d, targets, gd, none, T)
+            # near rows: lse is off by half a step of 512
+            near = 2.0**-16 * torch.softmax(d / T, 1)
+            _close(l1, r, _far_bound(r, d, scale, T, dtype) + scale * (near + 16 * E * hot))
+            r = R.distill(d, ids, t, T)[2] * gd.double()[:, None]
+            hot = torch.zeros((rows, cols), dtype=torch.float64).scatter_(1, ids.clamp_min(0), 1.0)
+            scale = (gd.abs().double() * T)[:, None]
+            _close(l2, r, _far_bound(r, d, scale, T, dtype) + scale * (near + 1200 * E * hot))
+            assert bool((out[:, 0] == 7).all()) and bool((out[:, 1 + cols:] == 7).all())
+
+        def fill(first):
+            x = _logits(rows, cols, dtype, 31 + first).round()
+            x[first::3] = (x[first::3].float() + 2048).to(dtype)
+            xd.copy_(x)
+            return x
+
+        x = fill(0)
+        step()
+        check(x)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            step()
+        for first in (1, 2, 0):
+            x = fill(first)
+            l1.zero_()
+            l2.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            check(x)
+            step()
