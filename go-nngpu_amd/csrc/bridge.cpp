@@ -11,6 +11,8 @@
 #include <vector>
 
 #include "common.h"
+#include "adjust.h"
+#include "int8.h"
 #include "logits.h"
 #include "mxfp4.h"
 
@@ -971,6 +973,64 @@ int gn_mxfp4_gemm(int a_dtype, long M, long N, long K, float alpha, const void *
   if (int rc = gn::check_mxfp4_gemm(d, err)) return rc;
   if (!gn::context(err)) return -1;
   return gn::launch_mxfp4_gemm(d, gn::resolve_stream(stream), err);
+}
+
+int gn_int8_quantize(int dtype, const void *x, long rows, long cols, long ldx, const float *col_scale, int8_t *q, long ldq,
+                     float *scales, void *stream, CError *err) {
+  const gn::Int8QuantizeDesc d{dtype, x, rows, cols, ldx, col_scale, q, ldq, scales};
+  if (int rc = gn::check_int8_quantize(d, err)) return rc;
+  if (!gn::context(err)) return -1;
+  return gn::launch_int8_quantize(d, gn::resolve_stream(stream), err);
+}
+
+int gn_int8_dequantize(const int8_t *q, const float *scales, long rows, long cols, long ldq, int dtype, void *out, long ldo,
+                       void *stream, CError *err) {
+  if (int rc = gn::check_int8_dequantize(q, scales, rows, cols, ldq, dtype, out, ldo, err)) return rc;
+  if (!gn::context(err)) return -1;
+  return gn::launch_int8_dequantize(q, scales, rows, cols, ldq, dtype, out, ldo, gn::resolve_stream(stream), err);
+}
+
+int gn_int8_gemm(long M, long N, long K, float alpha, const int8_t *A, long lda, const float *a_scales, const int8_t *B,
+                 long ldb, const float *b_scales, float beta, float *C, long ldc, const float *bias, int act, float act_alpha,
+                 void *stream, CError *err) {
+  const gn::Int8GemmDesc d{M, N, K, alpha, beta, A, lda, a_scales, B, ldb, b_scales, C, ldc, bias, act, act_alpha};
+  if (int rc = gn::check_int8_gemm(d, err)) return rc;
+  if (!gn::context(err)) return -1;
+  return gn::launch_int8_gemm(d, gn::resolve_stream(stream), err);
+}
+
+size_t gn_int8_linear_workspace(long M, long N, long K) { return gn::int8_linear_workspace(M, N, K); }
+
+int gn_int8_linear(int dtype, long M, long N, long K, float alpha, const void *x, long ldx, const float *col_scale,
+                   const int8_t *B, long ldb, const float *b_scales, float beta, float *C, long ldc, const float *bias, int act,
+                   float act_alpha, void *workspace, size_t workspace_bytes, void *stream, CError *err) {
+  const gn::Int8LinearDesc d{dtype, x, ldx, col_scale,
+                             {M, N, K, alpha, beta, nullptr, 0, nullptr, B, ldb, b_scales, C, ldc, bias, act, act_alpha},
+                             workspace, workspace_bytes};
+  if (int rc = gn::check_int8_linear(d, err)) return rc;
+  if (!gn::context(err)) return -1;
+  return gn::launch_int8_linear(d, gn::resolve_stream(stream), err);
+}
+
+int gn_adjust_logits(int dtype, const void *logits, long rows, long cols, long ld, const int64_t *history, long history_len,
+                     const int64_t *prompt, const float *repetition, const float *frequency, const float *presence,
+                     const int64_t *bias_ids, const float *bias, int biases, const uint32_t *mask, long ldmask, void *out,
+                     long ldo, void *stream, CError *err) {
+  const gn::AdjustDesc d{dtype, logits, rows, cols, ld, history, history_len, prompt, repetition, frequency, presence,
+                         bias_ids, bias, biases, mask, ldmask, out, ldo};
+  if (int rc = gn::check_adjust(d, err)) return rc;
+  if (!gn::context(err)) return -1;
+  return gn::launch_adjust(d, gn::resolve_stream(stream), err);
+}
+
+int gn_adjust_logits_backward(int dtype, const void *logits, long rows, long cols, long ld, const void *grad_out, long ldg,
+                              const int64_t *history, long history_len, const float *repetition, const uint32_t *mask,
+                              long ldmask, void *grad_logits, long ldo, void *stream, CError *err) {
+  const gn::AdjustGradDesc d{dtype, logits, rows, cols, ld, grad_out, ldg, history, history_len, repetition, mask, ldmask,
+                             grad_logits, ldo};
+  if (int rc = gn::check_adjust_backward(d, err)) return rc;
+  if (!gn::context(err)) return -1;
+  return gn::launch_adjust_backward(d, gn::resolve_stream(stream), err);
 }
 
 size_t gn_logits_workspace(long rows, long cols, int k) { return gn::logits_workspace(rows, cols, k); }

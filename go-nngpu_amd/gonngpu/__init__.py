@@ -118,6 +118,13 @@ SIGNATURES = {
     "gn_token_logprobs_backward": (_I, [_I, _VP, _L, _L, _L, _F, _VP, _VP, _VP, _VP, _VP, _VP, _L, _VP, _ERR]),
     "gn_distill_forward": (_I, [_I, _VP, _L, _L, _L, _F, _VP, _VP, _I, _VP, _VP, _VP, _SZ, _VP, _ERR]),
     "gn_distill_backward": (_I, [_I, _VP, _L, _L, _L, _F, _VP, _VP, _I, _VP, _VP, _VP, _L, _VP, _ERR]),
+    "gn_adjust_logits": (_I, [_I, _VP, _L, _L, _L, _VP, _L, _VP, _VP, _VP, _VP, _VP, _VP, _I, _VP, _L, _VP, _L, _VP, _ERR]),
+    "gn_adjust_logits_backward": (_I, [_I, _VP, _L, _L, _L, _VP, _L, _VP, _L, _VP, _VP, _L, _VP, _L, _VP, _ERR]),
+    "gn_int8_quantize": (_I, [_I, _VP, _L, _L, _L, _VP, _VP, _L, _VP, _VP, _ERR]),
+    "gn_int8_dequantize": (_I, [_VP, _VP, _L, _L, _L, _I, _VP, _L, _VP, _ERR]),
+    "gn_int8_gemm": (_I, [_L, _L, _L, _F, _VP, _L, _VP, _VP, _L, _VP, _F, _VP, _L, _VP, _I, _F, _VP, _ERR]),
+    "gn_int8_linear_workspace": (_SZ, [_L, _L, _L]),
+    "gn_int8_linear": (_I, [_I, _L, _L, _L, _F, _VP, _L, _VP, _VP, _L, _VP, _F, _VP, _L, _VP, _I, _F, _VP, _SZ, _VP, _ERR]),
     "gn_spmm_csr": (_I, [_L, _L, _L, _L, _VP, _VP, _VP, _VP, _L, _VP, _L, _VP, _VP, _ERR]),
     "gn_spmv_csr": (_I, [_L, _L, _L, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _ERR]),
     "gn_spmv_plan_create": (_I, [_L, _L, _L, _VP, _VP, ctypes.POINTER(_VP), _VP, _ERR]),
@@ -507,23 +514,26 @@ def _logits_workspace_bytes(rows, cols, k):
     return load().gn_logits_workspace(rows, cols, k)
 
 
-def _logits_workspace(logits, rows, cols, k, device, stream_ptr):
-    """Scratch for one call, from torch's allocator (which keeps what a captured graph uses), of the pool of the stream
+def _scratch(like, n, device, stream_ptr):
+    """n bytes of scratch for one call, from torch's allocator (which keeps what a captured graph uses), of the pool of the stream
     that the call runs on: a block of another stream's pool may still be in use there. A handle of 0 asked for is the library's
     stream, whereas torch's default stream, whose handle is 0 too, is None asked for (the call is then waited for). Asked
-    for in the logits' type (the bytes are a multiple of 8): naming a type and a device takes 1.3 us more."""
+    for in the type of `like`, float32 or float16 (n is a multiple of 4): naming a type and a device takes 1.3 us more."""
     T = _types()
-    n = _logits_workspace_bytes(rows, cols, k)
-    if n == 0:
-        return None, 0
-    size = n // (4 if logits.dtype is T.float32 else 2)
+    size = n // (4 if like.dtype is T.float32 else 2)
     if stream_ptr is None:
-        return logits.new_empty((size,)), n
+        return like.new_empty((size,))
     stream_ptr = stream_ptr or stream()
     if stream_ptr == _current_stream(device):
-        return logits.new_empty((size,)), n
+        return like.new_empty((size,))
     with T.cuda.stream(T.cuda.ExternalStream(stream_ptr, device=device)):
-        return logits.new_empty((size,)), n
+        return like.new_empty((size,))
+
+
+def _logits_workspace(logits, rows, cols, k, device, stream_ptr):
+    """The workspace of a call on logits (see _scratch) and its bytes."""
+    n = _logits_workspace_bytes(rows, cols, k)
+    return (_scratch(logits, n, device, stream_ptr) if n else None), n
 
 
 def token_logprobs(logits, targets, logprob, *, lse=None, entropy=None, top_ids=None, top_logprobs=None,
@@ -607,6 +617,178 @@ def distill_backward(logits, ids, teacher, lse, grad_loss, grad_logits, *, tempe
     device = _device_of(logits, ids, teacher, lse, grad_loss, grad_logits)
     _dispatch_on(device, stream_ptr, "gn_distill_backward", dt, logits.data_ptr(), rows, cols, ld, temperature, ids.data_ptr(),
                  teacher.data_ptr(), k, _ptr(lse), grad_loss.data_ptr(), grad_logits.data_ptr(), ldg)
+
+
+def int8_empty(rows, cols, device="cuda"):
+    """The two arrays (int8 values, float32 scales) of a rows x cols int8 matrix, not filled in. Rows start at
+    multiples of 16 bytes, as the products need them."""
+    T = _types()
+    q = T.empty((rows, -(-cols // 16) * 16), dtype=T.int8, device=device)
+    return q[:, :cols], T.empty((rows,), dtype=T.float32, device=device)
+
+
+def _int8_matrix(what, q):
+    """(rows, cols, bytes from row to row) of an int8 matrix whose rows are dense."""
+    if q.dtype is not _types().int8:
+        _refuse(f"{what}: int8 is needed, got {q.dtype}")
+    strides = q.stride()
+    if len(strides) == 2:
+        rows, cols = q.size(0), q.size(1)
+        if (strides[1] == 1 or cols <= 1) and (strides[0] >= cols or rows <= 1):
+            return rows, cols, (strides[0] if rows > 1 else cols)
+    _refuse(f"{what}: a matrix of dense rows is needed, got shape {tuple(q.shape)}, strides {strides}")
+
+
+def int8_quantize(x, q, scales, *, col_scale=None, stream_ptr=None):
+    """A float32 or float16 matrix, times a factor for each column if one is given, brought to 8-bit integers with a scale for
+    each row, into the arrays of int8_empty(*x.shape)."""
+    T = _types()
+    dt, rows, cols, ld = _matrix("int8_quantize", x)
+    qrows, qcols, ldq = _int8_matrix("int8_quantize: q", q)
+    if (qrows, qcols) != (rows, cols):
+        _refuse(f"int8_quantize: {rows} x {cols} values, {qrows} x {qcols} integers")
+    _expect("int8_quantize: scales", scales, T.float32, rows)
+    if col_scale is not None:
+        _expect("int8_quantize: col_scale", col_scale, T.float32, cols)
+    device = _device_of(x, q, scales, col_scale)
+    _dispatch_on(device, stream_ptr, "gn_int8_quantize", dt, x.data_ptr(), rows, cols, ld, _ptr(col_scale), q.data_ptr(), ldq,
+                 scales.data_ptr())
+
+
+def int8_dequantize(q, scales, out, stream_ptr=None):
+    """The values of an int8 matrix, to a float32 or float16 matrix of its size."""
+    dt, rows, cols, ld = _matrix("int8_dequantize", out)
+    qrows, qcols, ldq = _int8_matrix("int8_dequantize: q", q)
+    if (qrows, qcols) != (rows, cols):
+        _refuse(f"int8_dequantize: {qrows} x {qcols} integers, {rows} x {cols} values")
+    _expect("int8_dequantize: scales", scales, _types().float32, rows)
+    device = _device_of(q, scales, out)
+    _dispatch_on(device, stream_ptr, "gn_int8_dequantize", q.data_ptr(), scales.data_ptr(), rows, cols, ldq, dt, out.data_ptr(), ld)
+
+
+def _int8_product(what, rows, K, B, C, bias):
+    """Checks the sides that int8_gemm and int8_linear share: (weights, their scales, M, N, bytes from row to row, ldc)."""
+    T = _types()
+    dtc, M, N, ldc = _matrix(what + ": C", C)
+    if dtc != GN_F32:
+        _refuse(what + ": C is float32")
+    w, w_scales = B
+    wrows, wcols, ldb = _int8_matrix(what + ": B", w)
+    if rows != M or wrows != N or wcols != K:
+        _refuse(f"{what}: {rows} x {K} times the transposed {wrows} x {wcols} is not {M} x {N}")
+    if w_scales is not None:
+        _expect(what + ": scales of B", w_scales, T.float32, N)
+    if bias is not None:
+        _expect(what + ": bias", bias, T.float32, N)
+    return w, w_scales, M, N, ldb, ldc
+
+
+def int8_gemm(A, B, C, *, alpha=1.0, beta=0.0, bias=None, act=ACT_NONE, act_alpha=0.0, stream_ptr=None):
+    """C = act(alpha*A*B^T + beta*C + bias) with A = (int8 values, scales) of a rows x inputs matrix and B the same of an
+    outputs x inputs one, as in int8_empty. Scales may be None (1 for each row)."""
+    a, a_scales = A
+    rows, K, lda = _int8_matrix("int8_gemm: A", a)
+    w, w_scales, M, N, ldb, ldc = _int8_product("int8_gemm", rows, K, B, C, bias)
+    if a_scales is not None:
+        _expect("int8_gemm: scales of A", a_scales, _types().float32, M)
+    device = _device_of(a, a_scales, w, w_scales, C, bias)
+    _dispatch_on(device, stream_ptr, "gn_int8_gemm", M, N, K, alpha, a.data_ptr(), lda, _ptr(a_scales), w.data_ptr(), ldb,
+                 _ptr(w_scales), beta, C.data_ptr(), ldc, _ptr(bias), act, act_alpha)
+
+
+@functools.lru_cache(maxsize=256)
+def _int8_workspace_bytes(M, N, K):
+    return load().gn_int8_linear_workspace(M, N, K)
+
+
+def int8_linear(x, B, C, *, col_scale=None, alpha=1.0, beta=0.0, bias=None, act=ACT_NONE, act_alpha=0.0, stream_ptr=None):
+    """int8_gemm with a float32 or float16 matrix x that int8_quantize brings to 8 bits on the way (col_scale: a factor for
+    each of its columns). With the gradient of a layer's outputs as x, the layer's scales as col_scale and
+    (the transposed weights, None) as B: the gradient of the layer's inputs."""
+    dt, rows, K, ldx = _matrix("int8_linear: x", x)
+    w, w_scales, M, N, ldb, ldc = _int8_product("int8_linear", rows, K, B, C, bias)
+    if col_scale is not None:
+        _expect("int8_linear: col_scale", col_scale, _types().float32, K)
+    device = _device_of(x, col_scale, w, w_scales, C, bias)
+    n = _int8_workspace_bytes(M, N, K)
+    ws = _scratch(x, n, device, stream_ptr) if n else None
+    _dispatch_on(device, stream_ptr, "gn_int8_linear", dt, M, N, K, alpha, x.data_ptr(), ldx, _ptr(col_scale), w.data_ptr(), ldb,
+                 _ptr(w_scales), beta, C.data_ptr(), ldc, _ptr(bias), act, act_alpha, _ptr(ws), n)
+
+
+def _history(what, history, rows):
+    """Tokens to a row, 0 without a history."""
+    if history is None:
+        return 0
+    h = _width(history)
+    _expect_rows(what + ": history", history, _types().int64, rows, h)
+    return h
+
+
+def _mask(what, mask, rows, cols):
+    """Words from row to row of a mask, 0 without one."""
+    if mask is None:
+        return 0
+    words, strides = -(-cols // 32), mask.stride()
+    if (mask.dtype is not _types().int32 or mask.dim() != 2 or mask.size(0) != rows or mask.size(1) != words
+            or (strides[1] != 1 and words > 1) or (strides[0] < words and rows > 1)):
+        _refuse(f"{what}: mask: {rows} x {words} int32 with dense rows is needed, got {mask.dtype} {tuple(mask.shape)}, strides {strides}")
+    return strides[0] if rows > 1 else words
+
+
+def adjust_logits(logits, out, *, history=None, prompt=None, repetition=None, frequency=None, presence=None, bias_ids=None,
+                  bias=None, mask=None, stream_ptr=None):
+    """The logits (float32 or float16) as a sampler takes them, to out (their type and shape; may be the logits themselves).
+    history: each row's tokens so far (int64, rows x any number, below 0: none), the first prompt[r] (int64) of them its prompt;
+    repetition, frequency, presence: a float32 for each row; bias_ids, bias: tokens (int64) and
+    what is added to their logits (float32), rows x up to 1024; mask: int32 words of 32 columns, a bit for each allowed one."""
+    T = _types()
+    dt, rows, cols, ld = _matrix("adjust_logits", logits)
+    do, orows, ocols, ldo = _matrix("adjust_logits: out", out)
+    if (do, orows, ocols) != (dt, rows, cols):
+        _refuse("adjust_logits: out has the type and shape of logits")
+    if (bias_ids is None) != (bias is None):
+        _refuse("adjust_logits: bias_ids and bias are given together")
+    if history is None and not (prompt is repetition is frequency is presence is None):
+        _refuse("adjust_logits: penalties and prompt lengths need a history")
+    h = _history("adjust_logits", history, rows)
+    if prompt is not None:
+        _expect("adjust_logits: prompt", prompt, T.int64, rows)
+    for what, t in (("repetition", repetition), ("frequency", frequency), ("presence", presence)):
+        if t is not None:
+            _expect("adjust_logits: " + what, t, T.float32, rows)
+    biases = 0
+    if bias is not None:
+        biases = _width(bias)
+        _expect_rows("adjust_logits: bias_ids", bias_ids, T.int64, rows, biases)
+        _expect_rows("adjust_logits: bias", bias, T.float32, rows, biases)
+    ldmask = _mask("adjust_logits", mask, rows, cols)
+    device = _device_of(logits, out, history, prompt, repetition, frequency, presence, bias_ids, bias, mask)
+    _dispatch_on(device, stream_ptr, "gn_adjust_logits", dt, logits.data_ptr(), rows, cols, ld, _ptr(history), h, _ptr(prompt),
+                 _ptr(repetition), _ptr(frequency), _ptr(presence), _ptr(bias_ids), _ptr(bias), biases, _ptr(mask), ldmask,
+                 out.data_ptr(), ldo)
+
+
+def adjust_logits_backward(logits, grad_out, grad_logits, *, history=None, repetition=None, mask=None, stream_ptr=None):
+    """The gradient of the logits (as they were before adjust_logits) from that of its result, all of one type and
+    shape; grad_logits may be grad_out or the logits. What is only added to logits has no part in it."""
+    T = _types()
+    dt, rows, cols, ld = _matrix("adjust_logits_backward", logits)
+    lds = []
+    for what, t in (("grad_out", grad_out), ("grad_logits", grad_logits)):
+        *kind, ldt = _matrix("adjust_logits_backward: " + what, t)
+        if kind != [dt, rows, cols]:
+            _refuse(f"adjust_logits_backward: {what} has the type and shape of logits")
+        lds.append(ldt)
+    h = _history("adjust_logits_backward", history, rows)
+    if repetition is not None:
+        if history is None:
+            _refuse("adjust_logits_backward: a repetition penalty needs a history")
+        _expect("adjust_logits_backward: repetition", repetition, T.float32, rows)
+    ldmask = _mask("adjust_logits_backward", mask, rows, cols)
+    device = _device_of(logits, grad_out, grad_logits, history, repetition, mask)
+    _dispatch_on(device, stream_ptr, "gn_adjust_logits_backward", dt, logits.data_ptr(), rows, cols, ld, grad_out.data_ptr(), lds[0],
+                 _ptr(history), h, _ptr(repetition), _ptr(mask), ldmask, grad_logits.data_ptr(), lds[1])
 
 
 def spmm_csr(M, N, K, nnz, rowptr, col, val, D, C, flags=None, ldd=None, ldc=None, stream_ptr=None):

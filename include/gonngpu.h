@@ -490,6 +490,63 @@ int gn_distill_backward(int dtype, const void *logits, long rows, long cols, lon
                         const int64_t *ids, const float *teacher, int k, const float *lse, const float *grad_loss,
                         void *grad_logits, long ldg, void *stream, CError *err);
 
+/* Logits before they are sampled from (GN_F32 or GN_F16, rows x cols, cols >= 1, ld >= cols elements from row to row), for
+ * each row in fp32, in this order and each step rounded once:
+ *   y = x / repetition[r] where x > 0, else x repetition[r], for a token of its history
+ *   y -= frequency[r] n, then y -= presence[r], for a token that occurs n > 0 times in its answer
+ *   y += bias, for a token of its bias list
+ *   y = -inf where the mask has no bit
+ * and rounded to the logits' type; other logits are copied as they are. history is rows x history_len tokens, the first
+ * prompt[r] of which are the prompt (prompt NULL: none) and the others the answer. bias_ids and bias are rows x
+ * biases, 0 to 1024; the biases of a token that is listed several times are added up in their order. A token below 0, or of cols or
+ * above, stands for no token. Penalties that are NULL are not applied; repetition is above 0. mask: bit j % 32 of
+ * word j / 32 of a row (ldmask >= ceil(cols / 32) words from row to row) says that column j is allowed; what is masked is -inf
+ * whatever it was, also in a row that allows nothing. out has the logits' type, ldo >= cols, and may be the logits
+ * themselves (ldo == ld). history_len below 2^30. Asynchronous; allocates nothing and may be captured. No result depends on timing.
+ * Codes: -1 invalid argument, -6 launch error. */
+int gn_adjust_logits(int dtype, const void *logits, long rows, long cols, long ld, const int64_t *history, long history_len,
+                     const int64_t *prompt, const float *repetition, const float *frequency, const float *presence,
+                     const int64_t *bias_ids, const float *bias, int biases, const uint32_t *mask, long ldmask, void *out,
+                     long ldo, void *stream, CError *err);
+/* The gradient of the logits from that of the adjusted ones: grad_out divided by repetition[r] where the logit
+ * (as it was before) is above 0, times it otherwise, for a token of the history; grad_out for another; 0 where the mask has
+ * no bit, whatever grad_out holds. All three matrices have one type; grad_logits may be grad_out (ldo == ldg) or the logits
+ * (ldo == ld). Without a history or a repetition the logits are not read (may be NULL). */
+int gn_adjust_logits_backward(int dtype, const void *logits, long rows, long cols, long ld, const void *grad_out, long ldg,
+                              const int64_t *history, long history_len, const float *repetition, const uint32_t *mask,
+                              long ldmask, void *grad_logits, long ldo, void *stream, CError *err);
+
+/* 8-bit integer matrices: a row is int8 values q and one fp32 scale s, and stands for q s. Rows may start anywhere (ldq >= cols
+ * bytes from row to row); the products need them at multiples of 16 bytes.
+ * gn_int8_quantize: x (GN_F32 or GN_F16, rows x cols, ldx >= cols elements from row to row) row by row. With y = x
+ * col_scale[column] in fp32 (y = x where col_scale is NULL): s = max(max |y| / 127, 2^-126) in fp32, q the integer nearest to the
+ * exact quotient y / s, ties to the even one (-127 to 127). A row with an infinity or NaN among its y has scale NaN and q = 0. Bytes
+ * past cols are not written. At most 2^22 rows and 65535 * 2048 columns here and in gn_int8_dequantize. Asynchronous; allocates
+ * nothing and may be captured, as do all of the gn_int8_* calls. Codes: -1 invalid argument, -6 launch error. */
+int gn_int8_quantize(int dtype, const void *x, long rows, long cols, long ldx, const float *col_scale, int8_t *q, long ldq,
+                     float *scales, void *stream, CError *err);
+/* q s, in fp32 and then rounded to GN_F32 or GN_F16; out[r, j] past cols is not written. */
+int gn_int8_dequantize(const int8_t *q, const float *scales, long rows, long cols, long ldq, int dtype, void *out, long ldo,
+                       void *stream, CError *err);
+/* C[M,N] = act( alpha * S * b_scales[n] * a_scales[m] + beta * C + bias[n] ) with S = sum_k A[m,k] B[n,k] (A M x K, B
+ * N x K: a linear layer's weights, outputs x inputs). S is exact, brought to fp32 and multiplied by the column's and then by the row's
+ * scale, each rounded once; scales that are NULL are 1. A, B and, with several rows, lda and ldb are multiples of 16 bytes, the
+ * leading dimensions at most 2^22; a row's bytes from K to the next multiple of 16 are read, the last row's too, and count for
+ * nothing. K is below 2^17, M and N at most 2^25. C and bias are fp32; bias may be NULL; beta == 0 never reads C; act and act_alpha
+ * as gn_gemm; K == 0 gives act(beta * C + bias). Codes: -1 invalid argument, -6 launch error. */
+int gn_int8_gemm(long M, long N, long K, float alpha, const int8_t *A, long lda, const float *a_scales, const int8_t *B,
+                 long ldb, const float *b_scales, float beta, float *C, long ldc, const float *bias, int act, float act_alpha,
+                 void *stream, CError *err);
+/* gn_int8_gemm with activations x (GN_F32 or GN_F16, M x K, ldx elements from row to row) that are brought to 8 bits as by
+ * gn_int8_quantize (the same result, bit for bit). With the gradient of a layer's outputs as x, its weights' scales as col_scale and
+ * the transposed int8 weights without scales as B it gives the gradient of the layer's inputs. At most 2^22 rows of x.
+ * workspace: gn_int8_linear_workspace(M, N, K) bytes at a multiple of 16 (may be NULL where that is 0), not shared by calls
+ * that may overlap. */
+size_t gn_int8_linear_workspace(long M, long N, long K);
+int gn_int8_linear(int dtype, long M, long N, long K, float alpha, const void *x, long ldx, const float *col_scale,
+                   const int8_t *B, long ldb, const float *b_scales, float beta, float *C, long ldc, const float *bias, int act,
+                   float act_alpha, void *workspace, size_t workspace_bytes, void *stream, CError *err);
+
 /* CSR SpMM on device arrays: C[M,N] = S[M,K] * D[K,N] (ld = row pitch in elements).
  * Accumulates each output in CSR order with one fused multiply-add per stored entry.
  * error_flags (2 ints, may be NULL) receive nonzero values if a row pointer pair is
