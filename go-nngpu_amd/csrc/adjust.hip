@@ -16,13 +16,6 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kMaxBiases = 1024;
 
-typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
-
-// 16 bytes at any address that is a multiple of T's size (the hardware takes unaligned vectors).
-template <typename T>
-struct __attribute__((packed, aligned(sizeof(T)))) Unaligned16 {
-  u32x4_t v;
-};
 template <typename T>
 constexpr int kVec = 16 / (int)sizeof(T);
 

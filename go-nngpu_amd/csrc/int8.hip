@@ -13,50 +13,12 @@
 namespace gn {
 namespace {
 
-typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
-typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 
 constexpr long kMaxRows = 1L << 22;  // a workgroup of up to 1024 threads to a row, below 2^32 threads
 
-// 16 bytes at any address that is a multiple of T's size (the hardware takes unaligned vectors).
-template <typename T>
-struct __attribute__((packed, aligned(sizeof(T)))) Unaligned16 {
-  u32x4_t v;
-};
 struct __attribute__((packed, aligned(1))) Unaligned8 {
   u32x2_t v;
-};
-
-// Eight values in their own type, 0 for those at or past `left`.
-template <typename T>
-struct Eight;
-template <>
-struct Eight<float> {
-  u32x4_t v[2];
-  __device__ __forceinline__ float operator[](int i) const { return __uint_as_float(v[i / 4][i % 4]); }
-  __device__ __forceinline__ void load(const float *p, long left) {
-    if (left >= 8) {
-      v[0] = reinterpret_cast<const Unaligned16<float> *>(p)[0].v;
-      v[1] = reinterpret_cast<const Unaligned16<float> *>(p)[1].v;
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i / 4][i % 4] = i < left ? __float_as_uint(p[i]) : 0u;
-    }
-  }
-};
-template <>
-struct Eight<_Float16> {
-  half8_t v;
-  __device__ __forceinline__ float operator[](int i) const { return (float)v[i]; }
-  __device__ __forceinline__ void load(const _Float16 *p, long left) {
-    if (left >= 8) {
-      v = __builtin_bit_cast(half8_t, reinterpret_cast<const Unaligned16<_Float16> *>(p)->v);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = i < left ? p[i] : (_Float16)0.0f;
-    }
-  }
 };
 
 // ------------------------------------------------------------------ quantisation

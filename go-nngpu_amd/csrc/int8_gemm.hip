@@ -1,12 +1,13 @@
 // int8_gemm.hip — products of 8-bit integers, C = act(alpha (sum_k A B) b_scale a_scale + beta C + bias).
 //
-// The sums are exact in 32 bits (K below 2^17). A sum becomes fp32 and is multiplied by its column's scale and then by
-// its row's, each rounded once.
+// The sums are exact in 32 bits (K below 2^17). A sum becomes fp32, is multiplied by its column's scale, and then by alpha times its
+// row's in one step with the addition of what beta and the bias give.
 #include <algorithm>
 #include <climits>
 
 #include "gemm_tile.h"
 #include "int8.h"
+#include "int8_round.h"
 
 namespace gn {
 namespace {
@@ -33,103 +34,318 @@ __device__ __forceinline__ i32x4_t first_bytes(i32x4_t v, int n) {
   return v;
 }
 
-__device__ __forceinline__ float finish(const Int8Params &p, float v, long m, long n) {
-  v *= p.alpha;
-  if (p.beta != 0.0f) v += p.beta * p.C[m * p.ldc + n];
-  if (p.bias) v += p.bias[n];
-  return apply_act(p.act, v, p.act_alpha);
+struct __attribute__((packed, aligned(4))) Unaligned4 {
+  float4_t v;  // the hardware takes vectors at any address that is a multiple of 4
+};
+
+// The factor of a row's sums, and what becomes of a sum times its column's scale.
+__device__ __forceinline__ float row_factor(const Int8Params &p, long m) { return p.as ? p.alpha * p.as[m] : p.alpha; }
+__device__ __forceinline__ float finish(const Int8Params &p, float v, float factor, long m, long n) {
+  float t = p.bias ? p.bias[n] : 0.0f;
+  if (p.beta != 0.0f) t = fmaf(p.beta, p.C[m * p.ldc + n], t);
+  return apply_act(p.act, fmaf(v, factor, t), p.act_alpha);
+}
+// Columns n .. n + 3 of row m, those inside the matrix.
+__device__ __forceinline__ void finish4(const Int8Params &p, i32x4_t q, float factor, long m, long n) {
+  if (n + 3 < p.N) {
+    const float4_t one = {1.0f, 1.0f, 1.0f, 1.0f}, zero = {0.0f, 0.0f, 0.0f, 0.0f};
+    const float4_t b = p.bs ? reinterpret_cast<const Unaligned4 *>(p.bs + n)->v : one;
+    float4_t v = p.bias ? reinterpret_cast<const Unaligned4 *>(p.bias + n)->v : zero;
+    float *dst = p.C + m * p.ldc + n;
+    if (p.beta != 0.0f) {
+      const float4_t old = reinterpret_cast<const Unaligned4 *>(dst)->v;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = fmaf(p.beta, old[e], v[e]);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = apply_act(p.act, fmaf((float)q[e] * b[e], factor, v[e]), p.act_alpha);
+    reinterpret_cast<Unaligned4 *>(dst)->v = v;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (n + e < p.N) p.C[m * p.ldc + n + e] = finish(p, (float)q[e] * (p.bs ? p.bs[n + e] : 1.0f), factor, m, n + e);
+  }
 }
 
 // K == 0: act(beta C + bias).
 __global__ void __launch_bounds__(256) i8_k0_kernel(Int8Params p) {
   for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < p.M * p.N; i += (long)gridDim.x * 256)
-    p.C[i / p.N * p.ldc + i % p.N] = finish(p, 0.0f, i / p.N, i % p.N);
+    p.C[i / p.N * p.ldc + i % p.N] = finish(p, 0.0f, 1.0f, i / p.N, i % p.N);
 }
 
-// ------------------------------------------------------------------ few rows
-// A workgroup takes all rows (MF blocks of 16) and 16 NF columns; its KW waves take steps of 128 k in turn, each with D
-// steps of A and B in registers, and their sums meet in LDS. Rows and columns past the matrix are the last ones again, not stored.
-template <int MF, int NF, int KW, int D>
-__global__ void __launch_bounds__(KW * 64) i8_rows_kernel(Int8Params p) {
-  __shared__ i32x4_t part[KW][MF * NF][64];
+// ------------------------------------------------------------------ small products
+// A workgroup takes 16 MF rows and 16 NF columns; its KW waves cut K among them, in steps of S bytes that they take in turn, and
+// their sums meet in LDS at the end. Each wave copies what it multiplies into slots of its own, NS steps ahead, so nothing is
+// waited for but a wave's own copies: there is no barrier in the loop.
+// A fragment asked for from memory as the instruction wants it (lane % 16 its row) spreads each four lanes over four rows, which a
+// CU's address unit takes at 38 KB/us, from the caches too; copied to LDS in whole pieces of S bytes to a row the same
+// bytes come at up to 90 (from L2; the Infinity Cache gives all CUs together 7.5 TB/s, 29 KB/us each).
+// A chunk of 1 KiB is RPC rows of S bytes; octet o of a row sits at place o ^ swizzle(row): the 16 rows that a phase of a fragment
+// read touches fall on distinct banks.
+template <int S>
+struct Chunk {
+  static_assert(S == 64 || S == 128, "bytes to a row");
+  static constexpr int RPC = 1024 / S, OCTETS = S / 16;
+  static __device__ __forceinline__ int swizzle(int row) { return S == 128 ? (row >> 1) & 7 : (row >> 2) & 3; }
+  static __device__ __forceinline__ int row(int lane) { return lane / OCTETS; }                            // of the chunk
+  static __device__ __forceinline__ int octet(int row, int lane) { return (lane % OCTETS) ^ swizzle(row); }
+  static __device__ __forceinline__ unsigned place(int row, int o) { return row * S + 16 * (o ^ swizzle(row)); }
+};
+
+// dma16 from voff + soff; both together below 2^31 where voff is in range.
+__device__ __forceinline__ void dma16_at(const BufRsrc &s, unsigned voff, unsigned soff, unsigned lds) {
+  int saved;
+  asm volatile(
+      "s_mov_b32 %0, m0\n\t"
+      "s_mov_b32 m0, %4\n\t"
+      "buffer_load_dwordx4 %1, %2, %3 offen lds\n\t"
+      "s_mov_b32 m0, %0"
+      : "=&s"(saved)
+      : "v"(voff), "s"(s.r), "s"(soff), "s"(lds)
+      : "memory");
+}
+
+// The waves' sums of MF x NF blocks, which take the slots' place in LDS, added up: write(i, j, v) for each block, by one wave.
+template <int MF, int NF, int KW, typename F>
+__device__ __forceinline__ void join_waves(char *smem, const i32x4_t (&acc)[MF][NF], int wave, int lane, F write) {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();  // no copy is under way
+  i32x4_t *part = reinterpret_cast<i32x4_t *>(smem);
+#pragma unroll
+  for (int i = 0; i < MF; ++i)
+#pragma unroll
+    for (int j = 0; j < NF; ++j) part[(wave * MF * NF + i * NF + j) * 64 + lane] = acc[i][j];
+  __syncthreads();
+#pragma unroll 1
+  for (int f = wave; f < MF * NF; f += KW) {
+    i32x4_t v = part[f * 64 + lane];
+#pragma unroll
+    for (int w = 1; w < KW; ++w) v += part[(w * MF * NF + f) * 64 + lane];
+    write(f / NF, f % NF, v);
+  }
+}
+
+template <int MF, int NF, int KW, int S, int NS>
+__global__ void __launch_bounds__(KW * 64) i8_stream_kernel(Int8Params p) {
+  using C = Chunk<S>;
+  constexpr int H = S / 64;                                // instructions' k to a step
+  constexpr int CA = 16 * MF / C::RPC, CB = 16 * NF / C::RPC, CPS = CA + CB, SLOT = CPS * 1024;
+  constexpr int RING = KW * NS * SLOT, PART = KW * MF * NF * 1024;
+  static_assert(CA >= 1 && CB >= 1 && (NS - 1) * CPS < 64, "copies");
+  __shared__ __attribute__((aligned(1024))) char smem[RING > PART ? RING : PART];
+  int tm, tn;
+  tile_coords(p, tm, tn);
+  const long m0 = (long)tm * 16 * MF, n0 = (long)tn * 16 * NF;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-  const long n0 = (long)blockIdx.x * 16 * NF, m0 = (long)blockIdx.y * 16 * MF;
-  const int8_t *ap[MF], *bp[NF];
+
+  const BufRsrc da = make_rsrc(static_cast<const char *>(p.A) + m0 * p.lda), db = make_rsrc(static_cast<const char *>(p.B) + n0 * p.ldb);
+  unsigned va[CA], vb[CB];
+  int ka[CA], kb[CB];
 #pragma unroll
-  for (int i = 0; i < MF; ++i) ap[i] = static_cast<const int8_t *>(p.A) + min(m0 + 16 * i + r, p.M - 1) * p.lda + 16 * g;
+  for (int i = 0; i < CA; ++i) {
+    const int row = C::RPC * i + C::row(lane);
+    ka[i] = 16 * C::octet(row, lane);
+    va[i] = m0 + row < p.M ? (unsigned)(row * p.lda) + ka[i] : kOutOfRange;
+  }
 #pragma unroll
-  for (int j = 0; j < NF; ++j) bp[j] = static_cast<const int8_t *>(p.B) + min(n0 + 16 * j + r, p.N - 1) * p.ldb + 16 * g;
+  for (int i = 0; i < CB; ++i) {
+    const int row = C::RPC * i + C::row(lane);
+    kb[i] = 16 * C::octet(row, lane);
+    vb[i] = n0 + row < p.N ? (unsigned)(row * p.ldb) + kb[i] : kOutOfRange;
+  }
+  const unsigned lds = lds_offset(smem) + wave * NS * SLOT;
+  const int K = (int)p.K;
+  auto issue = [&](int t, int slot) {  // of the wave's steps; past K all reads are zeros
+    const int k = (wave + t * KW) * S, left = K - k;
+    const unsigned to = lds + slot * SLOT;
+    if (left >= S) {
+#pragma unroll
+      for (int i = 0; i < CB; ++i) dma16_at(db, vb[i], k, __builtin_amdgcn_readfirstlane(to + (CA + i) * 1024));
+#pragma unroll
+      for (int i = 0; i < CA; ++i) dma16_at(da, va[i], k, __builtin_amdgcn_readfirstlane(to + i * 1024));
+    } else {
+#pragma unroll
+      for (int i = 0; i < CB; ++i)
+        dma16_at(db, kb[i] < left ? vb[i] : kOutOfRange, left > 0 ? k : 0, __builtin_amdgcn_readfirstlane(to + (CA + i) * 1024));
+#pragma unroll
+      for (int i = 0; i < CA; ++i)
+        dma16_at(da, ka[i] < left ? va[i] : kOutOfRange, left > 0 ? k : 0, __builtin_amdgcn_readfirstlane(to + i * 1024));
+    }
+  };
   i32x4_t acc[MF][NF];
 #pragma unroll
   for (int i = 0; i < MF; ++i)
 #pragma unroll
     for (int j = 0; j < NF; ++j) acc[i][j] = i32x4_t{0, 0, 0, 0};
+  const int steps = (K + S - 1) / S, mine = wave < steps ? (steps - wave + KW - 1) / KW : 0;
+#pragma unroll 1
+  for (int t = 0; t < NS; ++t) issue(t, t);
+  int slot = 0;
+  for (int t = 0; t < mine; ++t) {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NS - 1) * CPS) : "memory");
+    const char *at = smem + (wave * NS + slot) * SLOT;
+    i32x4_t a[H][MF], b[H][NF];
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+#pragma unroll
+      for (int j = 0; j < NF; ++j) b[h][j] = *reinterpret_cast<const i32x4_t *>(at + CA * 1024 + C::place(16 * j + r, 4 * h + g));
+#pragma unroll
+      for (int i = 0; i < MF; ++i) a[h][i] = *reinterpret_cast<const i32x4_t *>(at + C::place(16 * i + r, 4 * h + g));
+    }
+    const int left = K - (wave + t * KW) * S;
+    if (left < S) {  // A's bytes past K, which belong to its rows, as zeros
+#pragma unroll
+      for (int h = 0; h < H; ++h)
+#pragma unroll
+        for (int i = 0; i < MF; ++i) a[h][i] = first_bytes(a[h][i], left - 64 * h - 16 * g);
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the slot has been read
+    issue(t + NS, slot);
+#pragma unroll
+    for (int h = 0; h < H; ++h)
+#pragma unroll
+      for (int i = 0; i < MF; ++i)
+#pragma unroll
+        for (int j = 0; j < NF; ++j) acc[i][j] = mfma_i8(b[h][j], a[h][i], acc[i][j]);
+    slot = slot + 1 == NS ? 0 : slot + 1;
+  }
+  join_waves<MF, NF, KW>(smem, acc, wave, lane, [&](int i, int j, i32x4_t v) {
+    const long m = m0 + 16 * i + r;
+    if (m < p.M) finish4(p, v, row_factor(p, m), m, n0 + 16 * j + 4 * g);
+  });
+}
 
-  i32x4_t a[D][2][MF], b[D][2][NF];
-  auto load = [&](int d, long k) {
+// One token, or a few (up to kFewTokens rows), of activations that the kernel brings to 8 bits itself: each workgroup does so, into LDS,
+// while the first of its weights are on their way. A launch and a wait for it less than with a kernel before it.
+constexpr int kFewTokens = 8;
+constexpr int kTokenBytes = 48 * 1024;  // of LDS for the rows
+__host__ __device__ inline int token_pitch(long K) { return (int)((K + 127) / 128 * 128 + 16); }  // rows on distinct banks
+template <typename T, int NF, int KW, int NS>
+__global__ void __launch_bounds__(KW * 64) i8_token_kernel(Int8Params p, const T *x, long ldx, const float *col_scale) {
+  using C = Chunk<128>;
+  constexpr int CB = 16 * NF / C::RPC, SLOT = CB * 1024, HOLD = 4;
+  constexpr int RING = KW * NS * SLOT, PART = KW * NF * 1024;
+  static_assert((NS - 1) * CB < 64, "copies");
+  __shared__ uint32_t tops[KW];
+  __shared__ float scales[kFewTokens];
+  extern __shared__ __attribute__((aligned(1024))) char smem[];  // the slots, in the end the partial sums; the rows in 8 bits
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+  const int M = (int)p.M, K = (int)p.K, pitch = token_pitch(K);
+  char *rows = smem + (RING > PART ? RING : PART);
+  // Waves to a row, and this wave's part of its row: chunks of 8 values, a lane each.
+  const int lr = M <= 1 ? 0 : M <= 2 ? 1 : M <= 4 ? 2 : 3, per = KW >> lr, mine = wave / per, part = wave % per;
+  const T *row = x + (long)min(mine, M - 1) * ldx;
+  auto value = [&](const Eight<T> &v, const Eight<float> &c, int i) { return col_scale ? v[i] * c[i] : v[i]; };
+  Eight<T> v[HOLD];
+  Eight<float> c[HOLD];
+#pragma unroll
+  for (int e = 0; e < HOLD; ++e) {
+    const int at = 8 * ((e * per + part) * 64 + lane);
+    v[e].load(row + at, K - at);
+    if (col_scale) c[e].load(col_scale + at, K - at);
+  }
+  uint32_t top = 0;
+  auto reduce = [&](const Eight<T> &a, const Eight<float> &b) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(value(a, b, i)) & 0x7fffffffu);
+  };
+#pragma unroll
+  for (int e = 0; e < HOLD; ++e) reduce(v[e], c[e]);
+  for (int at = 8 * ((HOLD * per + part) * 64 + lane); at < K; at += 8 * per * 64) {
+    Eight<T> a;
+    Eight<float> b;
+    a.load(row + at, K - at);
+    if (col_scale) b.load(col_scale + at, K - at);
+    reduce(a, b);
+  }
+
+  // The row has been read: the weights' first steps on their way. (Before, the wait for the row would be one for them too.)
+  const long n0 = (long)blockIdx.x * 16 * NF;
+  const BufRsrc db = make_rsrc(static_cast<const char *>(p.B) + n0 * p.ldb);
+  unsigned vb[CB];
+  int kb[CB];
+#pragma unroll
+  for (int i = 0; i < CB; ++i) {
+    const int br = C::RPC * i + C::row(lane);
+    kb[i] = 16 * C::octet(br, lane);
+    vb[i] = n0 + br < p.N ? (unsigned)(br * p.ldb) + kb[i] : kOutOfRange;
+  }
+  const unsigned lds = lds_offset(smem) + wave * NS * SLOT;
+  auto issue = [&](int t, int slot) {  // of the wave's steps; past K all reads are zeros
+    const int k = (wave + t * KW) * 128, left = K - k;
+    const unsigned to = lds + slot * SLOT;
+    if (left >= 128) {
+#pragma unroll
+      for (int i = 0; i < CB; ++i) dma16_at(db, vb[i], k, __builtin_amdgcn_readfirstlane(to + i * 1024));
+    } else {
+#pragma unroll
+      for (int i = 0; i < CB; ++i)
+        dma16_at(db, kb[i] < left ? vb[i] : kOutOfRange, left > 0 ? k : 0, __builtin_amdgcn_readfirstlane(to + i * 1024));
+    }
+  };
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int t = 0; t < NS; ++t) issue(t, t);
+  __builtin_amdgcn_sched_barrier(0);
+
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
+  if (lane == 0) tops[wave] = top;
+  lds_barrier();
+  for (int w = 0; w < per; ++w) top = max(top, tops[mine * per + w]);
+  const float s = int8_scale(top), inv = 1.0f / s;
+  const bool bad = s != s;
+  if (mine < M) {
+    if (part == 0 && lane == 0) scales[mine] = s;
+    auto store = [&](const Eight<T> &a, const Eight<float> &b, int at) {
+      float y[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = bad ? 0.0f : int8_round(value(a, b, i), s, inv);
+      *reinterpret_cast<u32x2_t *>(rows + mine * pitch + at) = u32x2_t{int8_pack(y[0], y[1], y[2], y[3]), int8_pack(y[4], y[5], y[6], y[7])};
+    };
+    const int end = pitch - 16;  // zeros from K on
+#pragma unroll
+    for (int e = 0; e < HOLD; ++e) {
+      const int at = 8 * ((e * per + part) * 64 + lane);
+      if (at < end) store(v[e], c[e], at);
+    }
+    for (int at = 8 * ((HOLD * per + part) * 64 + lane); at < end; at += 8 * per * 64) {
+      Eight<T> a;
+      Eight<float> b;
+      a.load(row + at, K - at);
+      if (col_scale) b.load(col_scale + at, K - at);
+      store(a, b, at);
+    }
+  }
+  lds_barrier();
+
+  i32x4_t acc[1][NF];
+#pragma unroll
+  for (int j = 0; j < NF; ++j) acc[0][j] = i32x4_t{0, 0, 0, 0};
+  const int steps = (K + 127) / 128, count = wave < steps ? (steps - wave + KW - 1) / KW : 0;
+  const char *arow = rows + min(r, M - 1) * pitch + 16 * g;
+  int slot = 0;
+  for (int t = 0; t < count; ++t) {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NS - 1) * CB) : "memory");
+    const char *at = smem + (wave * NS + slot) * SLOT;
+    i32x4_t a[2], b[2][NF];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
 #pragma unroll
-      for (int j = 0; j < NF; ++j) b[d][h][j] = *reinterpret_cast<const i32x4_t *>(bp[j] + k + 64 * h);
-#pragma unroll
-      for (int i = 0; i < MF; ++i) a[d][h][i] = *reinterpret_cast<const i32x4_t *>(ap[i] + k + 64 * h);
+      for (int j = 0; j < NF; ++j) b[h][j] = *reinterpret_cast<const i32x4_t *>(at + C::place(16 * j + r, 4 * h + g));
+      a[h] = *reinterpret_cast<const i32x4_t *>(arow + (wave + t * KW) * 128 + 64 * h);
     }
-  };
-  auto multiply = [&](int d) {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the slot has been read
+    issue(t + NS, slot);
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int i = 0; i < MF; ++i)
-#pragma unroll
-        for (int j = 0; j < NF; ++j) acc[i][j] = mfma_i8(a[d][h][i], b[d][h][j], acc[i][j]);
-  };
-  const int full = (int)(p.K / 128);  // whole steps; this wave has steps wave, wave + KW, ...
-  const int mine = wave < full ? (full - wave + KW - 1) / KW : 0;
-  const long k0 = 128L * wave;
-#pragma unroll
-  for (int d = 0; d < D; ++d)
-    if (d < mine) load(d, k0 + 128L * KW * d);
-  for (int t = 0; t < mine; t += D) {
-#pragma unroll
-    for (int d = 0; d < D; ++d) {
-      if (t + d >= mine) break;
-      multiply(d);
-      if (t + d + D < mine) load(d, k0 + 128L * KW * (t + d + D));
-      __builtin_amdgcn_sched_barrier(0);
-    }
+      for (int j = 0; j < NF; ++j) acc[0][j] = mfma_i8(b[h][j], a[h], acc[0][j]);
+    slot = slot + 1 == NS ? 0 : slot + 1;
   }
-  // The rest of K: chunks of 16 that begin inside it (their other bytes belong to the rows too), A's bytes past K as zeros.
-  if (p.K % 128 != 0 && wave == full % KW) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const long k = 128L * full + 64 * h;
-      const int left = (int)(p.K - k) - 16 * g;  // of this lane's chunk
-#pragma unroll
-      for (int j = 0; j < NF; ++j) b[0][h][j] = left > 0 ? *reinterpret_cast<const i32x4_t *>(bp[j] + k) : i32x4_t{0, 0, 0, 0};
-#pragma unroll
-      for (int i = 0; i < MF; ++i)
-        a[0][h][i] = left > 0 ? first_bytes(*reinterpret_cast<const i32x4_t *>(ap[i] + k), left) : i32x4_t{0, 0, 0, 0};
-    }
-    multiply(0);
-  }
-#pragma unroll
-  for (int i = 0; i < MF; ++i)
-#pragma unroll
-    for (int j = 0; j < NF; ++j) part[wave][i * NF + j][lane] = acc[i][j];
-  __syncthreads();
-  for (int f = wave; f < MF * NF; f += KW) {
-    i32x4_t v = part[0][f][lane];
-#pragma unroll
-    for (int w = 1; w < KW; ++w) v += part[w][f][lane];
-    const long n = n0 + 16 * (f % NF) + r;
-    if (n >= p.N) continue;
-    const float bs = p.bs ? p.bs[n] : 1.0f;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const long m = m0 + 16 * (f / NF) + 4 * g + e;
-      if (m < p.M) p.C[m * p.ldc + n] = finish(p, (float)v[e] * bs * (p.as ? p.as[m] : 1.0f), m, n);
-    }
-  }
+  join_waves<1, NF, KW>(smem, acc, wave, lane, [&](int, int j, i32x4_t v) {
+    if (r < M) finish4(p, v, p.alpha * scales[r], r, n0 + 16 * j + 4 * g);
+  });
 }
 
 // ------------------------------------------------------------------ many rows
@@ -138,15 +354,22 @@ __global__ void __launch_bounds__(KW * 64) i8_rows_kernel(Int8Params p) {
 // in LDS. A stage is two steps of 64 k: while one is multiplied the next one's fragments are read, and before the
 // second the next stage has landed (one wait and one barrier to a stage) and the copies of the one NS ahead start.
 // Where K ends inside a chunk of 16 the wave that copied it clears A's bytes past K before that barrier.
+template <int WM, int WN, int FM, int FN, int NS>
+struct I8Tile {
+  static constexpr int BM = WM * FM * 16, BN = WN * FN * 16, STAGE = (BM + BN) * 128;
+  static constexpr int ALL = BM * (BN + 4) * 4, PARTS = ALL > 140 * 1024 ? 2 : 1, SUMS = ALL / PARTS;  // the sums, all at once or in halves
+  static constexpr int EPI = SUMS + (BM + 2 * BN) * 4;                                                 // with the scales and the bias
+  static constexpr int BYTES = NS * STAGE > EPI ? NS * STAGE : EPI;
+};
 template <int WM, int WN, int FM, int FN, int NS, int WPE>
 __global__ void __launch_bounds__(WM * WN * 64) __attribute__((amdgpu_waves_per_eu(WPE, WPE)))
 i8_tile_kernel(Int8Params p) {
-  constexpr int NW = WM * WN, NT = NW * 64, BM = WM * FM * 16, BN = WN * FN * 16;
+  using Tile = I8Tile<WM, WN, FM, FN, NS>;
+  constexpr int NW = WM * WN, NT = NW * 64, BM = Tile::BM, BN = Tile::BN, STAGE = Tile::STAGE;
   constexpr int CA = BM / 8 / NW, CB = BN / 8 / NW, CPW = CA + CB;
-  constexpr int STAGE = (BM + BN) * 128, EPI = WM * 16 * (BN + 4) * 4;
-  static_assert(CA * NW * 8 == BM && CB * NW * 8 == BN && CA % 2 == 0 && CB % 2 == 0, "chunks");
-  static_assert(EPI + (BM + BN) * 4 <= NS * STAGE && (NS - 1) * CPW < 64 && NS >= 2, "LDS");
-  __shared__ __attribute__((aligned(1024))) char smem[NS * STAGE];
+  static_assert(CA * NW * 8 == BM && CB * NW * 8 == BN, "chunks");
+  static_assert((NS - 1) * CPW < 64 && NS >= 2 && FM % Tile::PARTS == 0 && NT >= BN / 4, "copies and rows");
+  __shared__ __attribute__((aligned(1024))) char smem[Tile::BYTES];
 
   int tm, tn;
   tile_coords(p, tm, tn);
@@ -163,7 +386,7 @@ i8_tile_kernel(Int8Params p) {
     const int at = threadIdx.x + i * NT;
     scale[i] = 1.0f;
     if (at < BM) {
-      if (p.as && m0 + at < p.M) scale[i] = p.as[m0 + at];
+      scale[i] = p.alpha * (p.as && m0 + at < p.M ? p.as[m0 + at] : 1.0f);
     } else if (at < BM + BN) {
       if (p.bs && n0 + at - BM < p.N) scale[i] = p.bs[n0 + at - BM];
     }
@@ -239,11 +462,11 @@ i8_tile_kernel(Int8Params p) {
 #pragma unroll
     for (int i = i0; i < i1; ++i)
 #pragma unroll
-      for (int j = 0; j < FN; ++j) acc[i][j] = mfma_i8(fa[h][i], fb[h][j], acc[i][j]);
+      for (int j = 0; j < FN; ++j) acc[i][j] = mfma_i8(fb[h][j], fa[h][i], acc[i][j]);
   };
 
   const bool tail = p.K % 16 != 0;
-#pragma unroll
+#pragma unroll 1
   for (int t = 0; t < NS; ++t) {
     issue_a(t, t);
     issue_b(t, t);
@@ -290,29 +513,89 @@ i8_tile_kernel(Int8Params p) {
     cur = nxt;
   }
   __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
-  __syncthreads();  // no copy is under way and all waves are done with the stages: the epilogue takes their place
-  constexpr int LP = BN + 4;
-  float *stg = reinterpret_cast<float *>(smem), *sa = reinterpret_cast<float *>(smem + EPI), *sb = sa + BM;
+  __syncthreads();  // no copy is under way and all waves are done with the stages: the sums take their place
+  // The sides of the products are changed, so that lane (r, g) of a block has row r, columns 4 g .. 4 g + 3: one 16-byte write to
+  // LDS for each block, and from there whole rows of the tile go out through a short loop. Straight code for all of
+  // a thread's sums, as the other products' epilogue has it, costs more in instructions that nobody has in a cache yet (70 KB of
+  // code; a single tile of 256 x 256 with K = 128 took 13.5 us) than what it does.
+  float *sa = reinterpret_cast<float *>(smem + Tile::SUMS), *sb = sa + BM, *bias = sb + BN;
 #pragma unroll
-  for (int i = 0; i < SPT; ++i)
-    if (threadIdx.x + i * NT < BM + BN) sa[threadIdx.x + i * NT] = scale[i];
-  store_tile_passes<BM, BN, WM, WN>(p, m0, n0, 0, stg, [&](int f) {
-    const float4_t s = *reinterpret_cast<const float4_t *>(sa + (wm * FM + f) * 16 + 4 * g);
+  for (int i = 0; i < SPT; ++i) {
+    const int at = threadIdx.x + i * NT;
+    if (at < BM + BN) sa[at] = scale[i];
+  }
+  for (int i = threadIdx.x; i < BN; i += NT) bias[i] = p.bias && n0 + i < p.N ? p.bias[n0 + i] : 0.0f;
+  constexpr int LP = BN + 4, CPR = BN / 4, RPS = NT / CPR, PARTS = Tile::PARTS, FP = FM / PARTS, ROWS = BM / PARTS;
+  int *sums = reinterpret_cast<int *>(smem);
+  const int c4 = threadIdx.x % CPR, r0 = threadIdx.x / CPR;  // threads with r0 >= RPS only write to LDS
+  const long col = n0 + 4 * c4;
+  auto dump = [&](auto part) {
+    constexpr int P = decltype(part)::value;
 #pragma unroll
-    for (int j = 0; j < FN; ++j) {
-      const int col = (wn * FN + j) * 16 + r;
+    for (int i = 0; i < FP; ++i)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) stg[(wm * 16 + 4 * g + e) * LP + col] = (float)acc[f][j][e] * sb[col] * s[e];
+      for (int j = 0; j < FN; ++j)
+        *reinterpret_cast<i32x4_t *>(sums + ((wm * FP + i) * 16 + r) * LP + (wn * FN + j) * 16 + 4 * g) = acc[P * FP + i][j];
+  };
+  auto sweep = [&](int part, auto act_c) {
+    constexpr int ACT = decltype(act_c)::value;
+    const int act = ACT == kActRuntime ? p.act : ACT;
+    const float4_t bs = *reinterpret_cast<const float4_t *>(sb + 4 * c4), bv = *reinterpret_cast<const float4_t *>(bias + 4 * c4);
+#pragma unroll 2
+    for (int t = r0; t < ROWS; t += RPS) {
+      const int row = (t / (FP * 16) * FM + part * FP) * 16 + t % (FP * 16);  // of the tile
+      if (m0 + row >= p.M) continue;
+      const i32x4_t q = *reinterpret_cast<const i32x4_t *>(sums + t * LP + 4 * c4);
+      const float as = sa[row];
+      float *dst = p.C + (m0 + row) * p.ldc + col;
+      float4_t v = bv;
+      if (col + 3 < p.N) {
+        if (p.beta != 0.0f) {
+          const float4_t old = reinterpret_cast<const Unaligned4 *>(dst)->v;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = fmaf(p.beta, old[e], v[e]);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = apply_act(act, fmaf((float)q[e] * bs[e], as, v[e]), p.act_alpha);
+        __builtin_nontemporal_store(v, &reinterpret_cast<Unaligned4 *>(dst)->v);  // C is not read again: keep L2 for A and B
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (col + e < p.N) {
+            if (p.beta != 0.0f) v[e] = fmaf(p.beta, dst[e], v[e]);
+            dst[e] = apply_act(act, fmaf((float)q[e] * bs[e], as, v[e]), p.act_alpha);
+          }
+        }
+      }
     }
-  });
+  };
+#pragma unroll 1
+  for (int part = 0; part < PARTS; ++part) {
+    if (part == 0)
+      dump(ActCode<0>{});
+    else
+      dump(ActCode<PARTS - 1>{});
+    lds_barrier();
+    if (r0 < RPS) {
+      switch (p.act) {
+        case -1: sweep(part, ActCode<-1>{}); break;
+        case 0: sweep(part, ActCode<0>{}); break;
+        case 7: sweep(part, ActCode<7>{}); break;
+        default: sweep(part, ActCode<kActRuntime>{}); break;
+      }
+    }
+    lds_barrier();
+  }
 }
 
 unsigned grid_of(long n, long per) { return (unsigned)std::max(1L, std::min((n + per - 1) / per, 1L << 20)); }
 
-template <int MF, int NF, int KW, int D>
-void launch_rows(const Int8Params &p, hipStream_t s) {
-  const dim3 grid((unsigned)((p.N + 16 * NF - 1) / (16 * NF)), (unsigned)((p.M + 16 * MF - 1) / (16 * MF)));
-  hipLaunchKernelGGL((i8_rows_kernel<MF, NF, KW, D>), grid, dim3(KW * 64), 0, s, p);
+template <int MF, int NF, int KW, int S, int NS>
+void launch_stream(Int8Params p, hipStream_t s) {
+  p.tiles_m = (int)((p.M + 16 * MF - 1) / (16 * MF));
+  p.tiles_n = (int)((p.N + 16 * NF - 1) / (16 * NF));
+  p.group_m = p.tiles_m;  // the rows' blocks of some columns side by side: those columns are read once by their XCD
+  hipLaunchKernelGGL((i8_stream_kernel<MF, NF, KW, S, NS>), dim3((unsigned)(p.tiles_m * p.tiles_n)), dim3(KW * 64), 0, s, p);
 }
 
 template <int WM, int WN, int FM, int FN, int NS, int WPE>
@@ -321,6 +604,73 @@ void launch_tiles(Int8Params p, hipStream_t s) {
   p.tiles_m = (int)((p.M + BM - 1) / BM);
   p.tiles_n = (int)((p.N + BN - 1) / BN);
   hipLaunchKernelGGL((i8_tile_kernel<WM, WN, FM, FN, NS, WPE>), dim3((unsigned)(p.tiles_m * p.tiles_n)), dim3(WM * WN * 64), 0, s, p);
+}
+
+// The kind of tile with which a CU's share takes the least time, the first of equals. Of a tile alone on a CU: fixed, in 10 ns, and
+// for each 128 of K; more: for each further tile of its share.
+struct TileCost {
+  int bm, bn, fixed, alone, more;
+};
+// Measured, us: 4096 -> 11008 ...
+constexpr TileCost kTiles[] = {{16, 16, 250, 7, 7},    {16, 64, 250, 20, 19},  {32, 16, 250, 13, 14},  {32, 32, 250, 16, 17},
+                               {32, 64, 250, 28, 19},  {64, 64, 250, 33, 20},  {64, 128, 250, 40, 33}, {128, 128, 300, 65, 60},
+                               {128, 192, 350, 80, 72}, {128, 256, 400, 100, 90}, {256, 256, 1000, 125, 180}};
+void launch_product(const Int8Params &p, hipStream_t s) {
+  const long stages = (p.K + 127) / 128;
+  int best = 0;
+  long least = 0;
+  for (int i = 0; i < (int)(sizeof(kTiles) / sizeof(kTiles[0])); ++i) {
+    const TileCost &k = kTiles[i];
+    const long tiles = ((p.M + k.bm - 1) / k.bm) * ((p.N + k.bn - 1) / k.bn), share = (tiles + 255) / 256;  // 256 CUs
+    const long cost = k.fixed + stages * (k.alone + (share - 1) * k.more);
+    if (i == 0 || cost < least) best = i, least = cost;
+  }
+  switch (best) {
+    case 0: return launch_stream<1, 1, 4, 128, 4>(p, s);
+    case 1: return launch_stream<1, 4, 8, 128, 2>(p, s);
+    case 2: return launch_stream<2, 1, 8, 128, 2>(p, s);
+    case 3: return launch_stream<2, 2, 8, 128, 2>(p, s);
+    case 4: return launch_stream<2, 4, 8, 64, 2>(p, s);
+    case 5: return launch_tiles<2, 2, 2, 2, 4, 2>(p, s);
+    case 6: return launch_tiles<2, 2, 2, 4, 3, 2>(p, s);
+    case 7: return launch_tiles<2, 4, 4, 2, 3, 2>(p, s);
+    case 8: return launch_tiles<2, 4, 4, 3, 3, 2>(p, s);
+    case 9: return launch_tiles<2, 4, 4, 4, 3, 2>(p, s);
+    default: return launch_tiles<2, 4, 8, 4, 2, 2>(p, s);
+  }
+}
+
+// Few tokens' activations, brought to 8 bits in the product's kernel.
+bool few_tokens(long M, long K) { return M <= kFewTokens && M * token_pitch(K) <= kTokenBytes; }
+template <typename T, int NF, int KW, int NS>
+void launch_token(const Int8LinearDesc &d, const Int8Params &p, hipStream_t s) {
+  const int ring = KW * NF * 1024 * std::max(1, 2 * NS);
+  hipLaunchKernelGGL((i8_token_kernel<T, NF, KW, NS>), dim3((unsigned)((p.N + 16 * NF - 1) / (16 * NF))), dim3(KW * 64),
+                     ring + (int)p.M * token_pitch(p.K), s, p, static_cast<const T *>(d.x), d.gemm.M > 1 ? d.ldx : 0, d.col_scale);
+}
+template <typename T>
+void launch_tokens(const Int8LinearDesc &d, const Int8Params &p, hipStream_t s) {
+  launch_token<T, 1, 8, 2>(d, p, s);
+}
+
+Int8Params params_of(const Int8GemmDesc &d) {
+  Int8Params p{};
+  p.A = d.A;
+  p.as = d.a_scales;
+  p.B = d.B;
+  p.bs = d.b_scales;
+  p.C = d.C;
+  p.bias = d.bias;
+  p.M = d.M, p.N = d.N, p.K = d.K, p.ldc = d.ldc;
+  p.lda = d.M > 1 ? d.lda : 0;
+  p.ldb = d.N > 1 ? d.ldb : 0;
+  p.alpha = d.alpha, p.beta = d.beta, p.act = d.act, p.act_alpha = d.act_alpha;
+  return p;
+}
+
+int launched(const char *what, CError *err) {
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? 0 : hip_error(err, -6, what, e);
 }
 
 }  // namespace
@@ -355,35 +705,17 @@ int check_int8_gemm(const Int8GemmDesc &d, CError *err) {
 
 int launch_int8_gemm(const Int8GemmDesc &d, hipStream_t s, CError *err) {
   if (d.M == 0 || d.N == 0) return 0;
-  Int8Params p{};
-  p.A = d.A;
-  p.as = d.a_scales;
-  p.B = d.B;
-  p.bs = d.b_scales;
-  p.C = d.C;
-  p.bias = d.bias;
-  p.M = d.M, p.N = d.N, p.K = d.K, p.ldc = d.ldc;
-  p.lda = d.M > 1 ? d.lda : 0;
-  p.ldb = d.N > 1 ? d.ldb : 0;
-  p.alpha = d.alpha, p.beta = d.beta, p.act = d.act, p.act_alpha = d.act_alpha;
-  if (d.K == 0) {
+  const Int8Params p = params_of(d);
+  if (d.K == 0)
     hipLaunchKernelGGL(i8_k0_kernel, dim3(grid_of(d.M * d.N, 256)), dim3(256), 0, s, p);
-  } else if (d.M <= 16) {
-    launch_rows<1, 1, 8, 2>(p, s);
-  } else if (d.M <= 64) {
-    launch_rows<4, 1, 8, 1>(p, s);
-  } else if (d.M * d.N >= 256L * 256 * 200) {
-    launch_tiles<2, 4, 8, 4, 2, 2>(p, s);
-  } else {
-    launch_tiles<2, 2, 4, 4, 2, 2>(p, s);
-  }
-  const hipError_t e = hipGetLastError();
-  return e == hipSuccess ? 0 : hip_error(err, -6, "int8 gemm launch", e);
+  else
+    launch_product(p, s);
+  return launched("int8 gemm launch", err);
 }
 
 size_t int8_linear_workspace(long M, long N, long K) {
   size_t n;
-  if (M < 1 || N < 1 || K < 1 || K > kInt8MaxK || !matrix_bytes(M, int8_pitch(K) + 4, 1, &n)) return 0;
+  if (M < 1 || N < 1 || K < 1 || K > kInt8MaxK || few_tokens(M, K) || !matrix_bytes(M, int8_pitch(K) + 4, 1, &n)) return 0;
   return (n + 15) / 16 * 16;
 }
 
@@ -413,6 +745,14 @@ int launch_int8_linear(const Int8LinearDesc &d, hipStream_t s, CError *err) {
   Int8GemmDesc g = d.gemm;
   if (g.M == 0 || g.N == 0) return 0;
   if (g.K == 0) return launch_int8_gemm(g, s, err);
+  if (few_tokens(g.M, g.K)) {
+    const Int8Params p = params_of(g);
+    if (d.dtype == GN_F16)
+      launch_tokens<_Float16>(d, p, s);
+    else
+      launch_tokens<float>(d, p, s);
+    return launched("int8 linear launch", err);
+  }
   const long pitch = int8_pitch(g.K);
   auto *q = static_cast<int8_t *>(d.workspace);
   auto *scales = reinterpret_cast<float *>(q + g.M * pitch);
