@@ -40,9 +40,10 @@ CASES = [
         ("dtype", dict(dtype=FP4)), ("leading", dict(ldx=99)), ("NULL", dict(x=None)), ("aligned", dict(x=P + 2)), ("aligned", dict(cs=P + 2))]),
     ("gn_adjust_logits", ADJUST, [
         ("dtype", dict(dtype=FP4)), ("size", dict(rows=-1)), ("size", dict(cols=0)), ("size", dict(cols=1 << 31, ld=1 << 31, ldo=1 << 31, ldmask=1 << 27)),
-        ("too large", dict(rows=BIG)), ("leading", dict(ld=99)), ("leading", dict(ldo=99)), ("NULL", dict(x=None)), ("NULL", dict(out=None)),
+        ("too large", dict(rows=BIG)), ("too large", dict(rows=1 << 24)), ("too large", dict(rows=1 << 22, h=2048)),
+        ("leading", dict(ld=99)), ("leading", dict(ldo=99)), ("NULL", dict(x=None)), ("NULL", dict(out=None)),
         ("aligned", dict(x=P + 2)), ("aligned", dict(out=P + 2)), ("aligned", dict(dtype=F16, x=P + 1)), ("in place", dict(out=P, ldo=101)),
-        ("history", dict(h=-1)), ("history", dict(h=1 << 30)), ("NULL history", dict(hist=None)), ("history", dict(hist=P + 4)),
+        ("history", dict(h=-1)), ("history", dict(h=1 << 29)), ("NULL history", dict(hist=None)), ("history", dict(hist=P + 4)),
         ("without a history", dict(h=0)), ("aligned", dict(prompt=P + 4)), ("aligned", dict(rep=P + 2)), ("aligned", dict(freq=P + 1)),
         ("aligned", dict(pres=P + 2)), ("biases", dict(nb=-1)), ("biases", dict(nb=1025)), ("NULL biases", dict(bids=None)),
         ("NULL biases", dict(bias=None)), ("aligned", dict(bids=P + 4)), ("aligned", dict(bias=P + 2)), ("words", dict(ldmask=3)),
