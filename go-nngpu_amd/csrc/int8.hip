@@ -13,8 +13,6 @@
 namespace gn {
 namespace {
 
-typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
-
 constexpr long kMaxRows = 1L << 22;  // a workgroup of up to 1024 threads to a row, below 2^32 threads
 
 struct __attribute__((packed, aligned(1))) Unaligned8 {
@@ -58,10 +56,14 @@ __global__ void __launch_bounds__(TX < 256 ? 256 : TX) int8_quantize_kernel(Int8
   auto reduce = [&](long c0) {
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      float y[8];
-      scaled(c0, e, y);
+      if constexpr (SCALED) {
+        float y[8];
+        scaled(c0, e, y);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(y[i]) & 0x7fffffffu);
+        for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(y[i]) & 0x7fffffffu);
+      } else {
+        top = max(top, v[e].top());
+      }
     }
   };
   load(0);
@@ -81,7 +83,6 @@ __global__ void __launch_bounds__(TX < 256 ? 256 : TX) int8_quantize_kernel(Int8
     for (int w = 0; w < W; ++w) top = max(top, tops[w]);
   }
   const float s = int8_scale(top), inv = 1.0f / s;
-  const bool bad = s != s;
   if (tx == 0) p.scales[r] = s;
   int8_t *q = p.q + r * p.ldq;
   auto store = [&](long c0) {
@@ -90,9 +91,7 @@ __global__ void __launch_bounds__(TX < 256 ? 256 : TX) int8_quantize_kernel(Int8
       const long at = c0 + 8L * (e * TX + tx), left = p.cols - at;
       float y[8];
       scaled(c0, e, y);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = bad ? 0.0f : int8_round(y[i], s, inv);
-      const u32x2_t b = {int8_pack(y[0], y[1], y[2], y[3]), int8_pack(y[4], y[5], y[6], y[7])};
+      const u32x2_t b = int8_round8(y, s, inv);
       if (left >= 8) {
         reinterpret_cast<Unaligned8 *>(q + at)->v = b;
       } else {

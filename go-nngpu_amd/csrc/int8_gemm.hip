@@ -24,6 +24,10 @@ __device__ __forceinline__ i32x4_t mfma_i8(i32x4_t a, i32x4_t b, i32x4_t c) {
   return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0);
 }
 
+// Offset v of a copy that begins at k if that is below left, else one out of range. (Without a comparison, whose result
+// would take scalar registers for each of a wave's copies.)
+__device__ __forceinline__ unsigned below(unsigned v, int k, int left) { return v | ((unsigned)(left - 1 - k) & kOutOfRange); }
+
 // The first `n` bytes of v, zeros after them.
 __device__ __forceinline__ i32x4_t first_bytes(i32x4_t v, int n) {
 #pragma unroll
@@ -111,13 +115,15 @@ __device__ __forceinline__ void join_waves(char *smem, const i32x4_t (&acc)[MF][
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();  // no copy is under way
   i32x4_t *part = reinterpret_cast<i32x4_t *>(smem);
+  if (wave < KW) {  // there may be others
 #pragma unroll
-  for (int i = 0; i < MF; ++i)
+    for (int i = 0; i < MF; ++i)
 #pragma unroll
-    for (int j = 0; j < NF; ++j) part[(wave * MF * NF + i * NF + j) * 64 + lane] = acc[i][j];
+      for (int j = 0; j < NF; ++j) part[(wave * MF * NF + i * NF + j) * 64 + lane] = acc[i][j];
+  }
   __syncthreads();
 #pragma unroll 1
-  for (int f = wave; f < MF * NF; f += KW) {
+  for (int f = wave; f < MF * NF; f += blockDim.x / 64) {
     i32x4_t v = part[f * 64 + lane];
 #pragma unroll
     for (int w = 1; w < KW; ++w) v += part[(w * MF * NF + f) * 64 + lane];
@@ -166,10 +172,10 @@ __global__ void __launch_bounds__(KW * 64) i8_stream_kernel(Int8Params p) {
     } else {
 #pragma unroll
       for (int i = 0; i < CB; ++i)
-        dma16_at(db, kb[i] < left ? vb[i] : kOutOfRange, left > 0 ? k : 0, __builtin_amdgcn_readfirstlane(to + (CA + i) * 1024));
+        dma16_at(db, below(vb[i], kb[i], left), left > 0 ? k : 0, __builtin_amdgcn_readfirstlane(to + (CA + i) * 1024));
 #pragma unroll
       for (int i = 0; i < CA; ++i)
-        dma16_at(da, ka[i] < left ? va[i] : kOutOfRange, left > 0 ? k : 0, __builtin_amdgcn_readfirstlane(to + i * 1024));
+        dma16_at(da, below(va[i], ka[i], left), left > 0 ? k : 0, __builtin_amdgcn_readfirstlane(to + i * 1024));
     }
   };
   i32x4_t acc[MF][NF];
@@ -215,60 +221,34 @@ __global__ void __launch_bounds__(KW * 64) i8_stream_kernel(Int8Params p) {
   });
 }
 
-// One token, or a few (up to kFewTokens rows), of activations that the kernel brings to 8 bits itself: each workgroup does so, into LDS,
-// while the first of its weights are on their way. A launch and a wait for it less than with a kernel before it.
-constexpr int kFewTokens = 8;
-constexpr int kTokenBytes = 48 * 1024;  // of LDS for the rows
+// Few rows of activations that the kernel brings to 8 bits itself, into LDS: a launch and a wait for it less than with a kernel before
+// it. QW waves do that while the first weights of the KW others are on their way (a wave's own wait for the rows would be
+// one for its weights too).
 __host__ __device__ inline int token_pitch(long K) { return (int)((K + 127) / 128 * 128 + 16); }  // rows on distinct banks
-template <typename T, int NF, int KW, int NS>
-__global__ void __launch_bounds__(KW * 64) i8_token_kernel(Int8Params p, const T *x, long ldx, const float *col_scale) {
+template <typename T, int NF, int KW, int NS, int QW>
+__global__ void __launch_bounds__((KW + QW) * 64) i8_token_kernel(Int8Params p, const T *x, long ldx, const float *col_scale) {
   using C = Chunk<128>;
-  constexpr int CB = 16 * NF / C::RPC, SLOT = CB * 1024, HOLD = 4;
+  constexpr int CB = 16 * NF / C::RPC, SLOT = CB * 1024;
   constexpr int RING = KW * NS * SLOT, PART = KW * NF * 1024;
-  static_assert((NS - 1) * CB < 64, "copies");
-  __shared__ uint32_t tops[KW];
-  __shared__ float scales[kFewTokens];
+  static_assert((NS - 1) * CB < 64 && RING >= PART, "copies");
+  __shared__ uint32_t tops[QW];
+  __shared__ float scales[16];
   extern __shared__ __attribute__((aligned(1024))) char smem[];  // the slots, in the end the partial sums; the rows in 8 bits
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-  const int M = (int)p.M, K = (int)p.K, pitch = token_pitch(K);
-  char *rows = smem + (RING > PART ? RING : PART);
-  // Waves to a row, and this wave's part of its row: chunks of 8 values, a lane each.
-  const int lr = M <= 1 ? 0 : M <= 2 ? 1 : M <= 4 ? 2 : 3, per = KW >> lr, mine = wave / per, part = wave % per;
-  const T *row = x + (long)min(mine, M - 1) * ldx;
-  auto value = [&](const Eight<T> &v, const Eight<float> &c, int i) { return col_scale ? v[i] * c[i] : v[i]; };
-  Eight<T> v[HOLD];
-  Eight<float> c[HOLD];
-#pragma unroll
-  for (int e = 0; e < HOLD; ++e) {
-    const int at = 8 * ((e * per + part) * 64 + lane);
-    v[e].load(row + at, K - at);
-    if (col_scale) c[e].load(col_scale + at, K - at);
-  }
-  uint32_t top = 0;
-  auto reduce = [&](const Eight<T> &a, const Eight<float> &b) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(value(a, b, i)) & 0x7fffffffu);
-  };
-#pragma unroll
-  for (int e = 0; e < HOLD; ++e) reduce(v[e], c[e]);
-  for (int at = 8 * ((HOLD * per + part) * 64 + lane); at < K; at += 8 * per * 64) {
-    Eight<T> a;
-    Eight<float> b;
-    a.load(row + at, K - at);
-    if (col_scale) b.load(col_scale + at, K - at);
-    reduce(a, b);
-  }
+  const int M = (int)p.M, K = (int)p.K, pitch = token_pitch(K), end = pitch - 16;
+  char *rows = smem + RING;
+  // Waves to a row, and the rows gone through side by side.
+  int per = QW, side = 1;
+  while (side < M && per > 1) per >>= 1, side <<= 1;
 
-  // The row has been read: the weights' first steps on their way. (Before, the wait for the row would be one for them too.)
-  const long n0 = (long)blockIdx.x * 16 * NF;
-  const BufRsrc db = make_rsrc(static_cast<const char *>(p.B) + n0 * p.ldb);
   unsigned vb[CB];
   int kb[CB];
+  const BufRsrc db = make_rsrc(static_cast<const char *>(p.B) + (long)blockIdx.x * 16 * NF * p.ldb);
 #pragma unroll
   for (int i = 0; i < CB; ++i) {
     const int br = C::RPC * i + C::row(lane);
     kb[i] = 16 * C::octet(br, lane);
-    vb[i] = n0 + br < p.N ? (unsigned)(br * p.ldb) + kb[i] : kOutOfRange;
+    vb[i] = (long)blockIdx.x * 16 * NF + br < p.N ? (unsigned)(br * p.ldb) + kb[i] : kOutOfRange;
   }
   const unsigned lds = lds_offset(smem) + wave * NS * SLOT;
   auto issue = [&](int t, int slot) {  // of the wave's steps; past K all reads are zeros
@@ -280,49 +260,68 @@ __global__ void __launch_bounds__(KW * 64) i8_token_kernel(Int8Params p, const T
     } else {
 #pragma unroll
       for (int i = 0; i < CB; ++i)
-        dma16_at(db, kb[i] < left ? vb[i] : kOutOfRange, left > 0 ? k : 0, __builtin_amdgcn_readfirstlane(to + i * 1024));
+        dma16_at(db, below(vb[i], kb[i], left), left > 0 ? k : 0, __builtin_amdgcn_readfirstlane(to + i * 1024));
     }
   };
-  __builtin_amdgcn_sched_barrier(0);
+  const int part = (wave - KW) % per, first = (wave - KW) / per;
+  // The values from `at` on times their columns' factors, zeros past the row.
+  auto load = [&](int m, int at, float (&y)[8]) {
+    Eight<T> v;
+    v.load(x + m * ldx + at, K - at);
+    if (col_scale) {
+      Eight<float> c;
+      c.load(col_scale + at, K - at);
 #pragma unroll
-  for (int t = 0; t < NS; ++t) issue(t, t);
-  __builtin_amdgcn_sched_barrier(0);
-
+      for (int i = 0; i < 8; ++i) y[i] = v[i] * c[i];
+    } else {
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
-  if (lane == 0) tops[wave] = top;
-  lds_barrier();
-  for (int w = 0; w < per; ++w) top = max(top, tops[mine * per + w]);
-  const float s = int8_scale(top), inv = 1.0f / s;
-  const bool bad = s != s;
-  if (mine < M) {
-    if (part == 0 && lane == 0) scales[mine] = s;
-    auto store = [&](const Eight<T> &a, const Eight<float> &b, int at) {
+      for (int i = 0; i < 8; ++i) y[i] = v[i];
+    }
+  };
+  auto top_of = [&](int m) {
+    uint32_t top = 0;
+#pragma unroll 1
+    for (int at = 8 * (part * 64 + lane); at < K; at += 8 * per * 64) {
       float y[8];
+      load(m, at, y);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = bad ? 0.0f : int8_round(value(a, b, i), s, inv);
-      *reinterpret_cast<u32x2_t *>(rows + mine * pitch + at) = u32x2_t{int8_pack(y[0], y[1], y[2], y[3]), int8_pack(y[4], y[5], y[6], y[7])};
-    };
-    const int end = pitch - 16;  // zeros from K on
+      for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(y[i]) & 0x7fffffffu);
+    }
 #pragma unroll
-    for (int e = 0; e < HOLD; ++e) {
-      const int at = 8 * ((e * per + part) * 64 + lane);
-      if (at < end) store(v[e], c[e], at);
+    for (int o = 32; o > 0; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
+    return top;
+  };
+  auto quantize = [&](int m, uint32_t top) {
+    const float s = int8_scale(top), inv = 1.0f / s;
+    if (part == 0 && lane == 0) scales[m] = s;
+#pragma unroll 1
+    for (int at = 8 * (part * 64 + lane); at < end; at += 8 * per * 64) {  // zeros from K on
+      float y[8];
+      load(m, at, y);
+      *reinterpret_cast<u32x2_t *>(rows + m * pitch + at) = int8_round8(y, s, inv);
     }
-    for (int at = 8 * ((HOLD * per + part) * 64 + lane); at < end; at += 8 * per * 64) {
-      Eight<T> a;
-      Eight<float> b;
-      a.load(row + at, K - at);
-      if (col_scale) b.load(col_scale + at, K - at);
-      store(a, b, at);
+  };
+  if (wave < KW) {
+#pragma unroll 1
+    for (int t = 0; t < NS; ++t) issue(t, t);
+    if (per > 1) lds_barrier();
+  } else if (per > 1) {
+    uint32_t top = first < M ? top_of(first) : 0;
+    if (lane == 0) tops[wave - KW] = top;
+    lds_barrier();
+    if (first < M) {
+      for (int w = 0; w < per; ++w) top = max(top, tops[first * per + w]);
+      quantize(first, top);
     }
+  } else {
+    for (int m = first; m < M; m += QW) quantize(m, top_of(m));
   }
   lds_barrier();
 
   i32x4_t acc[1][NF];
 #pragma unroll
   for (int j = 0; j < NF; ++j) acc[0][j] = i32x4_t{0, 0, 0, 0};
-  const int steps = (K + 127) / 128, count = wave < steps ? (steps - wave + KW - 1) / KW : 0;
+  const int steps = (K + 127) / 128, count = wave < min(steps, KW) ? (steps - wave + KW - 1) / KW : 0;
   const char *arow = rows + min(r, M - 1) * pitch + 16 * g;
   int slot = 0;
   for (int t = 0; t < count; ++t) {
@@ -343,8 +342,12 @@ __global__ void __launch_bounds__(KW * 64) i8_token_kernel(Int8Params p, const T
       for (int j = 0; j < NF; ++j) acc[0][j] = mfma_i8(b[h][j], a[h], acc[0][j]);
     slot = slot + 1 == NS ? 0 : slot + 1;
   }
+  // What only the end needs of the arguments is read again: kept through the quantisation it takes scalar registers that it has not.
+  auto *args = (const CONST_AS Int8Params *)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(args));
+  const Int8Params q = *(const Int8Params *)args;
   join_waves<1, NF, KW>(smem, acc, wave, lane, [&](int, int j, i32x4_t v) {
-    if (r < M) finish4(p, v, p.alpha * scales[r], r, n0 + 16 * j + 4 * g);
+    if (r < (int)q.M) finish4(q, v, q.alpha * scales[r], r, (long)blockIdx.x * 16 * NF + 16 * j + 4 * g);
   });
 }
 
@@ -417,7 +420,7 @@ i8_tile_kernel(Int8Params p) {
       for (int i = 0; i < count; ++i) dma16(d, v[i], __builtin_amdgcn_readfirstlane(to + i * 1024));
     } else {
 #pragma unroll
-      for (int i = 0; i < count; ++i) dma16(d, k_of(k, i) < left ? v[i] : kOutOfRange, __builtin_amdgcn_readfirstlane(to + i * 1024));
+      for (int i = 0; i < count; ++i) dma16(d, below(v[i], k_of(k, i), left), __builtin_amdgcn_readfirstlane(to + i * 1024));
     }
   };
   auto issue_a = [&](int t, int slot) { issue(a0, va, ka, CA, t, lds + slot * STAGE + wave * CA * 1024); };
@@ -640,17 +643,26 @@ void launch_product(const Int8Params &p, hipStream_t s) {
   }
 }
 
-// Few tokens' activations, brought to 8 bits in the product's kernel.
-bool few_tokens(long M, long K) { return M <= kFewTokens && M * token_pitch(K) <= kTokenBytes; }
-template <typename T, int NF, int KW, int NS>
+// Up to 4 rows of activations are brought to 8 bits in the product's kernel. Against a kernel before it, us of kernels: 1 row 1000 ->
+// 1000 4.5 / 5.9, 4096 -> 4096 7.4 / 8.8, 11008 -> 4096 12.9 / 15.3, 4096 -> 11008 11.7 / 12.8; 4 rows 9.7 / 9.0 and 13.8 / 13.1, where
+// the other's second launch costs a caller without a graph 3 us more. The rows stand beside up to 128 KiB of slots in LDS.
+bool few_tokens(long M, long K) { return M <= 4 && M * token_pitch(K) <= 24 * 1024; }
+template <typename T, int NF, int KW, int NS, int QW>
 void launch_token(const Int8LinearDesc &d, const Int8Params &p, hipStream_t s) {
-  const int ring = KW * NF * 1024 * std::max(1, 2 * NS);
-  hipLaunchKernelGGL((i8_token_kernel<T, NF, KW, NS>), dim3((unsigned)((p.N + 16 * NF - 1) / (16 * NF))), dim3(KW * 64),
+  const int ring = KW * NF * NS * 2048;
+  hipLaunchKernelGGL((i8_token_kernel<T, NF, KW, NS, QW>), dim3((unsigned)((p.N + 16 * NF - 1) / (16 * NF))), dim3((KW + QW) * 64),
                      ring + (int)p.M * token_pitch(p.K), s, p, static_cast<const T *>(d.x), d.gemm.M > 1 ? d.ldx : 0, d.col_scale);
 }
 template <typename T>
 void launch_tokens(const Int8LinearDesc &d, const Int8Params &p, hipStream_t s) {
-  launch_token<T, 1, 8, 2>(d, p, s);
+  // As few columns to a workgroup as leave no CU a second one: 1 row 4096 -> 4096 7.4 us with 16, 7.9 with 32, 9.2 with 64 columns;
+  // 4096 -> 11008 16.4, 15.5 and 11.7.
+  if (p.N <= 16 * 256)
+    launch_token<T, 1, 8, 2, 8>(d, p, s);
+  else if (p.N <= 32 * 256)
+    launch_token<T, 2, 8, 2, 8>(d, p, s);
+  else
+    launch_token<T, 4, 8, 2, 8>(d, p, s);
 }
 
 Int8Params params_of(const Int8GemmDesc &d) {
