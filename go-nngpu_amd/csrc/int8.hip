@@ -31,47 +31,40 @@ __global__ void __launch_bounds__(TX < 256 ? 256 : TX) int8_quantize_kernel(Int8
   const long r = (long)blockIdx.x * RPW + (TX < 256 ? threadIdx.x / TX : 0);
   if (r >= p.rows) return;  // whole waves, and only where rows have no barrier
   const T *x = static_cast<const T *>(p.x) + r * p.ldx;
-  Eight<T> v[E];
+  // Values in their own type, or (SCALED) times their columns' factors; zeros past the row.
+  using Kept = std::conditional_t<SCALED, Eight<float>, Eight<T>>;
+  Kept v[E];
+  auto place = [&](long c0, int e) { return c0 + 8L * (e * TX + tx); };
   auto load = [&](long c0) {
+    Eight<T> raw[SCALED ? E : 1];
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const long at = c0 + 8L * (e * TX + tx);
-      v[e].load(x + at, p.cols - at);
+      const long at = place(c0, e);
+      if constexpr (SCALED) {
+        raw[e].load(x + at, p.cols - at);
+        v[e].load(p.col_scale + at, p.cols - at);
+      } else {
+        v[e].load(x + at, p.cols - at);
+      }
     }
-  };
-  // Value i of part e times its column's factor; the factors past the row meet zeros.
-  auto scaled = [&](long c0, int e, float y[8]) {
-    const long at = c0 + 8L * (e * TX + tx);
     if constexpr (SCALED) {
-      Eight<float> c;
-      c.load(p.col_scale + at, p.cols - at);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = v[e][i] * c[i];
-    } else {
+      for (int e = 0; e < E; ++e)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = v[e][i];
+        for (int i = 0; i < 8; ++i) v[e].v[i / 4][i % 4] = __float_as_uint(raw[e][i] * v[e][i]);
     }
   };
   uint32_t top = 0;
-  auto reduce = [&](long c0) {
+  auto reduce = [&] {
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      if constexpr (SCALED) {
-        float y[8];
-        scaled(c0, e, y);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(y[i]) & 0x7fffffffu);
-      } else {
-        top = max(top, v[e].top());
-      }
-    }
+    for (int e = 0; e < E; ++e) top = max(top, v[e].top());
   };
   load(0);
-  reduce(0);
+  reduce();
   if constexpr (LOOP) {
     for (long c0 = 8L * TX * E; c0 < p.cols; c0 += 8L * TX * E) {
       load(c0);
-      reduce(c0);
+      reduce();
     }
   }
 #pragma unroll
@@ -88,9 +81,10 @@ __global__ void __launch_bounds__(TX < 256 ? 256 : TX) int8_quantize_kernel(Int8
   auto store = [&](long c0) {
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const long at = c0 + 8L * (e * TX + tx), left = p.cols - at;
+      const long at = place(c0, e), left = p.cols - at;
       float y[8];
-      scaled(c0, e, y);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = v[e][i];
       const u32x2_t b = int8_round8(y, s, inv);
       if (left >= 8) {
         reinterpret_cast<Unaligned8 *>(q + at)->v = b;
@@ -213,6 +207,9 @@ void launch_rows(const Int8QuantizeDesc &d, hipStream_t s) {
                        dim3((unsigned)((d.rows * TX + NT - 1) / NT)), dim3(NT), 0, s, d);
   };
   using std::integral_constant;
+  // As few threads as take the row at once with little left over. Measured, us: 4096 rows of 1000 fp32 a wave 5.6, 256 threads 7.1; 512 of 4096
+  // fp16 256 x 16 values 3.7, 256 x 32 4.7, 1024 x 8 4.3; 11008 of 4096 23, 29 and 48 (5.9 TB/s); 8192 of 8192 256 x 32 37, 512 x 16 37, 1024 x 8
+  // 44; 512 of 11008 fp32 with factors 512 x 32 7.7, 1024 x 16 7.7, 1024 x 32 12.
   if (d.cols <= 512)
     go(integral_constant<int, 64>{}, integral_constant<int, 1>{}, std::false_type{});
   else if (d.cols <= 1024)
@@ -222,7 +219,9 @@ void launch_rows(const Int8QuantizeDesc &d, hipStream_t s) {
   else if (d.cols <= 4096)
     go(integral_constant<int, 256>{}, integral_constant<int, 2>{}, std::false_type{});
   else if (d.cols <= 8192)
-    go(integral_constant<int, 256>{}, integral_constant<int, 4>{}, std::false_type{});
+    go(integral_constant<int, 512>{}, integral_constant<int, 2>{}, std::false_type{});
+  else if (d.cols <= 16384)
+    go(integral_constant<int, 512>{}, integral_constant<int, 4>{}, std::false_type{});
   else if (d.cols <= 32768)
     go(integral_constant<int, 1024>{}, integral_constant<int, 4>{}, std::false_type{});
   else

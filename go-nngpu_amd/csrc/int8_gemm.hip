@@ -364,13 +364,14 @@ struct I8Tile {
   static constexpr int EPI = SUMS + (BM + 2 * BN) * 4;                                                 // with the scales and the bias
   static constexpr int BYTES = NS * STAGE > EPI ? NS * STAGE : EPI;
 };
-template <int WM, int WN, int FM, int FN, int NS, int WPE>
-__global__ void __launch_bounds__(WM * WN * 64) __attribute__((amdgpu_waves_per_eu(WPE, WPE)))
+template <int WM, int WN, int FM, int FN, int NS>
+__global__ void __launch_bounds__(WM * WN * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 i8_tile_kernel(Int8Params p) {
   using Tile = I8Tile<WM, WN, FM, FN, NS>;
+  using C = Chunk<128>;
   constexpr int NW = WM * WN, NT = NW * 64, BM = Tile::BM, BN = Tile::BN, STAGE = Tile::STAGE;
-  constexpr int CA = BM / 8 / NW, CB = BN / 8 / NW, CPW = CA + CB;
-  static_assert(CA * NW * 8 == BM && CB * NW * 8 == BN, "chunks");
+  constexpr int CA = BM / C::RPC / NW, CB = BN / C::RPC / NW, CPW = CA + CB;
+  static_assert(CA * NW * C::RPC == BM && CB * NW * C::RPC == BN, "chunks");
   static_assert((NS - 1) * CPW < 64 && NS >= 2 && FM % Tile::PARTS == 0 && NT >= BN / 4, "copies and rows");
   __shared__ __attribute__((aligned(1024))) char smem[Tile::BYTES];
 
@@ -398,33 +399,29 @@ i8_tile_kernel(Int8Params p) {
   const char *a0 = static_cast<const char *>(p.A) + m0 * p.lda, *b0 = static_cast<const char *>(p.B) + n0 * p.ldb;
   unsigned va[CA], vb[CB];
   // A copy's first k in the stage, for even i; for odd i the octet's upper bit is the other way round (row >> 1 is 4 more).
-  const int ka = 16 * kc8_octet(8 * wave * CA + (lane >> 3), lane & 7), kb = 16 * kc8_octet(8 * wave * CB + (lane >> 3), lane & 7);
+  const int ka = 16 * C::octet(C::RPC * wave * CA + C::row(lane), lane), kb = 16 * C::octet(C::RPC * wave * CB + C::row(lane), lane);
   auto k_of = [](int k, int i) { return k ^ (i & 1 ? 64 : 0); };
 #pragma unroll
   for (int i = 0; i < CA; ++i) {
-    const int row = 8 * (wave * CA + i) + (lane >> 3);
+    const int row = C::RPC * (wave * CA + i) + C::row(lane);
     va[i] = m0 + row < p.M ? (unsigned)(row * p.lda) + k_of(ka, i) : kOutOfRange;
   }
 #pragma unroll
   for (int i = 0; i < CB; ++i) {
-    const int row = 8 * (wave * CB + i) + (lane >> 3);
+    const int row = C::RPC * (wave * CB + i) + C::row(lane);
     vb[i] = n0 + row < p.N ? (unsigned)(row * p.ldb) + k_of(kb, i) : kOutOfRange;
   }
   const unsigned lds = lds_offset(smem);
-  // Copies of a stage; chunks that begin at or past K read zeros.
-  auto issue = [&](const char *base, const unsigned *v, int k, int count, int t, unsigned to) {
+  // Part q of `parts` of a side's copies of stage t into a slot; chunks that begin at or past K read zeros.
+  auto issue = [&](const char *base, const unsigned *v, int k, int count, int t, unsigned to, int q, int parts) {
     const int left = (int)p.K - 128 * t;
     const BufRsrc d = make_rsrc(base + 128L * t);
-    if (left >= 128) {
 #pragma unroll
-      for (int i = 0; i < count; ++i) dma16(d, v[i], __builtin_amdgcn_readfirstlane(to + i * 1024));
-    } else {
-#pragma unroll
-      for (int i = 0; i < count; ++i) dma16(d, below(v[i], k_of(k, i), left), __builtin_amdgcn_readfirstlane(to + i * 1024));
-    }
+    for (int i = 0; i < count; ++i)
+      if (i * parts / count == q) dma16(d, below(v[i], k_of(k, i), left), __builtin_amdgcn_readfirstlane(to + i * 1024));
   };
-  auto issue_a = [&](int t, int slot) { issue(a0, va, ka, CA, t, lds + slot * STAGE + wave * CA * 1024); };
-  auto issue_b = [&](int t, int slot) { issue(b0, vb, kb, CB, t, lds + slot * STAGE + BM * 128 + wave * CB * 1024); };
+  auto issue_a = [&](int t, int slot, int q, int parts) { issue(a0, va, ka, CA, t, lds + slot * STAGE + wave * CA * 1024, q, parts); };
+  auto issue_b = [&](int t, int slot, int q, int parts) { issue(b0, vb, kb, CB, t, lds + slot * STAGE + BM * 128 + wave * CB * 1024, q, parts); };
   // This wave's chunks of A of the last stage, once they have landed (all that is under way behind them reads zeros).
   auto clear_tail = [&](int slot) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -440,13 +437,12 @@ i8_tile_kernel(Int8Params p) {
   };
 
   i32x4_t fa[2][FM], fb[2][FN];
+  // Of the half h of a stage's k.
   auto read_a = [&](int slot, int h, int i) {
-    const int row = (wm * FM + i) * 16 + r;
-    fa[h][i] = *reinterpret_cast<const i32x4_t *>(smem + slot * STAGE + (row >> 3) * 1024 + 16 * kc8_slot(row, 4 * h + g));
+    fa[h][i] = *reinterpret_cast<const i32x4_t *>(smem + slot * STAGE + C::place((wm * FM + i) * 16 + r, 4 * h + g));
   };
   auto read_b = [&](int slot, int h, int j) {
-    const int row = (wn * FN + j) * 16 + r;
-    fb[h][j] = *reinterpret_cast<const i32x4_t *>(smem + slot * STAGE + BM * 128 + (row >> 3) * 1024 + 16 * kc8_slot(row, 4 * h + g));
+    fb[h][j] = *reinterpret_cast<const i32x4_t *>(smem + slot * STAGE + BM * 128 + C::place((wn * FN + j) * 16 + r, 4 * h + g));
   };
   auto read_part = [&](int slot, int h, int q, int parts) {
 #pragma unroll
@@ -469,51 +465,70 @@ i8_tile_kernel(Int8Params p) {
   };
 
   const bool tail = p.K % 16 != 0;
+  // With two slots B's first copies are all before the loop, with more the last of them are in it.
+  constexpr bool SPREAD = NS > 2;
 #pragma unroll 1
   for (int t = 0; t < NS; ++t) {
-    issue_a(t, t);
-    issue_b(t, t);
+    issue_a(t, t, 0, 1);
+    if (!SPREAD || t < NS - 1) issue_b(t, t, 0, 1);
   }
-  __builtin_amdgcn_s_waitcnt(vmcnt_imm((NS - 1) * CPW));
+  __builtin_amdgcn_s_waitcnt(vmcnt_imm(SPREAD ? (NS - 2) * CPW + CA : (NS - 1) * CPW));
   if (tail && ns == 1) clear_tail(0);
   __syncthreads();
   read_part(0, 0, 0, 1);
-  int cur = 0;
+  int cur = 0, prev = NS - 1;
   for (int t = 0; t < ns; ++t) {
     const int nxt = cur + 1 == NS ? 0 : cur + 1;
-    __builtin_amdgcn_sched_barrier(0);
-    read_part(cur, 1, 0, 1);
-    mfma_rows(0, 0, FM);
-    sched_interleave<FM * FN, FM + FN>();
-    __builtin_amdgcn_sched_barrier(0);
-    __builtin_amdgcn_s_waitcnt(vmcnt_imm((NS - 2) * CPW));
-    if (tail && t + 2 == ns) clear_tail(nxt);
-    __syncthreads();
-    __builtin_amdgcn_sched_barrier(0);
-    if constexpr (FM >= 8) {
-      // The copies in two bursts, each once the matrix instructions have work.
+    auto arrive = [&] {  // stage t + 1 is there, in all waves
+      __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_s_waitcnt(vmcnt_imm((NS - 2) * CPW));
+      if (tail && t + 2 == ns) clear_tail(nxt);
+      __syncthreads();
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    if constexpr (SPREAD) {
+      // A step's products, row by row, with the next step's fragments and a share of the copies behind each row: a copy takes the
+      // address unit 20 cycles, and a wave that meets a full one waits there with all that it has behind it. B's copies of a stage wait
+      // for the step after A's. (All copies after the barrier, 512 rows 11008 -> 4096: 128 x 256 tiles 68 us instead of 57, 128 x 192 54.6 /
+      // 50.5, 128 x 128 42 / 41.)
+      auto step = [&](int h, int read_slot, auto copies) {
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < FM; ++i) {
+          mfma_rows(h, i, i + 1);
+          read_part(read_slot, 1 - h, i, FM);
+          __builtin_amdgcn_sched_barrier(0);
+          copies(i);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      };
+      step(0, cur, [&](int i) { issue_b(t + NS - 1, prev, i, FM); });
+      arrive();
+      step(1, nxt, [&](int i) { issue_a(t + NS, cur, i, FM); });
+    } else {
+      // Two slots leave no step to spread the copies over: in two bursts, each once the matrix instructions have work (8192^3 440 us; row
+      // by row 472; four slots of half a stage, with a barrier to each, 484).
       constexpr int R0 = FM / 2, NR = FM / 2 + FN / 2;
+      __builtin_amdgcn_sched_barrier(0);
+      read_part(cur, 1, 0, 1);
+      mfma_rows(0, 0, FM);
+      sched_interleave<FM * FN, FM + FN>();
+      arrive();
       mfma_rows(1, 0, 1);
       __builtin_amdgcn_sched_barrier(0);
-      issue_a(t + NS, cur);
+      issue_a(t + NS, cur, 0, 1);
       read_part(nxt, 0, 0, 2);
       mfma_rows(1, 1, R0);
       sched_interleave<(R0 - 1) * FN, NR>();
       __builtin_amdgcn_sched_barrier(0);
       mfma_rows(1, R0, R0 + 1);
       __builtin_amdgcn_sched_barrier(0);
-      issue_b(t + NS, cur);
+      issue_b(t + NS, cur, 0, 1);
       read_part(nxt, 0, 1, 2);
       mfma_rows(1, R0 + 1, FM);
       sched_interleave<(FM - R0 - 1) * FN, NR>();
-    } else {
-      issue_a(t + NS, cur);
-      issue_b(t + NS, cur);
-      read_part(nxt, 0, 0, 1);
-      mfma_rows(1, 0, FM);
-      sched_interleave<FM * FN, FM + FN>();
     }
-    cur = nxt;
+    prev = cur, cur = nxt;
   }
   __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
   __syncthreads();  // no copy is under way and all waves are done with the stages: the sums take their place
@@ -601,45 +616,53 @@ void launch_stream(Int8Params p, hipStream_t s) {
   hipLaunchKernelGGL((i8_stream_kernel<MF, NF, KW, S, NS>), dim3((unsigned)(p.tiles_m * p.tiles_n)), dim3(KW * 64), 0, s, p);
 }
 
-template <int WM, int WN, int FM, int FN, int NS, int WPE>
+template <int WM, int WN, int FM, int FN, int NS>
 void launch_tiles(Int8Params p, hipStream_t s) {
   constexpr int BM = WM * FM * 16, BN = WN * FN * 16;
   p.tiles_m = (int)((p.M + BM - 1) / BM);
   p.tiles_n = (int)((p.N + BN - 1) / BN);
-  hipLaunchKernelGGL((i8_tile_kernel<WM, WN, FM, FN, NS, WPE>), dim3((unsigned)(p.tiles_m * p.tiles_n)), dim3(WM * WN * 64), 0, s, p);
+  hipLaunchKernelGGL((i8_tile_kernel<WM, WN, FM, FN, NS>), dim3((unsigned)(p.tiles_m * p.tiles_n)), dim3(WM * WN * 64), 0, s, p);
 }
 
-// The kind of tile with which a CU's share takes the least time, the first of equals. Of a tile alone on a CU: fixed, in 10 ns, and
-// for each 128 of K; more: for each further tile of its share.
+// The kind of tile with which the busiest CU's share takes the least time, the first of equals. In 10 ns: fixed, and `stage` for each
+// 128 of K, for a tile alone on a CU; `next`, and `more` for each 128 of K, for each further tile of its share. Fitted to
+// these kinds' times on 23 sizes from 64 to 8192 rows and 100 to 11008 columns and K; of those the choice takes 0.7% more than the best kind
+// of each, at most 8% (32 rows 4096 -> 11008). Measured, us, 16 x 16 / 16 x 64 / 32 x 32 / 32 x 64 / 64 x 64 (8 waves) / 64 x 64 (4) / 64 x 128
+// (8) / 64 x 128 (4) / 128 x 128 / 128 x 192 / 128 x 256 / 256 x 256: 4096 -> 4096, 64 rows 11.2 / 7.9 / 7.4 / 9.2 / 10.2 / 11.3 / 13.7 / 15.0 /
+// 17.5 / 22.0 / 26.3 / 39.9, 256 rows 34.9 / 25.2 / 22.3 / 16.4 / 11.4 / 11.6 / 14.0 / 15.4 / 18.2 / 23.2 / 27.2 / 43.7, 2048 rows 308 / 197 /
+// 205 / 131 / 73.5 / 61.2 / 56.1 / 46.7 / 45.3 / 49.4 / 37.2 / 44.4; 512 rows 4096 -> 11008 166 / 139 / 112 / 77 / 54.0 / 44.7 / 41.8 / 38.0 / 38.5 /
+// 27.5 / 30.6 / 44.5, 11008 -> 4096 189 / 103 / 90 / 73 / 46.0 / 40.8 / 35.2 / 37.0 / 40.2 / 51.2 / 62.0 / 101.
 struct TileCost {
-  int bm, bn, fixed, alone, more;
+  unsigned bm, bn, fixed, stage, next, more;
 };
-// Measured, us: 4096 -> 11008 ...
-constexpr TileCost kTiles[] = {{16, 16, 250, 7, 7},    {16, 64, 250, 20, 19},  {32, 16, 250, 13, 14},  {32, 32, 250, 16, 17},
-                               {32, 64, 250, 28, 19},  {64, 64, 250, 33, 20},  {64, 128, 250, 40, 33}, {128, 128, 300, 65, 60},
-                               {128, 192, 350, 80, 72}, {128, 256, 400, 100, 90}, {256, 256, 1000, 125, 180}};
+constexpr TileCost kTiles[] = {{16, 16, 329, 4, 97, 4},        {16, 64, 423, 11, 274, 10},     {32, 32, 404, 9, 252, 9},
+                               {32, 64, 369, 18, 251, 16},     {64, 64, 356, 22, 225, 22},     {64, 64, 369, 24, 132, 18},
+                               {64, 128, 398, 32, 299, 36},    {64, 128, 441, 34, 194, 29},    {128, 128, 555, 41, 452, 56},
+                               {128, 192, 658, 54, 779, 67},   {128, 256, 689, 68, 835, 90},   {256, 256, 1084, 119, 1645, 162}};
+constexpr int kKinds = sizeof(kTiles) / sizeof(kTiles[0]);
 void launch_product(const Int8Params &p, hipStream_t s) {
-  const long stages = (p.K + 127) / 128;
+  const unsigned stages = (unsigned)(p.K + 127) / 128, M = (unsigned)p.M, N = (unsigned)p.N;
   int best = 0;
-  long least = 0;
-  for (int i = 0; i < (int)(sizeof(kTiles) / sizeof(kTiles[0])); ++i) {
+  uint64_t least = 0;
+  for (int i = 0; i < kKinds; ++i) {
     const TileCost &k = kTiles[i];
-    const long tiles = ((p.M + k.bm - 1) / k.bm) * ((p.N + k.bn - 1) / k.bn), share = (tiles + 255) / 256;  // 256 CUs
-    const long cost = k.fixed + stages * (k.alone + (share - 1) * k.more);
+    const uint64_t tiles = (uint64_t)((M + k.bm - 1) / k.bm) * ((N + k.bn - 1) / k.bn), others = (tiles - 1) / 256;  // 256 CUs
+    const uint64_t cost = k.fixed + stages * k.stage + others * (k.next + stages * k.more);
     if (i == 0 || cost < least) best = i, least = cost;
   }
   switch (best) {
     case 0: return launch_stream<1, 1, 4, 128, 4>(p, s);
     case 1: return launch_stream<1, 4, 8, 128, 2>(p, s);
-    case 2: return launch_stream<2, 1, 8, 128, 2>(p, s);
-    case 3: return launch_stream<2, 2, 8, 128, 2>(p, s);
-    case 4: return launch_stream<2, 4, 8, 64, 2>(p, s);
-    case 5: return launch_tiles<2, 2, 2, 2, 4, 2>(p, s);
-    case 6: return launch_tiles<2, 2, 2, 4, 3, 2>(p, s);
-    case 7: return launch_tiles<2, 4, 4, 2, 3, 2>(p, s);
-    case 8: return launch_tiles<2, 4, 4, 3, 3, 2>(p, s);
-    case 9: return launch_tiles<2, 4, 4, 4, 3, 2>(p, s);
-    default: return launch_tiles<2, 4, 8, 4, 2, 2>(p, s);
+    case 2: return launch_stream<2, 2, 8, 128, 2>(p, s);
+    case 3: return launch_stream<2, 4, 8, 64, 2>(p, s);
+    case 4: return launch_tiles<2, 4, 2, 1, 4>(p, s);
+    case 5: return launch_tiles<2, 2, 2, 2, 4>(p, s);
+    case 6: return launch_tiles<2, 4, 2, 2, 3>(p, s);
+    case 7: return launch_tiles<2, 2, 2, 4, 3>(p, s);
+    case 8: return launch_tiles<2, 4, 4, 2, 3>(p, s);
+    case 9: return launch_tiles<2, 4, 4, 3, 3>(p, s);
+    case 10: return launch_tiles<2, 4, 4, 4, 3>(p, s);
+    default: return launch_tiles<2, 4, 8, 4, 2>(p, s);
   }
 }
 

@@ -284,8 +284,7 @@ def _current_stream(device=None):
     """Handle of torch's current stream (on the current device). Building torch's Stream object for it takes 2.7 us, a
     third of what a small call costs the host; asking for the handle takes 0.4 us. The function for
     that is not part of torch's public interface: without it, the Stream object is built."""
-    import torch
-
+    torch = _types()
     try:
         raw = torch._C._cuda_getCurrentRawStream
     except AttributeError:
