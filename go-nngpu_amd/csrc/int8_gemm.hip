@@ -382,17 +382,20 @@ i8_tile_kernel(Int8Params p) {
   const int wm = wave / WN, wn = wave % WN, r = lane & 15, g = lane >> 4;
   const int ns = (int)((p.K + 127) / 128);
 
-  // The tile's scales: A's, then B's, thread by thread; in LDS once the stages are done with it.
-  constexpr int SPT = (BM + BN + NT - 1) / NT;
-  float scale[SPT];
+  // What the epilogue needs of each row and column: the rows' scales, the columns' scales and biases, thread by thread; not
+  // touched, which would be a wait for them, until the stages are done with LDS.
+  constexpr int LINES = BM + 2 * BN, SPT = (LINES + NT - 1) / NT;
+  float line[SPT];
 #pragma unroll
   for (int i = 0; i < SPT; ++i) {
     const int at = threadIdx.x + i * NT;
-    scale[i] = 1.0f;
+    line[i] = at < BM + BN ? 1.0f : 0.0f;
     if (at < BM) {
-      scale[i] = p.alpha * (p.as && m0 + at < p.M ? p.as[m0 + at] : 1.0f);
+      if (p.as && m0 + at < p.M) line[i] = p.as[m0 + at];
     } else if (at < BM + BN) {
-      if (p.bs && n0 + at - BM < p.N) scale[i] = p.bs[n0 + at - BM];
+      if (p.bs && n0 + at - BM < p.N) line[i] = p.bs[n0 + at - BM];
+    } else if (at < LINES) {
+      if (p.bias && n0 + at - BM - BN < p.N) line[i] = p.bias[n0 + at - BM - BN];
     }
   }
 
@@ -540,9 +543,8 @@ i8_tile_kernel(Int8Params p) {
 #pragma unroll
   for (int i = 0; i < SPT; ++i) {
     const int at = threadIdx.x + i * NT;
-    if (at < BM + BN) sa[at] = scale[i];
+    if (at < LINES) sa[at] = at < BM ? p.alpha * line[i] : line[i];
   }
-  for (int i = threadIdx.x; i < BN; i += NT) bias[i] = p.bias && n0 + i < p.N ? p.bias[n0 + i] : 0.0f;
   constexpr int LP = BN + 4, CPR = BN / 4, RPS = NT / CPR, PARTS = Tile::PARTS, FP = FM / PARTS, ROWS = BM / PARTS;
   int *sums = reinterpret_cast<int *>(smem);
   const int c4 = threadIdx.x % CPR, r0 = threadIdx.x / CPR;  // threads with r0 >= RPS only write to LDS
@@ -642,13 +644,13 @@ constexpr TileCost kTiles[] = {{16, 16, 329, 4, 97, 4},        {16, 64, 423, 11,
 constexpr int kKinds = sizeof(kTiles) / sizeof(kTiles[0]);
 void launch_product(const Int8Params &p, hipStream_t s) {
   const unsigned stages = (unsigned)(p.K + 127) / 128, M = (unsigned)p.M, N = (unsigned)p.N;
-  int best = 0;
-  uint64_t least = 0;
+  int best = kKinds - 1;
+  uint64_t least = ~0ull;
   for (int i = 0; i < kKinds; ++i) {
     const TileCost &k = kTiles[i];
     const uint64_t tiles = (uint64_t)((M + k.bm - 1) / k.bm) * ((N + k.bn - 1) / k.bn), others = (tiles - 1) / 256;  // 256 CUs
     const uint64_t cost = k.fixed + stages * k.stage + others * (k.next + stages * k.more);
-    if (i == 0 || cost < least) best = i, least = cost;
+    if (cost < least && tiles <= 1 << 22) best = i, least = cost;  // below 2^32 threads; the largest tiles are never more
   }
   switch (best) {
     case 0: return launch_stream<1, 1, 4, 128, 4>(p, s);
