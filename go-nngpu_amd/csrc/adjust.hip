@@ -350,7 +350,6 @@ int check_adjust(const AdjustDesc &d, CError *err) {
   if (d.biases < 0 || d.biases > kMaxBiases) return set_error(err, -1, "%s: 0 to %d biases to a row, got %d", what, kMaxBiases, d.biases);
   if (d.rows == 0) return 0;
   if (d.out == d.x && d.ldo != d.ld) return set_error(err, -1, "%s: in place the leading dimensions have to be equal", what);
-  if (d.h == 0 && d.prompt) return set_error(err, -1, "%s: prompt lengths without a history", what);
   if ((uintptr_t)d.prompt % 8 || (uintptr_t)d.repetition % 4 || (uintptr_t)d.frequency % 4 || (uintptr_t)d.presence % 4)
     return set_error(err, -1, "%s: prompt lengths or penalties not aligned to their type", what);
   if (d.biases > 0 && (!d.bias_ids || !d.bias)) return set_error(err, -1, "%s: NULL biases", what);

@@ -13,7 +13,7 @@
 namespace gn {
 namespace {
 
-constexpr long kMaxRows = 1L << 22;  // a workgroup of up to 1024 threads to a row, below 2^32 threads
+constexpr long kMaxRows = (1L << 22) - 1;  // a workgroup of up to 1024 threads to a row, below 2^32 threads
 
 struct __attribute__((packed, aligned(1))) Unaligned8 {
   u32x2_t v;

@@ -201,7 +201,8 @@ def call(name, *args):
         err = _errors.err = CError()
         _errors.ref = ctypes.byref(err)
     rc = getattr(L, name)(*args, _errors.ref)
-    _check(rc, err)
+    if rc != 0:
+        _check(rc, err)
     return rc
 
 

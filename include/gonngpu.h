@@ -522,7 +522,7 @@ int gn_adjust_logits_backward(int dtype, const void *logits, long rows, long col
  * gn_int8_quantize: x (GN_F32 or GN_F16, rows x cols, ldx >= cols elements from row to row) row by row. With y = x
  * col_scale[column] in fp32 (y = x where col_scale is NULL): s = max(max |y| / 127, 2^-126) in fp32, q the integer nearest to the
  * exact quotient y / s, ties to the even one (-127 to 127). A row with an infinity or NaN among its y has scale NaN and q = 0. Bytes
- * past cols are not written. At most 2^22 rows and 65535 * 2048 columns here and in gn_int8_dequantize. Asynchronous; allocates
+ * past cols are not written. Below 2^22 rows and at most 65535 * 2048 columns here and in gn_int8_dequantize. Asynchronous; allocates
  * nothing and may be captured, as do all of the gn_int8_* calls. Codes: -1 invalid argument, -6 launch error. */
 int gn_int8_quantize(int dtype, const void *x, long rows, long cols, long ldx, const float *col_scale, int8_t *q, long ldq,
                      float *scales, void *stream, CError *err);
@@ -540,7 +540,7 @@ int gn_int8_gemm(long M, long N, long K, float alpha, const int8_t *A, long lda,
                  void *stream, CError *err);
 /* gn_int8_gemm with activations x (GN_F32 or GN_F16, M x K, ldx elements from row to row) that are brought to 8 bits as by
  * gn_int8_quantize (the same result, bit for bit). With the gradient of a layer's outputs as x, its weights' scales as col_scale and
- * the transposed int8 weights without scales as B it gives the gradient of the layer's inputs. At most 2^22 rows of x.
+ * the transposed int8 weights without scales as B it gives the gradient of the layer's inputs. Below 2^22 rows of x.
  * workspace: gn_int8_linear_workspace(M, N, K) bytes at a multiple of 16 (may be NULL where that is 0), not shared by calls
  * that may overlap. */
 size_t gn_int8_linear_workspace(long M, long N, long K);

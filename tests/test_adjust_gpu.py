@@ -235,7 +235,6 @@ def test_empty_and_streams(dev):
     G.adjust_logits(torch.empty((0, 9), device=dev), torch.empty((0, 9), device=dev))
     c = _case(2, 700, 0, 0, torch.float32)  # a history without tokens
     d = _on(dev, c)
-    d.pop("prompt")
     x, out = d.pop("x"), torch.empty((2, 700), device=dev)
     want = R.adjust(c["x"], mask=c["mask"])
     G.adjust_logits(x, out, **d)

@@ -135,7 +135,7 @@ SIZES = [(1, 1, 1), (2, 3, 9), (70, 90, 1), (80, 100, 8), (100, 70, 33), (65, 1,
          (32, 200, 1152), (33, 257, 384), (48, 130, 2050), (64, 130, 96), (65, 129, 257), (100, 260, 1024), (128, 128, 128), (129, 256, 256),
          (200, 300, 515), (256, 512, 768), (300, 700, 1300), (513, 300, 260), (520, 1030, 4096), (1, 8200, 300), (7, 9000, 777), (20, 9100, 200),
          (60, 8300, 330), (100, 9000, 200), (200, 9000, 130), (300, 11000, 260), (1000, 11000, 140), (400, 11000, 328), (3900, 4000, 200),
-         (2, 20, 40000), (40, 20, 131071), (70, 40, 20001)]
+         (2, 20, 40000), (40, 20, 131071), (70, 40, 20001), (1, 50, 20000), (3, 33, 7000), (4, 5000, 100), (4, 17, 6000), (4, 17, 6200)]
 
 
 @pytest.mark.parametrize("M,N,K", SIZES)

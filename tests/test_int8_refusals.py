@@ -28,23 +28,24 @@ CASES = [
     ("gn_int8_quantize", QUANTIZE, [
         ("dtype", dict(dtype=FP4)), ("size", dict(rows=-1)), ("size", dict(cols=-1)), ("leading", dict(ldx=99)), ("leading", dict(ldq=99)),
         ("NULL", dict(x=None)), ("NULL", dict(q=None)), ("NULL", dict(scales=None)), ("aligned", dict(x=P + 2)), ("aligned", dict(scales=P + 2)),
-        ("aligned", dict(cs=P + 1)), ("aligned", dict(dtype=F16, x=P + 1)), ("size", dict(rows=BIG)), ("too large", dict(rows=(1 << 22) + 1)),
+        ("aligned", dict(cs=P + 1)), ("aligned", dict(dtype=F16, x=P + 1)), ("size", dict(rows=BIG)), ("too large", dict(rows=1 << 22)),
         ("too large", dict(cols=65535 * 2048 + 1, ldx=1 << 30, ldq=1 << 30))]),
     ("gn_int8_dequantize", DEQUANTIZE, [
         ("dtype", dict(dtype=7)), ("size", dict(rows=-1)), ("leading", dict(ldo=99)), ("leading", dict(ldq=99)), ("NULL", dict(out=None)),
-        ("NULL", dict(q=None)), ("NULL", dict(scales=None)), ("aligned", dict(out=P + 2)), ("too large", dict(rows=(1 << 22) + 1))]),
+        ("NULL", dict(q=None)), ("NULL", dict(scales=None)), ("aligned", dict(out=P + 2)), ("too large", dict(rows=1 << 22))]),
     ("gn_int8_gemm", GEMM, PRODUCT + [
         ("NULL A", dict(A=None)), ("leading", dict(lda=96)), ("multiples", dict(A=P + 4)), ("multiples", dict(lda=101)),
         ("too large", dict(lda=(1 << 22) + 16)), ("aligned", dict(sa=P + 3))]),
     ("gn_int8_linear", LINEAR, PRODUCT + [
-        ("dtype", dict(dtype=FP4)), ("leading", dict(ldx=99)), ("NULL", dict(x=None)), ("aligned", dict(x=P + 2)), ("aligned", dict(cs=P + 2))]),
+        ("dtype", dict(dtype=FP4)), ("leading", dict(ldx=99)), ("NULL", dict(x=None)), ("aligned", dict(x=P + 2)), ("aligned", dict(cs=P + 2)),
+        ("too large", dict(M=1 << 22))]),
     ("gn_adjust_logits", ADJUST, [
         ("dtype", dict(dtype=FP4)), ("size", dict(rows=-1)), ("size", dict(cols=0)), ("size", dict(cols=1 << 31, ld=1 << 31, ldo=1 << 31, ldmask=1 << 27)),
         ("too large", dict(rows=BIG)), ("too large", dict(rows=1 << 24)), ("too large", dict(rows=1 << 22, h=2048)),
         ("leading", dict(ld=99)), ("leading", dict(ldo=99)), ("NULL", dict(x=None)), ("NULL", dict(out=None)),
         ("aligned", dict(x=P + 2)), ("aligned", dict(out=P + 2)), ("aligned", dict(dtype=F16, x=P + 1)), ("in place", dict(out=P, ldo=101)),
         ("history", dict(h=-1)), ("history", dict(h=1 << 29)), ("NULL history", dict(hist=None)), ("history", dict(hist=P + 4)),
-        ("without a history", dict(h=0)), ("aligned", dict(prompt=P + 4)), ("aligned", dict(rep=P + 2)), ("aligned", dict(freq=P + 1)),
+        ("aligned", dict(prompt=P + 4)), ("aligned", dict(rep=P + 2)), ("aligned", dict(freq=P + 1)),
         ("aligned", dict(pres=P + 2)), ("biases", dict(nb=-1)), ("biases", dict(nb=1025)), ("NULL biases", dict(bids=None)),
         ("NULL biases", dict(bias=None)), ("aligned", dict(bids=P + 4)), ("aligned", dict(bias=P + 2)), ("words", dict(ldmask=3)),
         ("mask", dict(mask=P + 2))]),
