@@ -86,6 +86,8 @@ __global__ void __launch_bounds__(256) i8_k0_kernel(Int8Params p) {
 // bytes come at up to 90 (from L2; the Infinity Cache gives all CUs together 7.5 TB/s, 29 KB/us each).
 // A chunk of 1 KiB is RPC rows of S bytes; octet o of a row sits at place o ^ swizzle(row): the 16 rows that a phase of a fragment
 // read touches fall on distinct banks.
+// What bounds them is a chain of latencies: 27 rows 2027 -> 4099 in 5.8 us and 64 rows 4096 -> 4096 in 7.8, the waves waiting for 45% of their
+// cycles.
 template <int S>
 struct Chunk {
   static_assert(S == 64 || S == 128, "bytes to a row");
@@ -221,9 +223,11 @@ __global__ void __launch_bounds__(KW * 64) i8_stream_kernel(Int8Params p) {
   });
 }
 
-// Few rows of activations that the kernel brings to 8 bits itself, into LDS: a launch and a wait for it less than with a kernel before
-// it. QW waves do that while the first weights of the KW others are on their way (a wave's own wait for the rows would be
-// one for its weights too).
+// Up to kMaxTokens rows of activations that the kernel brings to 8 bits itself, into LDS: a launch and a wait for it less than with a
+// kernel before it. QW waves do that while the first weights of the KW others are on their way (a wave's own wait for the rows would be
+// one for its weights too). One row 4096 -> 11008 takes 11.7 us, of which its 45 MB would take 8.8 at a large copy's rate: one workgroup
+// to a CU, whose start, first weights and join nothing overlaps.
+constexpr int kMaxTokens = 4;
 __host__ __device__ inline int token_pitch(long K) { return (int)((K + 127) / 128 * 128 + 16); }  // rows on distinct banks
 template <typename T, int NF, int KW, int NS, int QW>
 __global__ void __launch_bounds__((KW + QW) * 64) i8_token_kernel(Int8Params p, const T *x, long ldx, const float *col_scale) {
@@ -231,15 +235,14 @@ __global__ void __launch_bounds__((KW + QW) * 64) i8_token_kernel(Int8Params p, 
   constexpr int CB = 16 * NF / C::RPC, SLOT = CB * 1024;
   constexpr int RING = KW * NS * SLOT, PART = KW * NF * 1024;
   static_assert((NS - 1) * CB < 64 && RING >= PART, "copies");
+  static_assert(QW % kMaxTokens == 0 && kMaxTokens == 4, "waves to a row");
   __shared__ uint32_t tops[QW];
-  __shared__ float scales[16];
+  __shared__ float scales[kMaxTokens];
   extern __shared__ __attribute__((aligned(1024))) char smem[];  // the slots, in the end the partial sums; the rows in 8 bits
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   const int M = (int)p.M, K = (int)p.K, pitch = token_pitch(K), end = pitch - 16;
   char *rows = smem + RING;
-  // Waves to a row, and the rows gone through side by side.
-  int per = QW, side = 1;
-  while (side < M && per > 1) per >>= 1, side <<= 1;
+  const int per = M == 1 ? QW : M == 2 ? QW / 2 : QW / kMaxTokens;  // waves to a row
 
   unsigned vb[CB];
   int kb[CB];
@@ -304,8 +307,8 @@ __global__ void __launch_bounds__((KW + QW) * 64) i8_token_kernel(Int8Params p, 
   if (wave < KW) {
 #pragma unroll 1
     for (int t = 0; t < NS; ++t) issue(t, t);
-    if (per > 1) lds_barrier();
-  } else if (per > 1) {
+    lds_barrier();
+  } else {
     uint32_t top = first < M ? top_of(first) : 0;
     if (lane == 0) tops[wave - KW] = top;
     lds_barrier();
@@ -313,8 +316,6 @@ __global__ void __launch_bounds__((KW + QW) * 64) i8_token_kernel(Int8Params p, 
       for (int w = 0; w < per; ++w) top = max(top, tops[first * per + w]);
       quantize(first, top);
     }
-  } else {
-    for (int m = first; m < M; m += QW) quantize(m, top_of(m));
   }
   lds_barrier();
 
@@ -355,8 +356,11 @@ __global__ void __launch_bounds__((KW + QW) * 64) i8_token_kernel(Int8Params p, 
 // WM x WN waves, each FM x FN blocks of 16 x 16. K goes in stages of 128 bytes to a row, copied straight to LDS by dma16 in chunks
 // of 8 rows (ring_plan.h's places: a wave's copies are whole 128-byte lines, its fragment reads fall on distinct banks), NS stages
 // in LDS. A stage is two steps of 64 k: while one is multiplied the next one's fragments are read, and before the
-// second the next stage has landed (one wait and one barrier to a stage) and the copies of the one NS ahead start.
+// second the next stage has landed (one wait and one barrier to a stage).
 // Where K ends inside a chunk of 16 the wave that copied it clears A's bytes past K before that barrier.
+// What bounds them: with 8192^3 the power that the matrix instructions take (434 us, 2.53 POP/s, at 1.7 GHz, the matrix units busy for 69% of
+// the cycles), with one tile to a CU the stages' latency (512 rows 4096 -> 11008 in 27 us, 11008 -> 4096 in 35: copies, fragments and
+// barriers take a stage of 128 x 192 1291 cycles and one of 64 x 128 818, where the matrix instructions alone take 768 and 256).
 template <int WM, int WN, int FM, int FN, int NS>
 struct I8Tile {
   static constexpr int BM = WM * FM * 16, BN = WN * FN * 16, STAGE = (BM + BN) * 128;
@@ -671,7 +675,7 @@ void launch_product(const Int8Params &p, hipStream_t s) {
 // Up to 4 rows of activations are brought to 8 bits in the product's kernel. Against a kernel before it, us of kernels: 1 row 1000 ->
 // 1000 4.5 / 5.9, 4096 -> 4096 7.4 / 8.8, 11008 -> 4096 12.9 / 15.3, 4096 -> 11008 11.7 / 12.8; 4 rows 9.7 / 9.0 and 13.8 / 13.1, where
 // the other's second launch costs a caller without a graph 3 us more. The rows stand beside up to 128 KiB of slots in LDS.
-bool few_tokens(long M, long K) { return M <= 4 && M * token_pitch(K) <= 24 * 1024; }
+bool few_tokens(long M, long K) { return M <= kMaxTokens && M * token_pitch(K) <= 24 * 1024; }
 template <typename T, int NF, int KW, int NS, int QW>
 void launch_token(const Int8LinearDesc &d, const Int8Params &p, hipStream_t s) {
   const int ring = KW * NF * NS * 2048;

@@ -523,7 +523,7 @@ int gn_adjust_logits_backward(int dtype, const void *logits, long rows, long col
  * col_scale[column] in fp32 (y = x where col_scale is NULL): s = max(max |y| / 127, 2^-126) in fp32, q the integer nearest to the
  * exact quotient y / s, ties to the even one (-127 to 127). A row with an infinity or NaN among its y has scale NaN and q = 0. Bytes
  * past cols are not written. Below 2^22 rows and at most 65535 * 2048 columns here and in gn_int8_dequantize. Asynchronous; allocates
- * nothing and may be captured, as do all of the gn_int8_* calls. Codes: -1 invalid argument, -6 launch error. */
+ * nothing and may be captured, as do all of the gn_int8_* calls; none may write where it reads, beyond C with beta. Codes: -1 invalid argument, -6 launch error. */
 int gn_int8_quantize(int dtype, const void *x, long rows, long cols, long ldx, const float *col_scale, int8_t *q, long ldq,
                      float *scales, void *stream, CError *err);
 /* q s, in fp32 and then rounded to GN_F32 or GN_F16; out[r, j] past cols is not written. */
