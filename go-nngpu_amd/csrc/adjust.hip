@@ -52,15 +52,16 @@ struct Vector {
   }
 };
 
-// The mask's bits of the kVec columns from `col` on (a multiple of kVec); all of them without a mask.
-template <typename T>
-__device__ __forceinline__ uint32_t allowed_bits(const uint32_t *mask, long col) {
-  return mask ? mask[col >> 5] >> (col & 31) : ~0u;
+// The mask's word with the bits of the kVec columns from `col` on (a multiple of kVec); ones without a mask. Its bits are not touched
+// here, which would be a wait for it.
+__device__ __forceinline__ uint32_t mask_word(const uint32_t *mask, long col, long cols) {
+  return mask ? mask[min(col, cols - 1) >> 5] : ~0u;
 }
 
 // A vector's masked values.
 template <typename T>
-__device__ __forceinline__ void apply_mask(Vector<T> &v, uint32_t bits, T masked) {
+__device__ __forceinline__ void apply_mask(Vector<T> &v, uint32_t word, long col, T masked) {
+  const uint32_t bits = word >> (col & 31);
   constexpr uint32_t ALL = (1u << kVec<T>) - 1;
   if ((bits & ALL) == ALL) return;
 #pragma unroll
@@ -68,22 +69,45 @@ __device__ __forceinline__ void apply_mask(Vector<T> &v, uint32_t bits, T masked
     if (!((bits >> j) & 1)) v.v[j] = masked;
 }
 
-// f(tokens, i) for this thread's share of a row's tokens, kTokens at a time, token u being the row's number i + u NT (-1 past its
-// end): their loads are in flight together.
+// This thread's share of a row's tokens, kTokens at a time, token u being the row's number i + u NT (-1 past its end): their loads
+// are in flight together, those of the first ones from the kernel's start.
 constexpr int kTokens = 4;
-template <int NT, typename F>
-__device__ __forceinline__ void for_tokens(const int64_t *ids, long n, F f) {
-  for (long i0 = threadIdx.x; i0 < n; i0 += kTokens * NT) {
-    int64_t id[kTokens];
+template <int NT>
+struct Tokens {
+  const int64_t *ids;
+  int n;  // below kMaxHistory: a token's place in bytes fits 32 bits
+  int64_t id[kTokens];
+  __device__ __forceinline__ Tokens(const int64_t *row, long h) : ids(row), n((int)h) { load(threadIdx.x); }
+  __device__ __forceinline__ void load(int i0) {
 #pragma unroll
-    for (int u = 0; u < kTokens; ++u) id[u] = i0 + u * NT < n ? ids[i0 + u * NT] : -1;
-    f(id, i0);
+    for (int u = 0; u < kTokens; ++u) {
+      const int i = i0 + u * NT;
+      id[u] = i < n ? *reinterpret_cast<const int64_t *>(reinterpret_cast<const char *>(ids) + 8u * (unsigned)i) : -1;
+    }
   }
+  // f(tokens, i) for all of them, the first of which are there.
+  template <typename F>
+  __device__ __forceinline__ void each(F f) {
+    for (int i0 = threadIdx.x; i0 < n;) {
+      f(id, i0);
+      i0 += kTokens * NT;
+      if (i0 < n) load(i0);
+    }
+  }
+  __device__ __forceinline__ void again() {
+    if (n > kTokens * NT) load(threadIdx.x);
+  }
+};
+
+// A token's column in the segment of `left` columns from col0 on, if it is below `left`.
+__device__ __forceinline__ unsigned place_of(int64_t id, long col0) {
+  const unsigned at = (unsigned)id - (unsigned)col0;
+  return (uint64_t)id >> 32 ? ~0u : at;
 }
 
 // What a column's cell of the counts says: bit 31 in the prompt, bit 30 there is a bias, bit 29 it has been put right, below them how
-// often in the answer.
-constexpr uint32_t kPrompt = 1u << 31, kBiased = 1u << 30, kDone = 1u << 29, kCount = kDone - 1;
+// often in the answer. Until its biases are added up, bit 29 says that it has several.
+constexpr uint32_t kPrompt = 1u << 31, kBiased = 1u << 30, kDone = 1u << 29, kSeveral = kDone, kCount = kDone - 1;
 
 // A row's penalties.
 struct Penalties {
@@ -104,7 +128,7 @@ __global__ void __launch_bounds__(NT) adjust_kernel(AdjustDesc p, int segs) {
   constexpr int SEG = NT * kPer, VECS = kPer / kVec<T>;
   __shared__ __attribute__((aligned(16))) uint32_t cells[SEG];
   __shared__ float sums[BIASES ? SEG : 1];  // of a token's biases, where its cell says that there are some
-  __shared__ int again;
+  __shared__ int again, hit;  // a token has several biases; there is one in the segment
   const long r = blockIdx.x / segs;
   const long col0 = (long)(blockIdx.x % segs) * SEG;
   const int left = (int)min(p.cols - col0, (long)SEG);
@@ -112,23 +136,34 @@ __global__ void __launch_bounds__(NT) adjust_kernel(AdjustDesc p, int segs) {
   T *out = static_cast<T *>(p.out) + r * p.ldo + col0;
   const int64_t *history = p.history + r * p.h, *bias_ids = p.bias_ids + r * p.biases;
   const float *bias = p.bias + r * p.biases;
+  // All that has to come from memory is asked for before anything is waited for.
+  const Penalties penalty{p.repetition ? p.repetition[r] : 1.0f, p.frequency ? p.frequency[r] : 0.0f, p.presence ? p.presence[r] : 0.0f};
+  const int prompt = p.prompt ? (int)min((int64_t)p.h, max((int64_t)0, p.prompt[r])) : 0;
+  Tokens<NT> tokens(history, p.h);
+  int64_t bias_id = -1;  // the row's bias threadIdx.x
+  float bias_value = 0.0f;
+  if (BIASES && (int)threadIdx.x < p.biases) bias_id = bias_ids[threadIdx.x], bias_value = bias[threadIdx.x];
   Vector<T> v[PATCH ? 1 : VECS];
+  uint32_t words[PATCH ? 1 : VECS];
   if constexpr (!PATCH) {
+    const uint32_t *mask = p.mask ? p.mask + r * p.ldmask : nullptr;
 #pragma unroll
-    for (int i = 0; i < VECS; ++i) v[i].load(x + place<T, NT>(i), left - place<T, NT>(i));
+    for (int i = 0; i < VECS; ++i) {
+      const int at = place<T, NT>(i);
+      words[i] = mask_word(mask, col0 + at, p.cols);
+      v[i].load(x + at, left - at);
+    }
   }
 #pragma unroll
   for (int i = 0; i < kPer / 4; ++i) reinterpret_cast<u32x4_t *>(cells)[i * NT + threadIdx.x] = u32x4_t{0, 0, 0, 0};
-  if (threadIdx.x == 0) again = 0;
+  if (threadIdx.x == 0) again = hit = 0;
   __syncthreads();
-  const long prompt = p.prompt ? p.prompt[r] : 0;
   bool any = false;
-  auto place_of = [&](int64_t id) { return (uint64_t)id - (uint64_t)col0; };  // in the segment if below `left`
-  for_tokens<NT>(history, p.h, [&](const int64_t (&id)[kTokens], long i0) {
+  tokens.each([&](const int64_t (&id)[kTokens], int i0) {
 #pragma unroll
     for (int u = 0; u < kTokens; ++u) {
-      const uint64_t at = place_of(id[u]);
-      if (at < (uint64_t)left) {
+      const unsigned at = place_of(id[u], col0);
+      if (at < (unsigned)left) {
         any = true;
         if (i0 + u * NT < prompt)
           atomicOr(&cells[at], kPrompt);
@@ -139,58 +174,67 @@ __global__ void __launch_bounds__(NT) adjust_kernel(AdjustDesc p, int segs) {
   });
   if constexpr (BIASES) {
     for (int i = threadIdx.x; i < p.biases; i += NT) {
-      const uint64_t at = place_of(bias_ids[i]);
-      if (at < (uint64_t)left) {
+      const unsigned at = place_of(i < NT ? bias_id : bias_ids[i], col0);
+      if (at < (unsigned)left) {
         any = true;
-        if (atomicOr(&cells[at], kBiased) & kBiased)
+        if (atomicOr(&cells[at], kBiased) & kBiased) {
+          atomicOr(&cells[at], kSeveral);
           again = 1;
-        else
-          sums[at] = bias[i];
+        } else {
+          sums[at] = i < NT ? bias_value : bias[i];
+        }
       }
     }
   }
-  const bool touched = __syncthreads_or(any);
-  // Where a token has several biases the first wave adds all of the segment's up anew, one after the other.
+  if (any) hit = 1;
+  __syncthreads();
+  const bool touched = hit;
+  // The biases of a token that has several are added up anew by the first wave, one after the other. A sum goes from lane to lane through
+  // LDS, which keeps a wave's order; so has the compiler to.
   if constexpr (BIASES) {
     if (again) {
       if (threadIdx.x < 64) {
-        for (int i0 = 0; i0 < p.biases; i0 += 64) {
-          const int i = i0 + threadIdx.x;
-          const uint64_t at = i < p.biases ? place_of(bias_ids[i]) : ~0ull;
-          if (at < (uint64_t)left) sums[at] = 0.0f;
+        auto several = [&](int i) {
+          const unsigned at = i >= p.biases ? ~0u : place_of(i < 64 ? bias_id : bias_ids[i], col0);
+          return at < (unsigned)left && (cells[at] & kSeveral) ? (int)at : -1;
+        };
+        for (int i = threadIdx.x; i < p.biases; i += 64) {
+          const int at = several(i);
+          if (at >= 0) sums[at] = 0.0f;
         }
-        // A sum goes from lane to lane through LDS, which keeps a wave's order; so has the compiler to.
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         for (int i0 = 0; i0 < p.biases; i0 += 64) {
-          const int i = i0 + threadIdx.x;
-          const uint64_t at = i < p.biases ? place_of(bias_ids[i]) : ~0ull;
-          const float b = i < p.biases ? bias[i] : 0.0f;
-          for (uint64_t here = __ballot(at < (uint64_t)left); here != 0; here &= here - 1) {
+          const int i = i0 + threadIdx.x, at = several(i);
+          const float b = at < 0 ? 0.0f : i < 64 ? bias_value : bias[i];
+          for (uint64_t here = __ballot(at >= 0); here != 0; here &= here - 1) {
             if ((int)threadIdx.x == __ffsll((unsigned long long)here) - 1) sums[at] += b;
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
           }
+        }
+        for (int i = threadIdx.x; PATCH && i < p.biases; i += 64) {
+          const int at = several(i);
+          if (at >= 0) atomicAnd(&cells[at], ~kSeveral);
         }
       }
       __syncthreads();
     }
   }
-  const Penalties penalty{p.repetition ? p.repetition[r] : 1.0f, p.frequency ? p.frequency[r] : 0.0f, p.presence ? p.presence[r] : 0.0f};
   if constexpr (PATCH) {
-    auto patch = [&](uint64_t at) {
-      if (at >= (uint64_t)left) return;
+    auto patch = [&](unsigned at) {
+      if (at >= (unsigned)left) return;
       const uint32_t cell = atomicOr(&cells[at], kDone);
       if (!(cell & kDone)) out[at] = (T)penalty((float)out[at], cell, BIASES ? sums[at] : 0.0f);
     };
     if (touched) {
-      for_tokens<NT>(history, p.h, [&](const int64_t (&id)[kTokens], long) {
+      tokens.again();
+      tokens.each([&](const int64_t (&id)[kTokens], int) {
 #pragma unroll
-        for (int u = 0; u < kTokens; ++u) patch(place_of(id[u]));
+        for (int u = 0; u < kTokens; ++u) patch(place_of(id[u], col0));
       });
       if constexpr (BIASES)
-        for (int i = threadIdx.x; i < p.biases; i += NT) patch(place_of(bias_ids[i]));
+        for (int i = threadIdx.x; i < p.biases; i += NT) patch(place_of(bias_ids[i], col0));
     }
   } else {
-    const uint32_t *mask = p.mask ? p.mask + r * p.ldmask : nullptr;
 #pragma unroll
     for (int i = 0; i < VECS; ++i) {
       const int at = place<T, NT>(i);
@@ -206,7 +250,7 @@ __global__ void __launch_bounds__(NT) adjust_kernel(AdjustDesc p, int segs) {
           }
         }
       }
-      apply_mask(v[i], allowed_bits<T>(mask, col0 + at), (T)-INFINITY);
+      apply_mask(v[i], words[i], col0 + at, (T)-INFINITY);
       v[i].store(out + at, left - at);
     }
   }
@@ -218,6 +262,7 @@ template <typename T, int NT, bool PATCH>
 __global__ void __launch_bounds__(NT) adjust_backward_kernel(AdjustGradDesc p, int segs) {
   constexpr int SEG = NT * kPer, VECS = kPer / kVec<T>;
   __shared__ uint32_t seen[SEG / 32], positive[SEG / 32];  // bits: a token so far, and whether its logit is above 0
+  __shared__ int hit;                                      // there is one in the segment
   const long r = blockIdx.x / segs;
   const long col0 = (long)(blockIdx.x % segs) * SEG;
   const int left = (int)min(p.cols - col0, (long)SEG);
@@ -226,25 +271,33 @@ __global__ void __launch_bounds__(NT) adjust_backward_kernel(AdjustGradDesc p, i
   const bool counts = p.repetition && p.h > 0;
   const float rho = p.repetition ? p.repetition[r] : 1.0f;
   auto factored = [&](T d, bool above) { return (T)as_fp32(above ? (float)d / rho : (float)d * rho); };
+  Tokens<NT> tokens(p.history + r * p.h, counts ? p.h : 0);
   Vector<T> v[PATCH ? 1 : VECS];
+  uint32_t words[PATCH ? 1 : VECS];
   if constexpr (!PATCH) {
+    const uint32_t *mask = p.mask ? p.mask + r * p.ldmask : nullptr;
 #pragma unroll
-    for (int i = 0; i < VECS; ++i) v[i].load(g + place<T, NT>(i), left - place<T, NT>(i));
+    for (int i = 0; i < VECS; ++i) {
+      const int at = place<T, NT>(i);
+      words[i] = mask_word(mask, col0 + at, p.cols);
+      v[i].load(g + at, left - at);
+    }
   }
   bool any = false;
   if (counts) {
+    if (threadIdx.x == 0) hit = 0;
     for (int i = threadIdx.x; i < SEG / 32; i += NT) seen[i] = positive[i] = 0;
     __syncthreads();
     // Whoever sets a token's bit first asks for its logit. They are read before anything is written: the
     // gradient may take their place.
-    for_tokens<NT>(p.history + r * p.h, p.h, [&](const int64_t (&id)[kTokens], long) {
+    tokens.each([&](const int64_t (&id)[kTokens], int) {
       int at[kTokens];
       float z[kTokens];
 #pragma unroll
       for (int u = 0; u < kTokens; ++u) {
-        const uint64_t a = (uint64_t)id[u] - (uint64_t)col0;
+        const unsigned a = place_of(id[u], col0);
         at[u] = -1;
-        if (a < (uint64_t)left && !(atomicOr(&seen[a >> 5], 1u << (a & 31)) & (1u << (a & 31)))) at[u] = (int)a, any = true;
+        if (a < (unsigned)left && !(atomicOr(&seen[a >> 5], 1u << (a & 31)) & (1u << (a & 31)))) at[u] = (int)a, any = true;
       }
 #pragma unroll
       for (int u = 0; u < kTokens; ++u) z[u] = at[u] >= 0 ? (float)x[at[u]] : 0.0f;
@@ -259,20 +312,21 @@ __global__ void __launch_bounds__(NT) adjust_backward_kernel(AdjustGradDesc p, i
     });
   }
   if constexpr (!PATCH) {
-    const bool touched = __syncthreads_or(any);
-    const uint32_t *mask = p.mask ? p.mask + r * p.ldmask : nullptr;
+    if (any) hit = 1;
+    if (counts) __syncthreads();
+    const bool touched = counts && hit;
 #pragma unroll
     for (int i = 0; i < VECS; ++i) {
       const int at = place<T, NT>(i);
       if (at >= left) break;
-      const uint32_t hit = touched ? seen[at >> 5] >> (at & 31) & ((1u << kVec<T>) - 1) : 0;
-      if (hit != 0) {
+      const uint32_t here = touched ? seen[at >> 5] >> (at & 31) & ((1u << kVec<T>) - 1) : 0;
+      if (here != 0) {
         const uint32_t above = positive[at >> 5] >> (at & 31);
 #pragma unroll
         for (int j = 0; j < kVec<T>; ++j)
-          if ((hit >> j) & 1) v[i].v[j] = factored(v[i].v[j], (above >> j) & 1);
+          if ((here >> j) & 1) v[i].v[j] = factored(v[i].v[j], (above >> j) & 1);
       }
-      apply_mask(v[i], allowed_bits<T>(mask, col0 + at), (T)0.0f);
+      apply_mask(v[i], words[i], col0 + at, (T)0.0f);
       v[i].store(out + at, left - at);
     }
   }
