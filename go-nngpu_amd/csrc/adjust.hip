@@ -4,9 +4,9 @@
 // in which they are added changes nothing), then goes once over the segment's logits, which were asked for before, and
 // looks each one's count up. In place and without a mask only the counted tokens change: each is put right by one thread, whoever
 // first sets a bit beside its count, and nothing else is read or written.
-// What bounds them: with many rows memory (4096 x 32768 in fp32, out of place, 207 us, 5.2 TB/s; the gradient, from another tensor than its
-// own, 238), with few the latency of the tokens, the counts and the logits one after the other (1 x 131072 4.0 us, 64 x 50257 in fp16
-// with 2048 tokens and 64 biases to a row 8.9).
+// What bounds them: with many rows memory (4096 x 32768 in fp32, out of place, 186 us, 5.9 TB/s; the gradient, from another tensor than its
+// own, 219), with few the latencies of the tokens, of counting them and of what is looked up (1 x 131072 3.1 us, 64 x 50257 in fp16
+// 5.2, with 2048 tokens and 64 biases to a row and a mask 7.9).
 #include <algorithm>
 #include <climits>
 #include <type_traits>
@@ -69,13 +69,48 @@ __device__ __forceinline__ void apply_mask(Vector<T> &v, uint32_t word, long col
     if (!((bits >> j) & 1)) v.v[j] = masked;
 }
 
+// A thread's value number j of all of its vectors', and that value replaced, without memory: a choice among its registers.
+template <typename T, int VECS>
+__device__ __forceinline__ T value_of(const Vector<T> (&v)[VECS], int j) {
+  constexpr int PER = 4 / (int)sizeof(T);
+  uint32_t w = 0;
+#pragma unroll
+  for (int k = 0; k < 4 * VECS; ++k) {
+    const u32x4_t four = __builtin_bit_cast(u32x4_t, v[k / 4].v);
+    w |= four[k % 4] & (j / PER == k ? ~0u : 0u);
+  }
+  if constexpr (PER == 1)
+    return __uint_as_float(w);
+  else
+    return __builtin_bit_cast(T, (uint16_t)(w >> (16 * (j % PER))));
+}
+template <typename T, int VECS>
+__device__ __forceinline__ void replace(Vector<T> (&v)[VECS], int j, T y) {
+  constexpr int PER = 4 / (int)sizeof(T);
+  uint32_t bits, mask;
+  if constexpr (PER == 1)
+    bits = __float_as_uint(y), mask = ~0u;
+  else
+    bits = (uint32_t)__builtin_bit_cast(uint16_t, y) << (16 * (j % PER)), mask = 0xffffu << (16 * (j % PER));
+#pragma unroll
+  for (int i = 0; i < VECS; ++i) {
+    u32x4_t w = __builtin_bit_cast(u32x4_t, v[i].v);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t m = j / PER == 4 * i + k ? mask : 0u;
+      w[k] = (w[k] & ~m) | (bits & m);
+    }
+    v[i].v = __builtin_bit_cast(decltype(v[i].v), w);
+  }
+}
+
 // This thread's share of a row's tokens, kTokens at a time, token u being the row's number i + u NT (-1 past its end): their loads
 // are in flight together, those of the first ones from the kernel's start.
 constexpr int kTokens = 4;
 template <int NT>
 struct Tokens {
   const int64_t *ids;
-  int n;  // below kMaxHistory: a token's place in bytes fits 32 bits
+  int n;  // below 2^29: a token's place in bytes fits 32 bits
   int64_t id[kTokens];
   __device__ __forceinline__ Tokens(const int64_t *row, long h) : ids(row), n((int)h) { load(threadIdx.x); }
   __device__ __forceinline__ void load(int i0) {
@@ -235,21 +270,26 @@ __global__ void __launch_bounds__(NT) adjust_kernel(AdjustDesc p, int segs) {
         for (int i = threadIdx.x; i < p.biases; i += NT) patch(place_of(bias_ids[i], col0));
     }
   } else {
+    if (touched) {
+      // The lanes' counted values one after the other: few rounds for a wave, as each lane has few. (All eight values in turn, those of any
+      // lane computed: 64 x 50257 with 2048 tokens 8.5 us instead of 7.9, 1 x 131072 3.2 / 3.1; only where the tokens are as many as half of the
+      // columns, 2048 x 8192 with 4096 of them, less: 31.7 / 34.3.)
+      uint32_t counted = 0;
+#pragma unroll
+      for (int j0 = 0; j0 < kPer; j0 += 4) {
+        const u32x4_t four = *reinterpret_cast<const u32x4_t *>(cells + place<T, NT>(j0 / kVec<T>) + j0 % kVec<T>);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) counted |= four[e] != 0 ? 1u << (j0 + e) : 0u;
+      }
+      for (; counted != 0; counted &= counted - 1) {
+        const int j = __ffs(counted) - 1, at = place<T, NT>(j / kVec<T>) + j % kVec<T>;
+        replace(v, j, (T)penalty((float)value_of(v, j), cells[at], BIASES ? sums[at] : 0.0f));
+      }
+    }
 #pragma unroll
     for (int i = 0; i < VECS; ++i) {
       const int at = place<T, NT>(i);
       if (at >= left) break;
-      if (touched) {
-#pragma unroll
-        for (int j0 = 0; j0 < kVec<T>; j0 += 4) {
-          const u32x4_t four = *reinterpret_cast<const u32x4_t *>(cells + at + j0);
-          if ((four[0] | four[1] | four[2] | four[3]) != 0) {
-#pragma unroll
-            for (int j = j0; j < j0 + 4; ++j)
-              if (four[j - j0] != 0) v[i].v[j] = (T)penalty((float)v[i].v[j], four[j - j0], BIASES ? sums[at + j] : 0.0f);
-          }
-        }
-      }
       apply_mask(v[i], words[i], col0 + at, (T)-INFINITY);
       v[i].store(out + at, left - at);
     }
@@ -315,17 +355,23 @@ __global__ void __launch_bounds__(NT) adjust_backward_kernel(AdjustGradDesc p, i
     if (any) hit = 1;
     if (counts) __syncthreads();
     const bool touched = counts && hit;
+    if (touched) {
+      uint32_t here = 0, above = 0;
+#pragma unroll
+      for (int i = 0; i < VECS; ++i) {
+        const int at = place<T, NT>(i);
+        here |= (seen[at >> 5] >> (at & 31) & ((1u << kVec<T>) - 1)) << (i * kVec<T>);
+        above |= (positive[at >> 5] >> (at & 31) & ((1u << kVec<T>) - 1)) << (i * kVec<T>);
+      }
+      for (; here != 0; here &= here - 1) {
+        const int j = __ffs(here) - 1;
+        replace(v, j, factored(value_of(v, j), (above >> j) & 1));
+      }
+    }
 #pragma unroll
     for (int i = 0; i < VECS; ++i) {
       const int at = place<T, NT>(i);
       if (at >= left) break;
-      const uint32_t here = touched ? seen[at >> 5] >> (at & 31) & ((1u << kVec<T>) - 1) : 0;
-      if (here != 0) {
-        const uint32_t above = positive[at >> 5] >> (at & 31);
-#pragma unroll
-        for (int j = 0; j < kVec<T>; ++j)
-          if ((here >> j) & 1) v[i].v[j] = factored(v[i].v[j], (above >> j) & 1);
-      }
       apply_mask(v[i], words[i], col0 + at, (T)0.0f);
       v[i].store(out + at, left - at);
     }
@@ -334,11 +380,11 @@ __global__ void __launch_bounds__(NT) adjust_backward_kernel(AdjustGradDesc p, i
 
 // ------------------------------------------------------------------ host
 // Threads to a workgroup: 256, 2048 logits, or 1024 where the row's tokens, all of which every workgroup reads, are many. Kernels with
-// 256 and with 1024, us (forward, gradient): 1 x 131072 fp32, 300 tokens 3.4 / 3.9, 3.4 / 4.0; 64 x 50257 fp16, 100 tokens 5.2 / 5.4,
-// 5.5 / 5.8; 256 x 131072, 1000 tokens 29.6 / 33.5, 31.2 / 37.5; 64 x 50257, 2048 tokens 10.1 / 9.3, 9.9 / 9.1; 16 x 131072, 4000
-// tokens 7.3 / 6.1, 8.2 / 6.6; 2048 x 8192, 4096 tokens 52 / 34, 62 / 42; 1 x 131072, 100000 tokens 40 / 17, 38 / 27. (32 logits to each
-// of 256 threads: 4096 x 32768 fp32 229 us, 207 with 8, 5.2 TB/s.)
-constexpr long kManyTokens = 2048;
+// 256 and with 1024, us (forward, gradient): 1 x 131072 fp32, 300 tokens 3.1 / 3.7, 3.2 / 3.7; 64 x 50257 fp16, 100 tokens 5.2 / 5.4,
+// 5.2 / 5.3, 1000 tokens 6.0 / 6.2, 6.9 / 6.2, 2048 tokens 7.9 / 7.0, 9.3 / 7.5; 256 x 131072 fp16, 1000 tokens 27.3 / 31.6, 31.2 / 31.2, 1500 tokens
+// 31.5 / 31.9, 38.9 / 33.1; 16 x 131072, 4000 tokens 6.0 / 4.7, 8.8 / 5.5; 2048 x 8192, 4096 tokens 51 / 33, 65 / 42; 1 x 131072, 100000 tokens
+// 43 / 18, 70 / 28; 4096 x 32768 fp32, 512 tokens 185 / 191, 219 / 220. (32 logits to each of 256 threads: 229 us where 8 took 207.)
+constexpr long kManyTokens = 1024;
 struct Split {
   int nt, segs;
 };

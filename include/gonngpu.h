@@ -503,7 +503,7 @@ int gn_distill_backward(int dtype, const void *logits, long rows, long cols, lon
  * word j / 32 of a row (ldmask >= ceil(cols / 32) words from row to row) says that column j is allowed; what is masked is -inf
  * whatever it was, also in a row that allows nothing. out has the logits' type, ldo >= cols, and may be the logits
  * themselves (ldo == ld). history_len below 2^29; fewer than 2^24
- * pieces of 2048 columns of rows, or with 2048 tokens of history and more 2^22 of 8192. Asynchronous; allocates nothing and may be captured. No result depends on timing.
+ * pieces of 2048 columns of rows, or with 1024 tokens of history and more 2^22 of 8192. Asynchronous; allocates nothing and may be captured. No result depends on timing.
  * Codes: -1 invalid argument, -6 launch error. */
 int gn_adjust_logits(int dtype, const void *logits, long rows, long cols, long ld, const int64_t *history, long history_len,
                      const int64_t *prompt, const float *repetition, const float *frequency, const float *presence,

@@ -107,6 +107,24 @@ def test_one_token_over_and_over(dev, dtype, in_place):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("cols,h,nb", [(40, 0, 64), (40, 300, 65), (300, 1023, 700), (300, 1024, 700), (2500, 100, 1024), (9000, 1100, 1024), (9000, 5000, 257)])
+def test_many_biases_of_few_tokens(dev, cols, h, nb, dtype, in_place):
+    """Tokens with many biases each beside tokens with one, in all of a workgroup's rounds; the sums in their order."""
+    _say("biases", cols, h, nb, dtype, in_place)
+    c = _case(3, cols, h, nb, dtype, 5, share=None)
+    g = torch.Generator().manual_seed(nb)
+    c["bias_ids"][:, ::3] = torch.randint(0, min(cols, 9), c["bias_ids"][:, ::3].shape, generator=g) * (cols // 9)
+    c["bias"] = c["bias"] * 10.0 ** torch.randint(-3, 3, c["bias"].shape, generator=g)
+    want = R.adjust(**c)
+    d = _on(dev, c)
+    x = d.pop("x")
+    out = x if in_place else torch.empty_like(x)
+    G.adjust_logits(x, out, **d)
+    assert _same(out, want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
 def test_infinities_and_nan(dev, dtype):
     """Where they are masked -inf, else what the arithmetic gives; the type's lowest value is a number as others."""
     low = torch.finfo(dtype).min
