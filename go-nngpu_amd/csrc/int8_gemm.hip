@@ -353,30 +353,32 @@ __global__ void __launch_bounds__((KW + QW) * 64) i8_token_kernel(Int8Params p, 
 }
 
 // ------------------------------------------------------------------ many rows
-// WM x WN waves, each FM x FN blocks of 16 x 16. K goes in stages of 128 bytes to a row, copied straight to LDS by dma16 in chunks
-// of 8 rows (ring_plan.h's places: a wave's copies are whole 128-byte lines, its fragment reads fall on distinct banks), NS stages
-// in LDS. A stage is two steps of 64 k: while one is multiplied the next one's fragments are read, and before the
-// second the next stage has landed (one wait and one barrier to a stage).
+// WM x WN waves, each FM x FN blocks of 16 x 16. K goes in pieces of 128 bytes to a row, copied straight to LDS by dma16 in chunks
+// of 8 rows (ring_plan.h's places: a wave's copies are whole 128-byte lines, its fragment reads fall on distinct banks), HS pieces to a
+// stage and NS stages in LDS. A piece is two steps of 64 k: while one is multiplied the next one's fragments are read, and before a
+// stage's last the next stage has landed (one wait and one barrier to a stage). Two pieces to a stage are for tiles whose
+// barrier weighs more than their products and which leave the room in LDS (512 rows 11008 -> 4096, 64 x 128 tiles: 34.6 us with one, 31.8; 256
+// rows 4096 -> 4096, 64 x 64 tiles 11.9 / 10.5; with four waves, of which two workgroups share a CU, 11.5 / 11.0 and 39.5 / 45.7).
 // Where K ends inside a chunk of 16 the wave that copied it clears A's bytes past K before that barrier.
 // What bounds them: with 8192^3 the power that the matrix instructions take (434 us, 2.53 POP/s, at 1.7 GHz, the matrix units busy for 69% of
-// the cycles), with one tile to a CU the stages' latency (512 rows 4096 -> 11008 in 27 us, 11008 -> 4096 in 35: copies, fragments and
-// barriers take a stage of 128 x 192 1291 cycles and one of 64 x 128 818, where the matrix instructions alone take 768 and 256).
-template <int WM, int WN, int FM, int FN, int NS>
+// the cycles), with one tile to a CU the stages' latency (512 rows 4096 -> 11008 in 28 us, 11008 -> 4096 in 32: copies, fragments and
+// barriers take a piece of 128 x 192 1291 cycles, where the matrix instructions alone take 768).
+template <int WM, int WN, int FM, int FN, int NS, int HS>
 struct I8Tile {
-  static constexpr int BM = WM * FM * 16, BN = WN * FN * 16, STAGE = (BM + BN) * 128;
+  static constexpr int BM = WM * FM * 16, BN = WN * FN * 16, PIECE = (BM + BN) * 128, STAGE = HS * PIECE;
   static constexpr int ALL = BM * (BN + 4) * 4, PARTS = ALL > 140 * 1024 ? 2 : 1, SUMS = ALL / PARTS;  // the sums, all at once or in halves
   static constexpr int EPI = SUMS + (BM + 2 * BN) * 4;                                                 // with the scales and the bias
   static constexpr int BYTES = NS * STAGE > EPI ? NS * STAGE : EPI;
 };
-template <int WM, int WN, int FM, int FN, int NS>
+template <int WM, int WN, int FM, int FN, int NS, int HS>
 __global__ void __launch_bounds__(WM * WN * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 i8_tile_kernel(Int8Params p) {
-  using Tile = I8Tile<WM, WN, FM, FN, NS>;
+  using Tile = I8Tile<WM, WN, FM, FN, NS, HS>;
   using C = Chunk<128>;
-  constexpr int NW = WM * WN, NT = NW * 64, BM = Tile::BM, BN = Tile::BN, STAGE = Tile::STAGE;
+  constexpr int NW = WM * WN, NT = NW * 64, BM = Tile::BM, BN = Tile::BN, PIECE = Tile::PIECE, STAGE = Tile::STAGE;
   constexpr int CA = BM / C::RPC / NW, CB = BN / C::RPC / NW, CPW = CA + CB;
   static_assert(CA * NW * C::RPC == BM && CB * NW * C::RPC == BN, "chunks");
-  static_assert((NS - 1) * CPW < 64 && NS >= 2 && FM % Tile::PARTS == 0 && NT >= BN / 4, "copies and rows");
+  static_assert((NS - 1) * HS * CPW < 64 && (NS > 2 || (NS == 2 && HS == 1)) && FM % Tile::PARTS == 0 && NT >= BN / 4, "copies and rows");
   __shared__ __attribute__((aligned(1024))) char smem[Tile::BYTES];
 
   int tm, tn;
@@ -384,7 +386,7 @@ i8_tile_kernel(Int8Params p) {
   const long m0 = (long)tm * BM, n0 = (long)tn * BN;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int wm = wave / WN, wn = wave % WN, r = lane & 15, g = lane >> 4;
-  const int ns = (int)((p.K + 127) / 128);
+  const int pieces = (int)((p.K + 127) / 128), ns = (pieces + HS - 1) / HS;
 
   // What the epilogue needs of each row and column: the rows' scales, the columns' scales and biases, thread by thread; not
   // touched, which would be a wait for them, until the stages are done with LDS.
@@ -419,7 +421,7 @@ i8_tile_kernel(Int8Params p) {
     vb[i] = n0 + row < p.N ? (unsigned)(row * p.ldb) + k_of(kb, i) : kOutOfRange;
   }
   const unsigned lds = lds_offset(smem);
-  // Part q of `parts` of a side's copies of stage t into a slot; chunks that begin at or past K read zeros.
+  // Part q of `parts` of a side's copies of piece h of stage t into a slot; chunks that begin at or past K read zeros.
   auto issue = [&](const char *base, const unsigned *v, int k, int count, int t, unsigned to, int q, int parts) {
     const int left = (int)p.K - 128 * t;
     const BufRsrc d = make_rsrc(base + 128L * t);
@@ -427,29 +429,34 @@ i8_tile_kernel(Int8Params p) {
     for (int i = 0; i < count; ++i)
       if (i * parts / count == q) dma16(d, below(v[i], k_of(k, i), left), __builtin_amdgcn_readfirstlane(to + i * 1024));
   };
-  auto issue_a = [&](int t, int slot, int q, int parts) { issue(a0, va, ka, CA, t, lds + slot * STAGE + wave * CA * 1024, q, parts); };
-  auto issue_b = [&](int t, int slot, int q, int parts) { issue(b0, vb, kb, CB, t, lds + slot * STAGE + BM * 128 + wave * CB * 1024, q, parts); };
-  // This wave's chunks of A of the last stage, once they have landed (all that is under way behind them reads zeros).
+  auto issue_a = [&](int t, int h, int slot, int q, int parts) {
+    issue(a0, va, ka, CA, t * HS + h, lds + slot * STAGE + h * PIECE + wave * CA * 1024, q, parts);
+  };
+  auto issue_b = [&](int t, int h, int slot, int q, int parts) {
+    issue(b0, vb, kb, CB, t * HS + h, lds + slot * STAGE + h * PIECE + BM * 128 + wave * CB * 1024, q, parts);
+  };
+  // This wave's chunks of A of the last piece, once they have landed (all that is under way behind them reads zeros).
   auto clear_tail = [&](int slot) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    const int left = (int)p.K - 128 * (ns - 1);
+    const int left = (int)p.K - 128 * (pieces - 1), h = (pieces - 1) % HS;
 #pragma unroll
     for (int i = 0; i < CA; ++i) {
       const int n = left - k_of(ka, i);
       if (n > 0 && n < 16) {
-        i32x4_t *c = reinterpret_cast<i32x4_t *>(smem + slot * STAGE + (wave * CA + i) * 1024 + lane * 16);
+        i32x4_t *c = reinterpret_cast<i32x4_t *>(smem + slot * STAGE + h * PIECE + (wave * CA + i) * 1024 + lane * 16);
         *c = first_bytes(*c, n);
       }
     }
   };
 
   i32x4_t fa[2][FM], fb[2][FN];
-  // Of the half h of a stage's k.
+  // Of step h of a stage, which is half a piece.
   auto read_a = [&](int slot, int h, int i) {
-    fa[h][i] = *reinterpret_cast<const i32x4_t *>(smem + slot * STAGE + C::place((wm * FM + i) * 16 + r, 4 * h + g));
+    fa[h & 1][i] = *reinterpret_cast<const i32x4_t *>(smem + slot * STAGE + h / 2 * PIECE + C::place((wm * FM + i) * 16 + r, 4 * (h & 1) + g));
   };
   auto read_b = [&](int slot, int h, int j) {
-    fb[h][j] = *reinterpret_cast<const i32x4_t *>(smem + slot * STAGE + BM * 128 + C::place((wn * FN + j) * 16 + r, 4 * h + g));
+    fb[h & 1][j] =
+        *reinterpret_cast<const i32x4_t *>(smem + slot * STAGE + h / 2 * PIECE + BM * 128 + C::place((wn * FN + j) * 16 + r, 4 * (h & 1) + g));
   };
   auto read_part = [&](int slot, int h, int q, int parts) {
 #pragma unroll
@@ -472,14 +479,18 @@ i8_tile_kernel(Int8Params p) {
   };
 
   const bool tail = p.K % 16 != 0;
-  // With two slots B's first copies are all before the loop, with more the last of them are in it.
+  // With two slots the first copies are all before the loop, with more all but the first of the last stage's are in it.
   constexpr bool SPREAD = NS > 2;
 #pragma unroll 1
   for (int t = 0; t < NS; ++t) {
-    issue_a(t, t, 0, 1);
-    if (!SPREAD || t < NS - 1) issue_b(t, t, 0, 1);
+#pragma unroll
+    for (int h = 0; h < HS; ++h) {
+      const bool all = !SPREAD || t < NS - 1;
+      if (all || h == 0) issue_a(t, h, t, 0, 1);
+      if (all) issue_b(t, h, t, 0, 1);
+    }
   }
-  __builtin_amdgcn_s_waitcnt(vmcnt_imm(SPREAD ? (NS - 2) * CPW + CA : (NS - 1) * CPW));
+  __builtin_amdgcn_s_waitcnt(vmcnt_imm(SPREAD ? (NS - 2) * HS * CPW + CA : (NS - 1) * HS * CPW));
   if (tail && ns == 1) clear_tail(0);
   __syncthreads();
   read_part(0, 0, 0, 1);
@@ -488,7 +499,7 @@ i8_tile_kernel(Int8Params p) {
     const int nxt = cur + 1 == NS ? 0 : cur + 1;
     auto arrive = [&] {  // stage t + 1 is there, in all waves
       __builtin_amdgcn_sched_barrier(0);
-      __builtin_amdgcn_s_waitcnt(vmcnt_imm((NS - 2) * CPW));
+      __builtin_amdgcn_s_waitcnt(vmcnt_imm((NS - 2) * HS * CPW));
       if (tail && t + 2 == ns) clear_tail(nxt);
       __syncthreads();
       __builtin_amdgcn_sched_barrier(0);
@@ -502,16 +513,20 @@ i8_tile_kernel(Int8Params p) {
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int i = 0; i < FM; ++i) {
-          mfma_rows(h, i, i + 1);
-          read_part(read_slot, 1 - h, i, FM);
+          mfma_rows(h & 1, i, i + 1);
+          read_part(read_slot, h + 1 < 2 * HS ? h + 1 : 0, i, FM);
           __builtin_amdgcn_sched_barrier(0);
           copies(i);
           __builtin_amdgcn_sched_barrier(0);
         }
       };
-      step(0, cur, [&](int i) { issue_b(t + NS - 1, prev, i, FM); });
+      step(0, cur, [&](int i) { issue_b(t + NS - 1, 0, prev, i, FM); });
+      if constexpr (HS == 2) {
+        step(1, cur, [&](int i) { issue_a(t + NS - 1, 1, prev, i, FM); });
+        step(2, cur, [&](int i) { issue_b(t + NS - 1, 1, prev, i, FM); });
+      }
       arrive();
-      step(1, nxt, [&](int i) { issue_a(t + NS, cur, i, FM); });
+      step(2 * HS - 1, nxt, [&](int i) { issue_a(t + NS, 0, cur, i, FM); });
     } else {
       // Two slots leave no step to spread the copies over: in two bursts, each once the matrix instructions have work (8192^3 440 us; row
       // by row 472; four slots of half a stage, with a barrier to each, 484).
@@ -523,14 +538,14 @@ i8_tile_kernel(Int8Params p) {
       arrive();
       mfma_rows(1, 0, 1);
       __builtin_amdgcn_sched_barrier(0);
-      issue_a(t + NS, cur, 0, 1);
+      issue_a(t + NS, 0, cur, 0, 1);
       read_part(nxt, 0, 0, 2);
       mfma_rows(1, 1, R0);
       sched_interleave<(R0 - 1) * FN, NR>();
       __builtin_amdgcn_sched_barrier(0);
       mfma_rows(1, R0, R0 + 1);
       __builtin_amdgcn_sched_barrier(0);
-      issue_b(t + NS, cur, 0, 1);
+      issue_b(t + NS, 0, cur, 0, 1);
       read_part(nxt, 0, 1, 2);
       mfma_rows(1, R0 + 1, FM);
       sched_interleave<(FM - R0 - 1) * FN, NR>();
@@ -622,28 +637,28 @@ void launch_stream(Int8Params p, hipStream_t s) {
   hipLaunchKernelGGL((i8_stream_kernel<MF, NF, KW, S, NS>), dim3((unsigned)(p.tiles_m * p.tiles_n)), dim3(KW * 64), 0, s, p);
 }
 
-template <int WM, int WN, int FM, int FN, int NS>
+template <int WM, int WN, int FM, int FN, int NS, int HS = 1>
 void launch_tiles(Int8Params p, hipStream_t s) {
   constexpr int BM = WM * FM * 16, BN = WN * FN * 16;
   p.tiles_m = (int)((p.M + BM - 1) / BM);
   p.tiles_n = (int)((p.N + BN - 1) / BN);
-  hipLaunchKernelGGL((i8_tile_kernel<WM, WN, FM, FN, NS>), dim3((unsigned)(p.tiles_m * p.tiles_n)), dim3(WM * WN * 64), 0, s, p);
+  hipLaunchKernelGGL((i8_tile_kernel<WM, WN, FM, FN, NS, HS>), dim3((unsigned)(p.tiles_m * p.tiles_n)), dim3(WM * WN * 64), 0, s, p);
 }
 
 // The kind of tile with which the busiest CU's share takes the least time, the first of equals. In 10 ns: fixed, and `stage` for each
 // 128 of K, for a tile alone on a CU; `next`, and `more` for each 128 of K, for each further tile of its share. Fitted to
-// these kinds' times on 23 sizes from 64 to 8192 rows and 100 to 11008 columns and K; of those the choice takes 0.7% more than the best kind
-// of each, at most 8% (32 rows 4096 -> 11008). Measured, us, 16 x 16 / 16 x 64 / 32 x 32 / 32 x 64 / 64 x 64 (8 waves) / 64 x 64 (4) / 64 x 128
-// (8) / 64 x 128 (4) / 128 x 128 / 128 x 192 / 128 x 256 / 256 x 256: 4096 -> 4096, 64 rows 11.2 / 7.9 / 7.4 / 9.2 / 10.2 / 11.3 / 13.7 / 15.0 /
-// 17.5 / 22.0 / 26.3 / 39.9, 256 rows 34.9 / 25.2 / 22.3 / 16.4 / 11.4 / 11.6 / 14.0 / 15.4 / 18.2 / 23.2 / 27.2 / 43.7, 2048 rows 308 / 197 /
-// 205 / 131 / 73.5 / 61.2 / 56.1 / 46.7 / 45.3 / 49.4 / 37.2 / 44.4; 512 rows 4096 -> 11008 166 / 139 / 112 / 77 / 54.0 / 44.7 / 41.8 / 38.0 / 38.5 /
-// 27.5 / 30.6 / 44.5, 11008 -> 4096 189 / 103 / 90 / 73 / 46.0 / 40.8 / 35.2 / 37.0 / 40.2 / 51.2 / 62.0 / 101.
+// these kinds' times on some 25 sizes from 16 to 8192 rows and 100 to 16000 columns and K; of 26 such sizes the choice takes 0.6% more than the best
+// kind of each, at most 13% (32 rows 4096 -> 11008). Measured, us, 16 x 16 / 16 x 64 / 32 x 32 / 32 x 64 / 64 x 64 (8 waves) / 64 x 64 (4) / 64 x 128
+// (8) / 64 x 128 (4) / 128 x 128 / 128 x 192 / 128 x 256 / 256 x 256: 4096 -> 4096, 64 rows 11.3 / 8.0 / 7.5 / 9.3 / 9.8 / 11.1 / 12.1 / 14.5 /
+// 17.8 / 22.1 / 26.4 / 40.2, 256 rows 36.1 / 25.4 / 22.3 / 16.3 / 10.3 / 11.3 / 12.2 / 14.7 / 18.2 / 23.2 / 27.5 / 44.0, 2048 rows 308 / 197 /
+// 205 / 131 / 68.2 / 58.7 / 55.4 / 46.8 / 43.7 / 49.1 / 35.2 / 44.3; 512 rows 4096 -> 11008 166 / 140 / 112 / 77 / 50.6 / 43.1 / 39.9 / 35.2 / 38.3 /
+// 27.9 / 29.1 / 43.6, 11008 -> 4096 190 / 103 / 90 / 73 / 42.1 / 38.8 / 32.0 / 34.5 / 41.0 / 52.0 / 62.7 / 101.
 struct TileCost {
   unsigned bm, bn, fixed, stage, next, more;
 };
 constexpr TileCost kTiles[] = {{16, 16, 329, 4, 97, 4},        {16, 64, 423, 11, 274, 10},     {32, 32, 404, 9, 252, 9},
-                               {32, 64, 369, 18, 251, 16},     {64, 64, 356, 22, 225, 22},     {64, 64, 369, 24, 132, 18},
-                               {64, 128, 398, 32, 299, 36},    {64, 128, 441, 34, 194, 29},    {128, 128, 555, 41, 452, 56},
+                               {32, 64, 369, 18, 251, 16},     {64, 64, 408, 19, 228, 19},     {64, 64, 369, 24, 132, 18},
+                               {64, 128, 447, 26, 218, 37},    {64, 128, 441, 34, 194, 29},    {128, 128, 555, 41, 452, 56},
                                {128, 192, 658, 54, 779, 67},   {128, 256, 689, 68, 835, 90},   {256, 256, 1084, 119, 1645, 162}};
 constexpr int kKinds = sizeof(kTiles) / sizeof(kTiles[0]);
 void launch_product(const Int8Params &p, hipStream_t s) {
@@ -661,9 +676,9 @@ void launch_product(const Int8Params &p, hipStream_t s) {
     case 1: return launch_stream<1, 4, 8, 128, 2>(p, s);
     case 2: return launch_stream<2, 2, 8, 128, 2>(p, s);
     case 3: return launch_stream<2, 4, 8, 64, 2>(p, s);
-    case 4: return launch_tiles<2, 4, 2, 1, 4>(p, s);
+    case 4: return launch_tiles<2, 4, 2, 1, 3, 2>(p, s);
     case 5: return launch_tiles<2, 2, 2, 2, 4>(p, s);
-    case 6: return launch_tiles<2, 4, 2, 2, 3>(p, s);
+    case 6: return launch_tiles<2, 4, 2, 2, 3, 2>(p, s);
     case 7: return launch_tiles<2, 2, 2, 4, 3>(p, s);
     case 8: return launch_tiles<2, 4, 4, 2, 3>(p, s);
     case 9: return launch_tiles<2, 4, 4, 3, 3>(p, s);

@@ -152,6 +152,18 @@ def test_product(dev, M, N, K):
         assert torch.equal(y.cpu(), R.product(a, ps, b, qs))
 
 
+@pytest.mark.parametrize("M,N,K", [(190, 9000, K) for K in (1, 16, 100, 128, 129, 140, 255, 256, 257, 300, 384, 400, 512, 515, 640, 700, 777)] +
+                         [(200, 3000, K) for K in (1025, 1040, 1152, 1153, 1279, 1280, 1285, 1408, 1500)])
+def test_ends_of_k(dev, M, N, K):
+    """K that ends at, inside and next to each piece of a stage; A's bytes past it are not zeros."""
+    _say("ends of K", M, N, K)
+    a, b = _ints(M, K, K), _ints(N, K, K + 1)
+    ad, bd = _stored(dev, a, 77), _stored(dev, b, -99)
+    y = torch.full((M, N), math.nan, device=dev)
+    G.int8_gemm((ad, None), (bd, None), y)
+    assert torch.equal(y.cpu(), R.product(a, None, b, None))
+
+
 @pytest.mark.parametrize("M,N", [(1, 20), (10, 20), (40, 20), (70, 20)])
 def test_largest_sums(dev, M, N):
     """Every product 128 x 128 over the largest K, and the same with the other sign."""
