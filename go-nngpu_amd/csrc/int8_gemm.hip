@@ -699,14 +699,18 @@ void launch_token(const Int8LinearDesc &d, const Int8Params &p, hipStream_t s) {
 }
 template <typename T>
 void launch_tokens(const Int8LinearDesc &d, const Int8Params &p, hipStream_t s) {
-  // As few columns to a workgroup as leave no CU a second one: 1 row 4096 -> 4096 7.4 us with 16, 7.9 with 32, 9.2 with 64 columns;
-  // 4096 -> 11008 16.4, 15.5 and 11.7.
+  // As few columns to a workgroup as leave no CU a second one: 1 row 4096 -> 4096 7.2 us with 16, 7.6 with 32, 8.8 with 64 columns;
+  // 4096 -> 8192 10.8, 11.3, 11.7; 4096 -> 11008 14.4, 12.8, 11.6. Where 64 are too few for that, small workgroups of which several share a CU, so
+  // that one's end falls into another's stream: 4096 -> 14000 13.6 (64 columns 13.0), 17000 15.9 (20.1), 32768 29.0 (34.6), 131072 93 (115, 5.8
+  // and 4.7 TB/s); 4 rows 4096 -> 32768 40.3 (38.1), 131072 119 (139).
   if (p.N <= 16 * 256)
     launch_token<T, 1, 8, 2, 8>(d, p, s);
   else if (p.N <= 32 * 256)
     launch_token<T, 2, 8, 2, 8>(d, p, s);
-  else
+  else if (p.N <= 64 * 256)
     launch_token<T, 4, 8, 2, 8>(d, p, s);
+  else
+    launch_token<T, 2, 4, 2, 4>(d, p, s);
 }
 
 Int8Params params_of(const Int8GemmDesc &d) {

@@ -189,6 +189,19 @@ def test_linear(dev, M, N, K, dtype, scaled):
     assert torch.equal(y.cpu(), R.product(q, s, b, sb))
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("M", [1, 2, 3, 4])
+@pytest.mark.parametrize("N,K", [(16384, 100), (16385, 100), (16400, 515), (40003, 1), (20000, 4100)])
+def test_few_rows_of_many_columns(dev, M, N, K, dtype):
+    _say("few rows", M, N, K, dtype)
+    x = (torch.randn((M, K), generator=torch.Generator().manual_seed(M + N))).to(dtype)
+    b, sb = _ints(N, K, N), _scales(N, 6)
+    y = torch.full((M, N), math.nan, device=dev)
+    G.int8_linear(x.to(dev), (_stored(dev, b, -99), sb.to(dev)), y)
+    q, s = R.quantize(x)
+    assert torch.equal(y.cpu(), R.product(q, s, b, sb))
+
+
 @pytest.mark.parametrize("M", [1, 3, 9, 20, 50, 90, 300])
 def test_linear_rows_with_nan_and_inf(dev, M):
     """Their rows are NaN and no others."""
