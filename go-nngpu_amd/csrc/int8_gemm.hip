@@ -662,6 +662,10 @@ constexpr TileCost kTiles[] = {{16, 16, 329, 4, 97, 4},        {16, 64, 423, 11,
                                {128, 192, 658, 54, 779, 67},   {128, 256, 689, 68, 835, 90},   {256, 256, 1084, 119, 1645, 162}};
 constexpr int kKinds = sizeof(kTiles) / sizeof(kTiles[0]);
 void launch_product(const Int8Params &p, hipStream_t s) {
+  // One block of rows and a stream of weights longer than the model looks ahead: small workgroups, several to a CU, so that one's end
+  // falls into another's stream. Against the model's choice, us, 16 rows: 4096 -> 32768 30.2 / 34.0, 50257 42.2 / 52.5, 131072 95.7 (5.6
+  // TB/s) / 121; 8192 -> 17000 36.7 / 41.9; 11008 -> 65536 134 / 163; 2600 -> 131072 77.7 / 72.3, 2048 56.6 / 50.4, 1000 38.9 / 31.5.
+  if (p.M <= 16 && p.N > 64 * 256 && p.K > 3584) return launch_stream<1, 2, 4, 128, 2>(p, s);
   const unsigned stages = (unsigned)(p.K + 127) / 128, M = (unsigned)p.M, N = (unsigned)p.N;
   int best = kKinds - 1;
   uint64_t least = ~0ull;

@@ -164,6 +164,15 @@ def test_ends_of_k(dev, M, N, K):
     assert torch.equal(y.cpu(), R.product(a, None, b, None))
 
 
+@pytest.mark.parametrize("M,N,K", [(1, 16385, 3585), (16, 16400, 3600), (5, 16390, 4097), (16, 16416, 5003), (17, 16400, 3600), (16, 16384, 3600), (16, 16400, 3584)])
+def test_few_rows_of_a_long_stream(dev, M, N, K):
+    _say("long stream", M, N, K)
+    a, b, sa, sb = _ints(M, K, M), _ints(N, K, N), _scales(M, 5), _scales(N, 6)
+    y = torch.full((M, N), math.nan, device=dev)
+    G.int8_gemm((_stored(dev, a), sa.to(dev)), (_stored(dev, b, -99), sb.to(dev)), y)
+    assert torch.equal(y.cpu(), R.product(a, sa, b, sb))
+
+
 @pytest.mark.parametrize("M,N", [(1, 20), (10, 20), (40, 20), (70, 20)])
 def test_largest_sums(dev, M, N):
     """Every product 128 x 128 over the largest K, and the same with the other sign."""
