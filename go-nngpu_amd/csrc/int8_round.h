@@ -69,21 +69,21 @@ __device__ __forceinline__ float int8_scale(uint32_t top) {
 // y / s rounded to the nearest integer, ties to the even one, of the exact quotient, for eight values, as bytes. k from an approximate
 // quotient is off by one at most, and only where the quotient is next to a middle. r = y - k s is exact there: for |y| >= s
 // both terms are multiples of s's last place and |r| is below s; below that k is 0, or 1 where r is exact or at least not
-// rounded past s / 2. inv: about 1 / s.
+// rounded past s / 2. r stands on the middle where 2 |r| = s: doubling is exact, and s / 2 is not for every s below 2^-125.
+// inv: about 1 / s.
 __device__ __forceinline__ u32x2_t int8_round8(const float (&y)[8], float s, float inv) {
-  const float half = 0.5f * s;
   float k[8], worst = 0.0f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     k[i] = rintf(y[i] * inv);
     worst = fmaxf(worst, fabsf(fmaf(-k[i], s, y[i])));
   }
-  if (worst >= half) {  // seldom
+  if (worst + worst >= s) {  // seldom
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float r = fmaf(-k[i], s, y[i]), a = fabsf(r);
+      const float r = fmaf(-k[i], s, y[i]), twice = fabsf(r + r);
       const bool odd = fabsf(k[i] - 2.0f * rintf(0.5f * k[i])) == 1.0f;
-      if (a > half || (a == half && odd)) k[i] += copysignf(1.0f, r);
+      if (twice > s || (twice == s && odd)) k[i] += copysignf(1.0f, r);
     }
   }
   u32x2_t q;
