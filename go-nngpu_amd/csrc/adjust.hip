@@ -408,7 +408,7 @@ int check_common(const char *what, int dtype, long rows, long cols, const int64_
   if (dtype != GN_F32 && dtype != GN_F16) return set_error(err, -1, "%s: unsupported dtype %d", what, dtype);
   if (rows < 0 || cols < 1 || cols > INT_MAX) return set_error(err, -1, "%s: invalid size %ld x %ld", what, rows, cols);
   const Split sp = split_of(cols, h);
-  if (rows >= (1L << 32) / sp.nt / sp.segs) return set_error(err, -1, "%s: %ld x %ld is too large", what, rows, cols);  // threads
+  if (rows > ((1L << 32) / sp.nt - 1) / sp.segs) return set_error(err, -1, "%s: %ld x %ld is too large", what, rows, cols);  // threads
   // Counts stay below the bits that stand beside them.
   if (h < 0 || h >= (long)kDone || !matrix_bytes(rows, h, 8, &n)) return set_error(err, -1, "%s: history of %ld tokens", what, h);
   if (rows == 0) return 0;
