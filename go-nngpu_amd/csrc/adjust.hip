@@ -147,10 +147,10 @@ constexpr uint32_t kPrompt = 1u << 31, kBiased = 1u << 30, kDone = 1u << 29, kSe
 // A row's penalties.
 struct Penalties {
   float rho, freq, pres;
-  // y of a counted token, whose biases' sum is `bias` where it has some.
+  // y of a counted token, whose biases' sum is `bias` where it has some. No product is left open to be taken with the sum after it.
   __device__ __forceinline__ float operator()(float y, uint32_t cell, float bias) const {
     const uint32_t n = cell & kCount;
-    if (n != 0 || (cell & kPrompt)) y = y > 0.0f ? y / rho : y * rho;
+    if (n != 0 || (cell & kPrompt)) y = y > 0.0f ? y / rho : as_fp32(y * rho);
     if (n != 0) y = (y - as_fp32(freq * (float)n)) - pres;
     if (cell & kBiased) y = as_fp32(y) + bias;
     return as_fp32(y);

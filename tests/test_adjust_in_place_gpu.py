@@ -134,3 +134,22 @@ def test_most_rows(dev, dtype, in_place):
     out = x if in_place else torch.full_like(x, 7.0)
     G.adjust_logits(x, out, history=history, repetition=rho)
     assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_penalty_is_rounded_before_the_next_is_taken_off(dev, dtype, in_place):
+    """x rho needs more than 24 bits and nearly equals the frequency's n: what is left shows whether it was rounded."""
+    cols, e = 64, 2.0**-11
+    x = torch.full((1, cols), -(1 + e)).to(dtype)
+    rho = torch.tensor([1 + 2.0**-23])
+    history = torch.arange(cols)[None]
+    c = dict(history=history, repetition=rho, frequency=torch.tensor([-(1 + e)]))
+    if dtype == torch.float16:
+        x = torch.full((1, cols), -(1 + 2.0**-10), dtype=dtype)
+        c["frequency"] = torch.tensor([-(1 + 2.0**-10)])
+    want = R.adjust(x, **c)
+    d = x.to(dev)
+    out = d if in_place else torch.empty_like(d)
+    G.adjust_logits(d, out, **_on(dev, c))
+    assert _same(out, want)
