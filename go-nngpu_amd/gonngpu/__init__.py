@@ -688,7 +688,8 @@ def _int8_product(what, rows, K, B, C, bias):
 
 def int8_gemm(A, B, C, *, alpha=1.0, beta=0.0, bias=None, act=ACT_NONE, act_alpha=0.0, stream_ptr=None):
     """C = act(alpha*A*B^T + beta*C + bias) with A = (int8 values, scales) of a rows x inputs matrix and B the same of an
-    outputs x inputs one, as in int8_empty. Scales may be None (1 for each row)."""
+    outputs x inputs one, as in int8_empty. Scales may be None (1 for each row). Rows begin at multiples of 16 bytes; the 16
+    bytes in which a row's last value lies are read whole, the last row's too, and what is no value there counts for nothing."""
     a, a_scales = A
     rows, K, lda = _int8_matrix("int8_gemm: A", a)
     w, w_scales, M, N, ldb, ldc = _int8_product("int8_gemm", rows, K, B, C, bias)
@@ -707,7 +708,7 @@ def _int8_workspace_bytes(M, N, K):
 def int8_linear(x, B, C, *, col_scale=None, alpha=1.0, beta=0.0, bias=None, act=ACT_NONE, act_alpha=0.0, stream_ptr=None):
     """int8_gemm with a float32 or float16 matrix x that int8_quantize brings to 8 bits on the way (col_scale: a factor for
     each of its columns). With the gradient of a layer's outputs as x, the layer's scales as col_scale and
-    (the transposed weights, None) as B: the gradient of the layer's inputs."""
+    (the transposed weights, None) as B: the gradient of the layer's inputs. B's rows are read as int8_gemm reads them."""
     dt, rows, K, ldx = _matrix("int8_linear: x", x)
     w, w_scales, M, N, ldb, ldc = _int8_product("int8_linear", rows, K, B, C, bias)
     if col_scale is not None:

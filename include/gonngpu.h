@@ -532,8 +532,8 @@ int gn_int8_dequantize(const int8_t *q, const float *scales, long rows, long col
 /* C[M,N] = act( alpha * S * b_scales[n] * a_scales[m] + beta * C + bias[n] ) with S = sum_k A[m,k] B[n,k] (A M x K, B
  * N x K: a linear layer's weights, outputs x inputs). S is exact; brought to fp32 it is multiplied by b_scales[n] and then by the
  * rounded alpha a_scales[m], in one step with the addition of beta C + bias[n]; scales that are NULL are 1. A, B and, with several rows, lda and ldb are multiples of 16 bytes, the
- * leading dimensions at most 2^22; a row's bytes from K to the next multiple of 16 are read, the last row's too, and count for
- * nothing. K is below 2^17, M and N at most 2^25. C and bias are fp32; bias may be NULL; beta == 0 never reads C; act and act_alpha
+ * leading dimensions at most 2^22; a row's bytes from K to the next multiple of 16 are read and count for nothing: the last row's
+ * too, so memory behind a matrix is read as far as the 16 aligned bytes reach in which its last value lies, and no farther. K is below 2^17, M and N at most 2^25. C and bias are fp32; bias may be NULL; beta == 0 never reads C; act and act_alpha
  * as gn_gemm; K == 0 gives act(beta * C + bias). Codes: -1 invalid argument, -6 launch error. */
 int gn_int8_gemm(long M, long N, long K, float alpha, const int8_t *A, long lda, const float *a_scales, const int8_t *B,
                  long ldb, const float *b_scales, float beta, float *C, long ldc, const float *bias, int act, float act_alpha,
