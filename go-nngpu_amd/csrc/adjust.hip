@@ -4,9 +4,11 @@
 // in which they are added changes nothing), then goes once over the segment's logits, which were asked for before, and
 // looks each one's count up. In place and without a mask only the counted tokens change: each is put right by one thread, whoever
 // first sets a bit beside its count, and nothing else is read or written.
-// What bounds them: with many rows memory (4096 x 32768 in fp32, out of place, 186 us, 5.9 TB/s; the gradient, from another tensor than its
-// own, 219), with few the latencies of the tokens, of counting them and of what is looked up (1 x 131072 3.1 us, 64 x 50257 in fp16
-// 5.2, with 2048 tokens and 64 biases to a row and a mask 7.9).
+// What bounds them: with many rows memory (4096 x 32768 in fp32, out of place, 182 us, 5.9 TB/s; the gradient, from another tensor than its
+// own, 216), with few the latencies of the tokens, of counting them and of what is looked up (1 x 131072 3.1 us, 64 x 50257 in fp16
+// 5.2, with 2048 tokens and 64 biases to a row and a mask 7.9). In place without a mask, where the tokens and what they name is all that a call
+// has to read, it is that every segment's workgroup reads all of its row's tokens: 256 x 131072 in fp16 with 1000 of them 25 us, several
+// times what the bytes would take.
 #include <algorithm>
 #include <climits>
 #include <type_traits>
@@ -384,6 +386,11 @@ __global__ void __launch_bounds__(NT) adjust_backward_kernel(AdjustGradDesc p, i
 // 5.2 / 5.3, 1000 tokens 6.0 / 6.2, 6.9 / 6.2, 2048 tokens 7.9 / 7.0, 9.3 / 7.5; 256 x 131072 fp16, 1000 tokens 27.3 / 31.6, 31.2 / 31.2, 1500 tokens
 // 31.5 / 31.9, 38.9 / 33.1; 16 x 131072, 4000 tokens 6.0 / 4.7, 8.8 / 5.5; 2048 x 8192, 4096 tokens 51 / 33, 65 / 42; 1 x 131072, 100000 tokens
 // 43 / 18, 70 / 28; 4096 x 32768 fp32, 512 tokens 185 / 191, 219 / 220. (32 logits to each of 256 threads: 229 us where 8 took 207.)
+// In place without a mask the kernels that touch only the tokens' columns are taken (PATCH). They and those that pass over the row, both in place,
+// us (forward, gradient): 1 x 131072 fp32, 300 tokens 2.8 / 3.1, 2.5 / 3.2; 64 x 50257 fp16, 100 tokens 3.8 / 5.4, 3.4 / 5.3, 1000 tokens
+// 5.4 / 6.0, 5.9 / 6.8, 2048 tokens 5.6 / 7.0, 5.6 / 7.7; 256 x 131072 fp16, 1000 tokens 25 / 28, 25 / 32; 16 x 131072, 4000 tokens 4.4 / 4.6, 4.9 / 5.5;
+// 2048 x 8192, 1500 tokens 18 / 23, 23 / 27; 4096 x 32768 fp32, 512 tokens 90 / 188, 115 / 223. They are the slower ones for long histories, 2048 x
+// 8192, 4096 tokens 36 / 30, 49 / 40; 1 x 131072, 20000 tokens 11.0 / 6.8, 9.6 / 9.1, 100000 tokens 40 / 18, 33 / 29: no border is drawn there.
 constexpr long kManyTokens = 1024;
 struct Split {
   int nt, segs;

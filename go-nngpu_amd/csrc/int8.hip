@@ -22,7 +22,7 @@ struct __attribute__((packed, aligned(1))) Unaligned8 {
 // ------------------------------------------------------------------ quantisation
 // TX threads to a row (a wave, or a workgroup), each E times 8 values in registers, lanes next to each other on values next to
 // each other: all loads in flight together, one read of the row. Longer rows (LOOP) are read twice, for their largest magnitude and
-// for their values. Many rows go at the memory's rate (11008 x 4096 fp16, 135 MB, 23 to 26 us).
+// for their values. Many rows go at the memory's rate (11008 x 4096 fp16, 135 MB, 26 to 28 us).
 template <typename T, int TX, int E, bool SCALED, bool LOOP>
 __global__ void __launch_bounds__(TX < 256 ? 256 : TX) int8_quantize_kernel(Int8QuantizeDesc p) {
   constexpr int RPW = TX < 256 ? 256 / TX : 1, W = TX / 64;  // rows to a workgroup, waves to a row
@@ -107,7 +107,7 @@ __global__ void __launch_bounds__(TX < 256 ? 256 : TX) int8_quantize_kernel(Int8
 
 // ------------------------------------------------------------------ and back
 // A thread takes 8 values of kRows rows, its loads in flight together; a workgroup is 1 << lx threads along a row by 256 >> lx rows.
-// Memory bounds it (11008 x 4096 to fp16 21 us, half of what it reads still in the Infinity Cache after the quantisation).
+// Memory bounds it (11008 x 4096 to fp16 21 to 22 us, half of what it reads still in the Infinity Cache after the quantisation).
 constexpr int kRows = 4;
 
 __device__ __forceinline__ void store8(float *p, long left, const float v[8]) {

@@ -2,6 +2,9 @@
 //
 // The sums are exact in 32 bits (K below 2^17). A sum becomes fp32, is multiplied by its column's scale, and then by alpha times its
 // row's in one step with the addition of what beta and the bias give.
+//
+// Times in this file: of a kernel among others in a captured graph, on three sets of inputs in turn, so that weights of up to some 80 MB
+// come from the Infinity Cache. They differ by 2 to 5% from run to run.
 #include <algorithm>
 #include <climits>
 
@@ -86,7 +89,7 @@ __global__ void __launch_bounds__(256) i8_k0_kernel(Int8Params p) {
 // bytes come at up to 90 (from L2; the Infinity Cache gives all CUs together 7.5 TB/s, 29 KB/us each).
 // A chunk of 1 KiB is RPC rows of S bytes; octet o of a row sits at place o ^ swizzle(row): the 16 rows that a phase of a fragment
 // read touches fall on distinct banks.
-// What bounds them is a chain of latencies: 27 rows 2027 -> 4099 in 5.8 us and 64 rows 4096 -> 4096 in 7.8, the waves waiting for 45% of their
+// What bounds them is a chain of latencies: 27 rows 2027 -> 4099 in 5.2 us and 64 rows 4096 -> 4096 in 7.5, the waves waiting for 45% of their
 // cycles.
 template <int S>
 struct Chunk {
@@ -225,8 +228,9 @@ __global__ void __launch_bounds__(KW * 64) i8_stream_kernel(Int8Params p) {
 
 // Up to kMaxTokens rows of activations that the kernel brings to 8 bits itself, into LDS: a launch and a wait for it less than with a
 // kernel before it. QW waves do that while the first weights of the KW others are on their way (a wave's own wait for the rows would be
-// one for its weights too). One row 4096 -> 11008 takes 11.7 us, of which its 45 MB would take 8.8 at a large copy's rate: one workgroup
-// to a CU, whose start, first weights and join nothing overlaps.
+// one for its weights too). One row 4096 -> 11008 takes 11.5 us (14.5 with weights from memory), of which its 45 MB would take 8.8 at a large
+// copy's rate: one workgroup to a CU, whose start, first weights and join nothing overlaps. 11008 -> 4096 takes 12.8 (16.4) and 4096 -> 4096
+// 6.9 (7.9; 3.3 at that rate): with 16 columns to a workgroup 32 KiB of a CU's 64 or 172 are on their way while the row is quantised.
 constexpr int kMaxTokens = 4;
 __host__ __device__ inline int token_pitch(long K) { return (int)((K + 127) / 128 * 128 + 16); }  // rows on distinct banks
 template <typename T, int NF, int KW, int NS, int QW>
@@ -360,8 +364,8 @@ __global__ void __launch_bounds__((KW + QW) * 64) i8_token_kernel(Int8Params p, 
 // barrier weighs more than their products and which leave the room in LDS (512 rows 11008 -> 4096, 64 x 128 tiles: 34.6 us with one, 31.8; 256
 // rows 4096 -> 4096, 64 x 64 tiles 11.9 / 10.5; with four waves, of which two workgroups share a CU, 11.5 / 11.0 and 39.5 / 45.7).
 // Where K ends inside a chunk of 16 the wave that copied it clears A's bytes past K before that barrier.
-// What bounds them: with 8192^3 the power that the matrix instructions take (434 us, 2.53 POP/s, at 1.7 GHz, the matrix units busy for 69% of
-// the cycles), with one tile to a CU the stages' latency (512 rows 4096 -> 11008 in 28 us, 11008 -> 4096 in 32: copies, fragments and
+// What bounds them: with 8192^3 the power that the matrix instructions take (442 us, 2.49 POP/s, at 1.7 GHz, the matrix units busy for 68% of
+// the cycles), with one tile to a CU the stages' latency (512 rows 4096 -> 11008 in 30 us, 11008 -> 4096 in 33: copies, fragments and
 // barriers take a piece of 128 x 192 1291 cycles, where the matrix instructions alone take 768).
 template <int WM, int WN, int FM, int FN, int NS, int HS>
 struct I8Tile {
