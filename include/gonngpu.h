@@ -502,8 +502,8 @@ int gn_distill_backward(int dtype, const void *logits, long rows, long cols, lon
  * above, stands for no token. Penalties that are NULL are not applied; repetition is above 0. mask: bit j % 32 of
  * word j / 32 of a row (ldmask >= ceil(cols / 32) words from row to row) says that column j is allowed; what is masked is -inf
  * whatever it was, also in a row that allows nothing. out has the logits' type, ldo >= cols, and may be the logits
- * themselves (ldo == ld). history_len below 2^29; fewer than 2^24
- * pieces of 2048 columns of rows, or with 1024 tokens of history and more 2^22 of 8192. Asynchronous; allocates nothing and may be captured. No result depends on timing.
+ * themselves (ldo == ld). cols and history_len are below 2^31 and 2^29; fewer than 2^24 pieces of 2048 columns of rows, or with 1024
+ * tokens of history and more 2^22 of 8192. Asynchronous; allocates nothing and may be captured. No result depends on timing.
  * Codes: -1 invalid argument, -6 launch error. */
 int gn_adjust_logits(int dtype, const void *logits, long rows, long cols, long ld, const int64_t *history, long history_len,
                      const int64_t *prompt, const float *repetition, const float *frequency, const float *presence,
@@ -533,8 +533,9 @@ int gn_int8_dequantize(const int8_t *q, const float *scales, long rows, long col
  * N x K: a linear layer's weights, outputs x inputs). S is exact; brought to fp32 it is multiplied by b_scales[n] and then by the
  * rounded alpha a_scales[m], in one step with the addition of beta C + bias[n]; scales that are NULL are 1. A, B and, with several rows, lda and ldb are multiples of 16 bytes, the
  * leading dimensions at most 2^22; a row's bytes from K to the next multiple of 16 are read and count for nothing: the last row's
- * too, so memory behind a matrix is read as far as the 16 aligned bytes reach in which its last value lies, and no farther. K is below 2^17, M and N at most 2^25. C and bias are fp32; bias may be NULL; beta == 0 never reads C; act and act_alpha
- * as gn_gemm; K == 0 gives act(beta * C + bias). Codes: -1 invalid argument, -6 launch error. */
+ * too, so memory behind a matrix is read as far as the 16 aligned bytes reach in which its last value lies, and no farther. K is
+ * below 2^17, M and N at most 2^25, and C at most 2^26 blocks of 16 x 16. C and bias are fp32; bias may be NULL; beta == 0 never reads C; act
+ * and act_alpha as gn_gemm; K == 0 gives act(beta * C + bias). Codes: -1 invalid argument, -6 launch error. */
 int gn_int8_gemm(long M, long N, long K, float alpha, const int8_t *A, long lda, const float *a_scales, const int8_t *B,
                  long ldb, const float *b_scales, float beta, float *C, long ldc, const float *bias, int act, float act_alpha,
                  void *stream, CError *err);
